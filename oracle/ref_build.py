@@ -101,7 +101,7 @@ def newer(target, *deps):
 
 
 def build(force=False):
-    if not os.path.isdir(REF):
+    if not os.path.isdir(os.path.join(REF, "src")):
         print(f"ref_build: {REF} absent; using prebuilt oracle/_ref",
               file=sys.stderr)
         return False
