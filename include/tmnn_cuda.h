@@ -82,7 +82,11 @@ typedef enum tmnn_grad_format {
   TMNN_GRAD_F16 = 2
 } tmnn_grad_format;
 
-typedef enum tmnn_dtype { TMNN_DTYPE_F32 = 0, TMNN_DTYPE_F16 = 1 } tmnn_dtype;
+/* BF16: class logits only (tables are F32 or F16). */
+typedef enum tmnn_dtype { TMNN_DTYPE_F32 = 0, TMNN_DTYPE_F16 = 1,
+                          TMNN_DTYPE_BF16 = 2 } tmnn_dtype;
+/* Integer type of class ids. */
+typedef enum tmnn_index { TMNN_INDEX_I32 = 0, TMNN_INDEX_I64 = 1 } tmnn_index;
 
 /* KernelSpec fields the hot path needs (include/tiny-metal-nn/kernels/
  * kernel_spec.h:17-58), validated with kernel_spec.cpp:12-44's limits. */
@@ -514,6 +518,106 @@ tmnn_status tmnn_cuda_mlp_forward(tmnn_mlp *mlp, const void *input_f16,
                                   float *output, uint32_t n);
 tmnn_status tmnn_cuda_mlp_stream(tmnn_mlp *mlp, void **stream);
 const char *tmnn_cuda_mlp_last_error(void);
+
+/* Operators over class logits (tmnn has none: its losses compare outputs
+ * with targets of their own shape).  A row x[0..classes) of logits at
+ * temperature T stands for the distribution p = softmax(x / T);
+ * lse = log sum exp(x / T).
+ *
+ * The calls take device pointers, queue their kernel on `stream` (a
+ * cudaStream_t of `device`; NULL is the device's default stream) and return
+ * without waiting.  They allocate nothing and keep nothing between calls, so
+ * they may be captured into graphs and run on several streams at once.
+ * Arithmetic and sums are fp32.  Results are the same from run to run.
+ *
+ * Rows: a class at -inf has probability 0.  A row with every class at -inf
+ * has no distribution: its log probabilities are -inf, its entropy and its
+ * gradient 0.  A NaN or +inf in a row makes the row's results NaN.
+ * Limits: 1 <= classes <= 524288; temperature in [1e-4, 1e4]; pointers
+ * aligned to their element.  n = 0 is a no-op. */
+typedef struct tmnn_logits {
+  const void *data;    /* [rows x classes], rows `row_stride` elements apart */
+  int64_t row_stride;  /* any value >= 0; the gradient's is >= classes */
+  uint32_t rows, classes;
+  int32_t dtype;       /* tmnn_dtype */
+  float temperature;
+} tmnn_logits;
+
+/* logprob[i] = x[tokens[i]] / T - lse and entropy[i] = -sum p log p.
+ * top_ids / top_logprobs [rows x top_k]: the classes with the largest logits,
+ * largest first, ties to the lowest class; where fewer than top_k classes are
+ * above -inf the rest is id -1 and -inf (all of it for a row with a NaN or
+ * +inf, whose top_logprobs are NaN).  top_k <= min(classes, 128), 0 for none.
+ * stats [rows x 3] = max x, sum exp((x - max) / T), entropy: what the backward
+ * call needs.  Each output may be NULL (top_ids and top_logprobs only with
+ * top_k = 0), and tokens when logprob is.  A token below 0 marks a padded
+ * row, which is not read: logprob, entropy and stats 0, no alternatives.  A
+ * token >= classes makes its logprob NaN. */
+tmnn_status tmnn_cuda_token_logprobs(int device, void *stream,
+                                     const tmnn_logits *logits,
+                                     const void *tokens, int32_t index_type,
+                                     uint32_t top_k, float *logprob,
+                                     float *entropy, int32_t *top_ids,
+                                     float *top_logprobs, float *stats);
+
+/* Gradient of sum_i d_logprob[i] logprob[i] + d_entropy[i] entropy[i] with
+ * respect to the logits, from the same logits, tokens, temperature and the
+ * stats of the forward call:
+ *   d_x = (d_logprob (delta_token - p) - d_entropy p (log p + entropy)) / T.
+ * d_logprob and tokens, or d_entropy, may be NULL.  d_logits has the logits'
+ * type, rows d_row_stride >= classes apart; it may be the logits' own memory
+ * (same address and stride) but not overlap them otherwise.  Every row's
+ * `classes` elements are written, columns behind them are left alone.  A
+ * padded row's gradient is 0, and that of a row whose token is >= classes is
+ * NaN. */
+tmnn_status tmnn_cuda_token_logprobs_backward(
+    int device, void *stream, const tmnn_logits *logits, const void *tokens,
+    int32_t index_type, const float *stats, const float *d_logprob,
+    const float *d_entropy, void *d_logits, int64_t d_row_stride);
+
+/* Distillation from a teacher's top logits.  Row i has k entries:
+ * teacher_ids [rows x k] and teacher_logits [rows x k] (teacher_dtype; log
+ * probabilities serve as well, a constant per row has no effect).
+ *   q = softmax(teacher_logits[i] / T) over the row's entries,
+ *   loss[i] = T^2 sum_k q_k (log q_k - log p[id_k]),
+ *   d_logits[i] = w_i d loss[i] / d x = w_i T (p - q),
+ * w_i = row_weight[i], or 1 / rows when row_weight is NULL (the gradient of
+ * the mean loss).  Entries with id < 0 or logit -inf are left out, and a row
+ * without entries is padding: it is not read, its loss and gradient are 0.
+ * Entries that name one class twice count each on its own.  An id >= classes
+ * or a NaN or +inf among the entries makes the row NaN.  d_logits NULL: the
+ * loss only (row_weight is not read); otherwise as in
+ * tmnn_cuda_token_logprobs_backward.  1 <= k <= 128. */
+tmnn_status tmnn_cuda_distill(int device, void *stream,
+                              const tmnn_logits *logits,
+                              const void *teacher_ids, int32_t index_type,
+                              const void *teacher_logits,
+                              int32_t teacher_dtype, uint32_t k,
+                              const float *row_weight, float *loss,
+                              void *d_logits, int64_t d_row_stride);
+const char *tmnn_cuda_logits_last_error(void);
+
+/* The same on a context whose outputs are class logits (classes =
+ * num_outputs).  Host arrays, or device pointers with TMNN_PTR_DEVICE, like
+ * the context's other calls; they run on the context's stream and wait.
+ * token_logprobs: evaluate, then tmnn_cuda_token_logprobs.  Any output may be
+ * NULL as above. */
+tmnn_status tmnn_cuda_ctx_token_logprobs(
+    tmnn_ctx *ctx, const float *positions, const void *tokens,
+    int32_t index_type, uint32_t n, uint32_t top_k, float temperature,
+    uint32_t flags, float *logprob, float *entropy, int32_t *top_ids,
+    float *top_logprobs);
+/* One training step of the distillation loss, averaged over the n points
+ * (over all ranks' points under data parallelism, equal n on every rank):
+ * forward, loss with its gradient, backward, Adam with gradient reset.  *loss
+ * = the mean loss.  Like tmnn_cuda_adam_step it runs without the numerics
+ * guard.  teacher_logits are float32. */
+tmnn_status tmnn_cuda_distill_step(tmnn_ctx *ctx, const float *positions,
+                                   const void *teacher_ids,
+                                   int32_t index_type,
+                                   const float *teacher_logits, uint32_t n,
+                                   uint32_t k, float temperature,
+                                   uint32_t flags, float *loss);
 
 /* Message of the last failure on this thread ("" if none). */
 const char *tmnn_cuda_last_error(void);

@@ -24,6 +24,7 @@
 #include "../../include/tmnn_cuda.h"
 #include "fused.h"
 #include "kernels.h"
+#include "logits.h"
 #include "tiled.h"
 #include "runtime.h"
 
@@ -160,6 +161,11 @@ struct tmnn_ctx {
   DevBuf<uint8_t> sort_tmp;
   DevBuf<__half> feat;   // Tiled family: encoded features [N x In]
   DevBuf<float> dfeat;   // Tiled family: dL/d(features) [N x In]
+  // class-logit calls: ids and float rows (teacher entries, results) of a
+  // batch, and the summed loss
+  DevBuf<uint8_t> cls_ids;
+  DevBuf<float> cls_rows;
+  DevBuf<double> cls_sum;
   StepStats *h_stats = nullptr;  // pinned copy of the step statistics
   double *h_loss = nullptr;      // &h_stats->loss
   // numerics guard
@@ -1699,6 +1705,130 @@ void backward_accumulate(tmnn_ctx &c, const float *pos, const float *dout,
   CK(cudaGetLastError());
 }
 
+// Ids of `count` entries in `staging`, or the caller's device pointer.
+const void *stage_ids(tmnn_ctx &c, const void *src, int type, size_t count,
+                      uint32_t flags) {
+  if (!src || (flags & TMNN_PTR_DEVICE)) return src;
+  const size_t bytes = count * (type == TMNN_INDEX_I64 ? 8 : 4);
+  c.cls_ids.ensure(bytes);
+  if (bytes)
+    CK(cudaMemcpyAsync(c.cls_ids.p, src, bytes, cudaMemcpyHostToDevice,
+                       c.stream));
+  return c.cls_ids.p;
+}
+
+tmnn_logits output_logits(const tmnn_ctx &c, const float *out, uint32_t N,
+                          float temperature) {
+  return {out, c.nd.O, N, (uint32_t)c.nd.O, TMNN_DTYPE_F32, temperature};
+}
+
+void ctx_token_logprobs(tmnn_ctx &c, const float *pos, const void *tokens,
+                        int index_type, uint32_t N, uint32_t top_k,
+                        float temperature, uint32_t flags, LogprobOut o) {
+  if (N > 0 && !pos)
+    throw std::invalid_argument("token_logprobs: null positions");
+  // the arguments' checks, before anything is queued
+  launch_token_logprobs(output_logits(c, nullptr, 0, temperature), tokens,
+                        index_type, top_k, o, c.stream);
+  if (top_k && (!o.top_ids || !o.top_logprobs))
+    throw std::invalid_argument("token_logprobs: null top_ids or top_logprobs");
+  if (o.logprob && !tokens)
+    throw std::invalid_argument("token_logprobs: logprob needs tokens");
+  if (N == 0) return;
+  CK(cudaSetDevice(c.device));
+  ensure_batch(c, N);
+  const float *p = stage_in(c, pos, (size_t)N * c.nd.d, c.pos_in, flags);
+  forward_dev(c, p, c.out_buf.p, N);
+  const void *ids = stage_ids(c, tokens, index_type, N, flags);
+  const bool dev = flags & TMNN_PTR_DEVICE;
+  LogprobOut d = o;
+  if (!dev) {
+    // [logprob | entropy | top_logprobs | top_ids] of the batch
+    c.cls_rows.ensure((size_t)N * (2 + 2 * (size_t)top_k));
+    float *r = c.cls_rows.p;
+    if (d.logprob) d.logprob = r;
+    if (d.entropy) d.entropy = r + N;
+    if (top_k) {
+      d.top_logprobs = r + 2 * (size_t)N;
+      d.top_ids = reinterpret_cast<int32_t *>(d.top_logprobs + (size_t)N * top_k);
+    }
+  }
+  c.launches += launch_token_logprobs(
+      output_logits(c, c.out_buf.p, N, temperature), ids, index_type, top_k, d,
+      c.stream);
+  if (!dev) {
+    if (o.logprob) copy_out(c, o.logprob, d.logprob, N, flags);
+    if (o.entropy) copy_out(c, o.entropy, d.entropy, N, flags);
+    if (top_k) {
+      copy_out(c, o.top_logprobs, d.top_logprobs, (size_t)N * top_k, flags);
+      copy_out(c, reinterpret_cast<float *>(o.top_ids),
+               reinterpret_cast<float *>(d.top_ids), (size_t)N * top_k, flags);
+    }
+  }
+  CK(cudaStreamSynchronize(c.stream));
+  CK(cudaGetLastError());
+}
+
+// One step of the distillation loss: forward, loss and its gradient, backward
+// of that gradient, Adam -- the split API (forward_for_training ->
+// backward_accumulate -> adam_step) on one stream with one wait at the end.
+void distill_step(tmnn_ctx &c, const float *pos, const void *ids,
+                  int index_type, const float *teacher, uint32_t N, uint32_t k,
+                  float temperature, uint32_t flags, float *loss) {
+  if (N > 0 && (!pos || !ids || !teacher))
+    throw std::invalid_argument("distill_step: null arguments");
+  if (c.n_pending)
+    throw std::invalid_argument(
+        "distill_step: enqueued steps are pending; finalize them first");
+  launch_distill(output_logits(c, nullptr, 0, temperature), ids, index_type,
+                 teacher, TMNN_DTYPE_F32, k, nullptr, 0.0f, nullptr, nullptr, 0,
+                 c.stream);
+  const uint64_t global_n = (uint64_t)N * (uint64_t)c.world;
+  if (loss) *loss = 0.0f;
+  if (N == 0) return;
+  CK(cudaSetDevice(c.device));
+  ensure_batch(c, N);
+  const float *p = stage_in(c, pos, (size_t)N * c.nd.d, c.pos_in, flags);
+  const void *id = stage_ids(c, ids, index_type, (size_t)N * k, flags);
+  const bool dev = flags & TMNN_PTR_DEVICE;
+  c.cls_rows.ensure((size_t)N * (1 + (dev ? 0 : (size_t)k)));
+  c.cls_sum.ensure(1);
+  float *row_loss = c.cls_rows.p;
+  const float *t = teacher;
+  if (!dev) {
+    float *staged = row_loss + N;
+    CK(cudaMemcpyAsync(staged, teacher, (size_t)N * k * sizeof(float),
+                       cudaMemcpyHostToDevice, c.stream));
+    t = staged;
+  }
+  forward_dev(c, p, c.out_buf.p, N);
+  // the gradient takes the place of the logits
+  c.launches += launch_distill(output_logits(c, c.out_buf.p, N, temperature),
+                               id, index_type, t, TMNN_DTYPE_F32, k, nullptr,
+                               1.0f / (float)global_n, row_loss, c.out_buf.p,
+                               c.nd.O, c.stream);
+  launch_row_sum(row_loss, N, c.cls_sum.p, c.stream);
+  c.launches++;
+  const float *g = c.out_buf.p;
+  if (c.cfg.morton_sort && N > 1) morton_sort(c, p, g, N, &p, &g);
+  fwd_bwd(c, p, nullptr, g, N, 0.0f);
+  if (c.comm && c.world > 1)
+    NK(ncclAllReduce(c.cls_sum.p, c.cls_sum.p, 1, ncclFloat64, ncclSum, c.comm,
+                     c.stream));
+  if (can_shard(c)) {
+    dp_update(c, false, nullptr);
+  } else {
+    allreduce_grads(c, false);
+    adam(c);
+  }
+  double sum = 0.0;
+  CK(cudaMemcpyAsync(&sum, c.cls_sum.p, sizeof sum, cudaMemcpyDeviceToHost,
+                     c.stream));
+  CK(cudaStreamSynchronize(c.stream));
+  CK(cudaGetLastError());
+  if (loss) *loss = (float)(sum / (double)global_n);
+}
+
 }  // namespace
 
 // ====================================================================== ABI
@@ -2084,6 +2214,33 @@ tmnn_status tmnn_cuda_adam_step(tmnn_ctx *c) {
     }
     CK(cudaStreamSynchronize(c->stream));
     CK(cudaGetLastError());
+  });
+}
+
+tmnn_status tmnn_cuda_ctx_token_logprobs(
+    tmnn_ctx *c, const float *positions, const void *tokens,
+    int32_t index_type, uint32_t n, uint32_t top_k, float temperature,
+    uint32_t flags, float *logprob, float *entropy, int32_t *top_ids,
+    float *top_logprobs) {
+  REQUIRE_CTX(c);
+  return guarded([&] {
+    BusyGuard g(c);
+    ctx_token_logprobs(*c, positions, tokens, index_type, n, top_k, temperature,
+                       flags,
+                       {logprob, entropy, top_ids, top_logprobs, nullptr});
+  });
+}
+
+tmnn_status tmnn_cuda_distill_step(tmnn_ctx *c, const float *positions,
+                                   const void *teacher_ids, int32_t index_type,
+                                   const float *teacher_logits, uint32_t n,
+                                   uint32_t k, float temperature,
+                                   uint32_t flags, float *loss) {
+  REQUIRE_CTX(c);
+  return guarded([&] {
+    BusyGuard g(c);
+    distill_step(*c, positions, teacher_ids, index_type, teacher_logits, n, k,
+                 temperature, flags, loss);
   });
 }
 

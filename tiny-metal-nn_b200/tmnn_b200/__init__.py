@@ -24,11 +24,14 @@ import numpy as np
 
 from . import _abi
 from ._abi import lib
+from .logits import (TokenLogprobs, distill_forward_backward, distill_loss,
+                     token_logprobs, token_logprobs_backward)
 
 __version__ = "0.1.0"
 __all__ = ["Trainer", "ClosedError", "ConcurrentTrainingStepError",
            "ConfigError", "DTypeError", "TmnnError", "dp_unique_id", "NerfField",
-           "__version__"]
+           "TokenLogprobs", "token_logprobs", "token_logprobs_backward",
+           "distill_loss", "distill_forward_backward", "__version__"]
 
 
 class TmnnError(RuntimeError):
@@ -545,6 +548,93 @@ class Trainer:
         return out, gradients
 
     inference_with_gradient = evaluate_with_gradient
+
+    # ------------------------------------------------- class-logit outputs
+    def _class_ids(self, ids, name, shape, flags):
+        """(pointer, index type, keepalive) of class ids placed like input."""
+        if ids is None:
+            return None, 0, None
+        if _is_cuda_tensor(ids) != bool(flags & _abi.PTR_DEVICE):
+            raise ValueError(f"input and {name} must both be host or both CUDA")
+        if flags & _abi.PTR_DEVICE:
+            contiguous, ptr = ids.is_contiguous(), C.c_void_p(ids.data_ptr())
+        else:
+            ids = np.asarray(ids)
+            contiguous = ids.flags["C_CONTIGUOUS"]
+            ptr = ids.ctypes.data_as(C.c_void_p)
+        kind = {"int32": _abi.INDEX_I32, "int64": _abi.INDEX_I64}.get(
+            str(ids.dtype).removeprefix("torch."))
+        if kind is None:
+            raise DTypeError(f"{name} must be int32 or int64, got {ids.dtype}")
+        if tuple(ids.shape) != shape:
+            raise ValueError(f"{name} must have shape {shape}")
+        if not contiguous:
+            raise ValueError(f"{name} must be contiguous")
+        return ptr, kind, ids
+
+    def _after_current_stream(self, input):
+        """Orders this trainer's stream behind the work already queued on the
+        current stream of a CUDA input's device."""
+        import torch
+        mine = torch.cuda.ExternalStream(self.stream(), device=input.device)
+        mine.wait_stream(torch.cuda.current_stream(input.device))
+
+    def token_logprobs(self, input, tokens=None, *, top_k=0, temperature=1.0):
+        """inference() read as class logits: a TokenLogprobs of each point
+        (classes = n_output; see tmnn_b200.token_logprobs; no stats).  Host
+        arrays or CUDA tensors, like inference()."""
+        h = self._handle()
+        pp, n, flags, _k = _arg(input, "input", self.n_input)
+        ip, it, _k2 = self._class_ids(tokens, "tokens", (n,), flags)
+        k = int(top_k)
+        if not 0 <= k <= min(self.n_output, _abi.MAX_TOP):
+            raise ValueError("top_k must be in [0, min(n_output, 128)]")
+        if flags & _abi.PTR_DEVICE:
+            import torch
+            def new(shape, t):
+                return torch.empty(shape, dtype=getattr(torch, t),
+                                   device=input.device)
+            def ptr(a):
+                return None if a is None else C.c_void_p(a.data_ptr())
+            self._after_current_stream(input)
+        else:
+            def new(shape, t):
+                return np.empty(shape, t)
+            def ptr(a):
+                return None if a is None else a.ctypes.data_as(C.c_void_p)
+        lp = None if tokens is None else new((n,), "float32")
+        ent = new((n,), "float32")
+        ids = new((n, k), "int32") if k else None
+        top = new((n, k), "float32") if k else None
+        self._guarded(lambda: _check(lib.tmnn_cuda_ctx_token_logprobs(
+            h, pp, ip, it, n, k, temperature, flags, ptr(lp), ptr(ent),
+            ptr(ids), ptr(top)), "token_logprobs"))
+        return TokenLogprobs(lp, ent, ids, top, None)
+
+    def distill_step(self, input, teacher_ids, teacher_logits, *,
+                     temperature=1.0):
+        """One training step of the distillation loss over class logits
+        (classes = n_output): forward, loss with its gradient, backward, Adam;
+        returns the mean loss.  teacher_ids [batch, k] (int32 or int64, below
+        0: no entry) and float32 teacher_logits [batch, k] are a teacher's top
+        classes of each point, e.g. what token_logprobs(top_k=k) returns.
+        Host arrays or CUDA tensors, all alike."""
+        h = self._handle()
+        pp, n, flags, _k = _arg(input, "input", self.n_input)
+        if len(teacher_ids.shape) != 2:
+            raise ValueError("teacher_ids must be 2D (batch_size, k)")
+        k = int(teacher_ids.shape[1])
+        ip, it, _k2 = self._class_ids(teacher_ids, "teacher_ids", (n, k), flags)
+        yp, ny, fy, _k3 = _arg(teacher_logits, "teacher_logits", k)
+        if ny != n or fy != flags:
+            raise ValueError("input and teacher_logits must match")
+        if flags & _abi.PTR_DEVICE:
+            self._after_current_stream(input)
+        loss = C.c_float()
+        self._guarded(lambda: _check(lib.tmnn_cuda_distill_step(
+            h, pp, ip, it, yp, n, k, temperature, flags, C.byref(loss)),
+            "distill_step"))
+        return loss.value
 
     def debug_morton_order(self, input, key_bits=0):
         """Device Morton permutation of a host batch (parity instrument)."""

@@ -24,7 +24,9 @@ BUF_FUSED_WEIGHTS, BUF_FUSED_M, BUF_FUSED_V = 7, 8, 9
 BUF_HASH_GATHER, BUF_TOUCHED = 20, 21
 LOSS = {"L2": 0, "L1": 1, "Huber": 2, "Cosine": 3}
 GRAD_FIXED16, GRAD_F32, GRAD_F16 = 0, 1, 2
-DTYPE_F32, DTYPE_F16 = 0, 1
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
+INDEX_I32, INDEX_I64 = 0, 1
+MAX_TOP = 128
 
 
 class Spec(C.Structure):
@@ -102,6 +104,12 @@ class ProbeResult(C.Structure):
                 ("output_min", C.c_float)]
 
 
+class Logits(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("row_stride", C.c_int64),
+                ("rows", C.c_uint32), ("classes", C.c_uint32),
+                ("dtype", C.c_int32), ("temperature", C.c_float)]
+
+
 class BufferView(C.Structure):
     _fields_ = [("device_ptr", C.c_void_p), ("bytes", C.c_size_t),
                 ("dtype", C.c_int32)]
@@ -176,6 +184,18 @@ _SIGS = [
     ("tmnn_cuda_nerf_inference", C.c_int, [P, P, P, P, P, u32, u32]),
     ("tmnn_cuda_nerf_profile", C.c_int, [P, P, C.POINTER(C.c_uint64)]),
     ("tmnn_cuda_nerf_last_error", C.c_char_p, []),
+    ("tmnn_cuda_token_logprobs", C.c_int,
+     [C.c_int, P, C.POINTER(Logits), P, C.c_int32, u32, P, P, P, P, P]),
+    ("tmnn_cuda_token_logprobs_backward", C.c_int,
+     [C.c_int, P, C.POINTER(Logits), P, C.c_int32, P, P, P, P, C.c_int64]),
+    ("tmnn_cuda_distill", C.c_int,
+     [C.c_int, P, C.POINTER(Logits), P, C.c_int32, P, C.c_int32, u32, P, P, P,
+      C.c_int64]),
+    ("tmnn_cuda_logits_last_error", C.c_char_p, []),
+    ("tmnn_cuda_ctx_token_logprobs", C.c_int,
+     [P, P, P, C.c_int32, u32, u32, C.c_float, u32, P, P, P, P]),
+    ("tmnn_cuda_distill_step", C.c_int,
+     [P, P, P, C.c_int32, P, u32, u32, C.c_float, u32, C.POINTER(C.c_float)]),
     ("tmnn_cuda_last_error", C.c_char_p, []),
     ("tmnn_cuda_launch_count", C.c_int, [P, C.POINTER(C.c_uint64)]),
 ]
