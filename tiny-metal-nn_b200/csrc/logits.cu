@@ -11,9 +11,11 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
 #include <cmath>
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 
 #include "logits.h"
 
@@ -97,143 +99,180 @@ __device__ __forceinline__ float load_value(const void *p, int64_t i,
   return to_f(static_cast<const __nv_bfloat16 *>(p)[i]);
 }
 
-// ------------------------------------------------------------ one CTA a row
-constexpr int kThreads = 256;
+// ------------------------------------------------------------ 16-byte granules
+// Rows are read in granules of 16 bytes that lie on 16-byte boundaries; the
+// first and the last one of a row may hold elements that are not the row's,
+// which count as -inf.
+template <class T>
+constexpr int kElems = 16 / (int)sizeof(T);
 
-struct OpAdd {
-  __device__ static float f(float a, float b) { return a + b; }
-};
-struct OpMax {
-  __device__ static float f(float a, float b) { return max_nan(a, b); }
-};
-template <class Op>
-__device__ float block_reduce(float v, float *buf) {
-  for (int o = 16; o; o >>= 1) v = Op::f(v, __shfl_xor_sync(~0u, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = buf[0];
-  for (int w = 1; w < kThreads / 32; ++w) v = Op::f(v, buf[w]);
-  return v;
+__device__ __forceinline__ uint64_t f2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
 }
-__device__ uint64_t block_max_key(uint64_t v, uint64_t *buf) {
+__device__ __forceinline__ void f2_split(uint64_t v, float &a, float &b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t word(const uint4 &g, int i) {
+  return i == 0 ? g.x : i == 1 ? g.y : i == 2 ? g.z : g.w;
+}
+// the i-th pair of a granule's values
+template <class T>
+__device__ __forceinline__ uint64_t pair_of(const uint4 &g, int i);
+template <>
+__device__ __forceinline__ uint64_t pair_of<float>(const uint4 &g, int i) {
+  return f2(__uint_as_float(word(g, 2 * i)), __uint_as_float(word(g, 2 * i + 1)));
+}
+template <>
+__device__ __forceinline__ uint64_t pair_of<__half>(const uint4 &g, int i) {
+  const uint32_t w = word(g, i);
+  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+  return f2(f.x, f.y);
+}
+template <>
+__device__ __forceinline__ uint64_t pair_of<__nv_bfloat16>(const uint4 &g,
+                                                           int i) {
+  const uint32_t w = word(g, i);
+  return f2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+// two values rounded to T: one word of 16-bit values, two of fp32
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Running maximum (NaN wins) of granules, in T (a maximum is exact).
+template <class T>
+struct GranuleMax {
+  uint32_t m[4];
+  __device__ __forceinline__ static uint32_t two(uint32_t a, uint32_t b) {
+    if constexpr (sizeof(T) == 4)
+      return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b)));
+    uint32_t r;
+    if constexpr (std::is_same<T, __half>::value)
+      asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else
+      asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  __device__ __forceinline__ void clear() {
+    const uint32_t w = sizeof(T) == 4                      ? 0xFF800000u
+                       : std::is_same<T, __half>::value ? 0xFC00FC00u
+                                                           : 0xFF80FF80u;
+    m[0] = m[1] = m[2] = m[3] = w;
+  }
+  __device__ __forceinline__ void add(const uint4 &g) {
+    m[0] = two(m[0], g.x);
+    m[1] = two(m[1], g.y);
+    m[2] = two(m[2], g.z);
+    m[3] = two(m[3], g.w);
+  }
+  __device__ __forceinline__ float get() const {
+    const uint4 g{two(two(m[0], m[1]), two(m[2], m[3])), 0, 0, 0};
+    if constexpr (sizeof(T) == 4) return __uint_as_float(g.x);
+    float a, b;
+    f2_split(pair_of<T>(g, 0), a, b);
+    return max_nan(a, b);
+  }
+};
+
+// s += sum e^t and, if U, u += sum e^t t log2(e) over a granule, in two lanes;
+// nm = -max and c = log2(e) / T twice
+template <class T, bool U>
+__device__ __forceinline__ void accumulate(const uint4 &g, uint64_t nm,
+                                           uint64_t c, uint64_t &s,
+                                           uint64_t &u) {
+#pragma unroll
+  for (int i = 0; i < kElems<T> / 2; ++i) {
+    const uint64_t t = f2_mul(f2_add(pair_of<T>(g, i), nm), c);
+    float a, b;
+    f2_split(t, a, b);
+    const uint64_t e = f2(ex2(a), ex2(b));
+    s = f2_add(s, e);
+    // where t is -inf e is 0: a finite t keeps 0 * t from being NaN
+    if (U) u = f2_fma(e, f2(fmaxf(a, -1e4f), fmaxf(b, -1e4f)), u);
+  }
+}
+
+// Softmax statistics of a part of a row: the maximum m, s = sum e^{t} and
+// u = sum e^{t} t log2(e), t = (x - m) / T.
+struct Stat {
+  float m, s, u;
+};
+// brings v to the maximum m
+__device__ __forceinline__ void rescale(Stat &v, float m, float c) {
+  const float d = (v.m - (m == -kInf ? 0.0f : m)) * c;
+  const float f = ex2(d);
+  v.s *= f;
+  v.u = v.u * f + v.s * fmaxf(d, -1e4f);
+  v.m = m;
+}
+__device__ __forceinline__ Stat warp_combine(Stat v, float c) {
+  float m = v.m;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(~0u, m, o));
+  rescale(v, m, c);
+#pragma unroll
   for (int o = 16; o; o >>= 1) {
-    const uint64_t u = __shfl_xor_sync(~0u, v, o);
-    v = u > v ? u : v;
+    v.s += __shfl_xor_sync(~0u, v.s, o);
+    v.u += __shfl_xor_sync(~0u, v.u, o);
   }
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = buf[0];
-  for (int w = 1; w < kThreads / 32; ++w) v = buf[w] > v ? buf[w] : v;
   return v;
 }
 
-template <class T>
-__global__ void __launch_bounds__(kThreads)
-    k_logprobs(RowArgs a, const void *tokens, int itype, int top_k,
-               LogprobOut o) {
-  __shared__ float buf[kThreads / 32];
-  __shared__ uint64_t kbuf[kThreads / 32];
-  const int tid = threadIdx.x;
-  for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const T *x = static_cast<const T *>(a.x) + (int64_t)row * a.stride;
-    const int64_t tok = tokens ? load_index(tokens, row, itype) : 0;
-    int32_t *tid_out = top_k ? o.top_ids + (int64_t)row * top_k : nullptr;
-    float *tlp = top_k ? o.top_logprobs + (int64_t)row * top_k : nullptr;
-    if (tok < 0) {
-      if (tid == 0) {
-        if (o.logprob) o.logprob[row] = 0.0f;
-        if (o.entropy) o.entropy[row] = 0.0f;
-        if (o.stats)
-          for (int i = 0; i < 3; ++i) o.stats[(int64_t)row * 3 + i] = 0.0f;
-      }
-      for (int k = tid; k < top_k; k += kThreads) {
-        tid_out[k] = -1;
-        tlp[k] = -kInf;
-      }
-      continue;
-    }
-    float m = -kInf;
-    for (int v = tid; v < a.classes; v += kThreads) m = max_nan(m, to_f(x[v]));
-    m = block_reduce<OpMax>(m, buf);
-    const bool bad = !(m < kInf);  // NaN or +inf
-    const bool empty = m == -kInf;
-    float s = 0.0f, u = 0.0f;
-    if (!bad && !empty)
-      for (int v = tid; v < a.classes; v += kThreads) {
-        const float t = (to_f(x[v]) - m) * a.c;
-        const float e = ex2(t);
-        s += e;
-        u += e * fmaxf(t, -1e4f);  // e is 0 there: no 0 * inf
-      }
-    s = block_reduce<OpAdd>(s, buf);
-    u = block_reduce<OpAdd>(u, buf);
-    const float ln_s = logf(s);
-    const float nan = __int_as_float(0x7FFFFFFF);
-    if (tid == 0) {
-      const float h = bad ? nan : empty ? 0.0f : ln_s - kLn2 * u / s;
-      if (o.entropy) o.entropy[row] = h;
-      if (o.logprob) {
-        float lp = nan;
-        if (!bad && tok < a.classes)
-          lp = empty ? -kInf : (to_f(x[tok]) - m) * a.inv_t - ln_s;
-        o.logprob[row] = lp;
-      }
-      if (o.stats) {
-        float *st = o.stats + (int64_t)row * 3;
-        st[0] = bad ? nan : m;
-        st[1] = bad ? nan : s;
-        st[2] = h;
-      }
-    }
-    uint64_t last = ~0ull;
-    for (int k = 0; k < top_k; ++k) {
-      uint64_t best = 0;
-      if (!bad && last)
-        for (int v = tid; v < a.classes; v += kThreads) {
-          const uint64_t key = key_of(to_f(x[v]), v);
-          if (key < last && key > best) best = key;
-        }
-      last = block_max_key(best, kbuf);
-      if (tid == 0) {
-        tid_out[k] = last ? class_of(last) : -1;
-        tlp[k] = bad    ? nan
-                 : last ? (value_of(last >> 32) - m) * a.inv_t - ln_s
-                        : -kInf;
-      }
-    }
-  }
+__device__ __forceinline__ uint32_t smem_addr(const void *p) {
+  return (uint32_t)__cvta_generic_to_shared(p);
 }
-
-template <class T>
-__global__ void __launch_bounds__(kThreads)
-    k_logprobs_backward(RowArgs a, const void *tokens, int itype,
-                        const float *stats, const float *d_logprob,
-                        const float *d_entropy, T *dx, int64_t d_stride) {
-  for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const T *x = static_cast<const T *>(a.x) + (int64_t)row * a.stride;
-    T *d = dx + (int64_t)row * d_stride;
-    const int64_t tok = tokens ? load_index(tokens, row, itype) : -1;
-    const float m = stats[(int64_t)row * 3], s = stats[(int64_t)row * 3 + 1],
-                h = stats[(int64_t)row * 3 + 2];
-    float g = d_logprob ? d_logprob[row] * a.inv_t : 0.0f;
-    const float b = d_entropy ? d_entropy[row] * a.inv_t : 0.0f;
-    if (tokens && tok >= a.classes) g = __int_as_float(0x7FFFFFFF);
-    const bool idle = s == 0.0f || (tokens && tok < 0);
-    const float ln_s = logf(s), inv_s = 1.0f / s;
-    for (int v = threadIdx.x; v < a.classes; v += kThreads) {
-      float r = 0.0f;
-      if (!idle) {
-        const float t = (to_f(x[v]) - m) * a.c;
-        const float p = ex2(t) * inv_s;
-        const float lp = fmaxf(t, -1e4f) * kLn2 - ln_s;
-        r = -p * (g + b * (lp + h));
-        if (v == tok) r += g;
-      }
-      d[v] = from_f<T>(r);
-    }
-  }
+__device__ __forceinline__ void copy16(void *smem, const void *global) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(smem)),
+               "l"(global)
+               : "memory");
+}
+__device__ __forceinline__ void copies_done() {
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// the address of `p` in the shared memory of another CTA of the cluster
+__device__ __forceinline__ uint32_t peer_addr(const void *p, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void peer_store(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+__device__ __forceinline__ void peer_store(uint32_t addr, uint64_t v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
 }
 
 struct Teacher {
@@ -241,83 +280,573 @@ struct Teacher {
   int itype, dtype, k;
 };
 
-template <class T>
-__global__ void __launch_bounds__(kThreads)
-    k_distill(RowArgs a, Teacher te, const float *row_weight, float weight,
-              float *loss, T *dx, int64_t d_stride) {
-  __shared__ float buf[kThreads / 32];
-  __shared__ float sq[kMaxTop];
-  __shared__ int32_t sid[kMaxTop];
-  const int tid = threadIdx.x;
+// ------------------------------------------------------------ a team a row
+// A team -- a warp, a CTA, or a cluster of CTAs each holding a part ("slab")
+// of the row in its shared memory -- reads a row once.  Every thread copies
+// its own granules (cp.async) and works on the same ones in each pass, so the
+// passes need no barrier between them: maximum, sums relative to the thread's
+// maximum, one exchange of (m, s, u) over the team, and then the alternatives
+// or the gradient from the slab.  Memory traffic is that of the operator
+// itself: the row once in, results or gradient once out.
+enum Mode { kRead = 0, kReadTop = 1, kLoss = 2, kLossGrad = 3 };
+
+constexpr int kMaxCluster = 16;
+constexpr uint32_t kLowestOrder = 0x00800000u;  // order of the lowest finite
+
+// Shared memory of a team, in bytes from its base: the slab, the exchange of
+// statistics, and what the mode needs.
+struct TeamLayout {
+  int stats, teacher, gmax, cand, merge, misc, total;
+  int cap;  // candidates for the alternatives
+};
+__host__ __device__ inline TeamLayout team_layout(int mode, int threads,
+                                                  int cluster, int k,
+                                                  int granules) {
+  TeamLayout l{};
+  int off = granules * 16;
+  l.stats = off;
+  off += cluster * (threads / 32) * 16;
+  l.teacher = off;
+  if (mode >= kLoss) off += (k * 8 + 15) / 16 * 16;
+  l.misc = off;
+  if (mode == kReadTop) {
+    off += 16;
+    l.gmax = off;
+    off += threads * 4;
+    l.cap = 4 * k > 256 ? 4 * k : 256;
+    l.cand = off;
+    off += l.cap * 8;
+    l.merge = off;
+    if (cluster > 1) off += cluster * k * 8;
+  }
+  l.total = (off + 15) / 16 * 16;
+  return l;
+}
+
+struct TeamArgs {
+  RowArgs a;
+  const void *tokens;
+  int itype, top_k;
+  LogprobOut o;
+  Teacher te;
+  const float *row_weight;
+  float weight;
+  float *loss;
+  void *dx;
+  int64_t d_stride;
+  int cluster;  // CTAs a row
+  int slab;     // elements a CTA, a multiple of the granule
+  TeamLayout l;
+};
+
+template <class T, int NT, int MODE>
+__global__ void __launch_bounds__(NT == 32 ? 128 : NT) k_team(TeamArgs p) {
+  extern __shared__ __align__(16) unsigned char smem_all[];
+  constexpr int E = kElems<T>;
+  constexpr bool kWarp = NT == 32;
+  constexpr int kTeams = kWarp ? 4 : 1;
+  constexpr int kWarps = NT / 32;
+  const RowArgs &a = p.a;
+  const int tid = kWarp ? threadIdx.x & 31 : threadIdx.x;
+  const int lane = threadIdx.x & 31, warp = kWarp ? 0 : threadIdx.x >> 5;
+  const int team = kWarp ? threadIdx.x >> 5 : 0;
+  const uint32_t C = kWarp ? 1 : p.cluster;
+  const uint32_t rank = kWarp ? 0 : blockIdx.x % C;
+  const uint32_t row = blockIdx.x / C * kTeams + team;
+  if (row >= a.rows) return;  // whole warps; CTA teams cover the rows exactly
+  unsigned char *smem = smem_all + team * p.l.total;
+  const bool leader = rank == 0;
   const float nan = __int_as_float(0x7FFFFFFF);
-  for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const T *x = static_cast<const T *>(a.x) + (int64_t)row * a.stride;
-    T *d = dx ? dx + (int64_t)row * d_stride : nullptr;
-    // the teacher's entry of this thread: id -1 when left out
-    float y = -kInf;
-    int32_t id = -1;
-    if (tid < te.k) {
-      const int64_t i = (int64_t)row * te.k + tid;
-      const int64_t q = load_index(te.ids, i, te.itype);
-      y = load_value(te.logits, i, te.dtype);
-      if (q >= 0 && y != -kInf) {
-        id = (int32_t)q;
-        if (q >= a.classes) y = nan, id = 0;
-      } else {
-        y = -kInf;
+  auto team_sync = [&] {
+    if constexpr (kWarp)
+      __syncwarp();
+    else
+      __syncthreads();
+  };
+
+  // ---- is the row padding?
+  int64_t tok = 0;
+  float *sq = reinterpret_cast<float *>(smem + p.l.teacher);
+  int32_t *sid = reinterpret_cast<int32_t *>(sq + p.te.k);
+  [[maybe_unused]] float ty[4], tq[4], ln_ys = 0.0f, ym = 0.0f;
+  [[maybe_unused]] int32_t tid_[4];
+  bool idle;
+  if constexpr (MODE == kRead || MODE == kReadTop) {
+    if (p.tokens) tok = load_index(p.tokens, row, p.itype);
+    idle = tok < 0;
+    if (idle && leader) {
+      if (tid == 0) {
+        if (p.o.logprob) p.o.logprob[row] = 0.0f;
+        if (p.o.entropy) p.o.entropy[row] = 0.0f;
+        if (p.o.stats)
+          for (int i = 0; i < 3; ++i) p.o.stats[(int64_t)row * 3 + i] = 0.0f;
+      }
+      if constexpr (MODE == kReadTop)
+        for (int k = tid; k < p.top_k; k += NT) {
+          p.o.top_ids[(int64_t)row * p.top_k + k] = -1;
+          p.o.top_logprobs[(int64_t)row * p.top_k + k] = -kInf;
+        }
+    }
+  } else {
+    // Every warp reads the entries, entry lane + 32 i in register i.
+    ym = -kInf;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      ty[i] = -kInf;
+      tid_[i] = -1;
+      const int k = lane + 32 * i;
+      if (k >= p.te.k) continue;
+      const int64_t at = (int64_t)row * p.te.k + k;
+      const int64_t id = load_index(p.te.ids, at, p.te.itype);
+      const float y = load_value(p.te.logits, at, p.te.dtype);
+      if (id < 0 || y == -kInf) continue;  // left out
+      tid_[i] = id < a.classes ? (int32_t)id : 0;
+      ty[i] = id < a.classes ? y : nan;
+      ym = max_nan(ym, ty[i]);
+    }
+    for (int o = 16; o; o >>= 1) ym = max_nan(ym, __shfl_xor_sync(~0u, ym, o));
+    idle = ym == -kInf;
+    if (idle && leader && tid == 0) p.loss[row] = 0.0f;
+  }
+  const int first = (int)rank * p.slab;
+  const int n = min(p.slab, a.classes - first);  // may be below 1
+  T *d = MODE == kLossGrad
+             ? static_cast<T *>(p.dx) + (int64_t)row * p.d_stride + first
+             : nullptr;
+  if (idle) {
+    if constexpr (MODE == kLossGrad) {
+      // zeros in granules of the gradient's own alignment
+      const int dm = (int)((uintptr_t)d & 15) / (int)sizeof(T);
+      uint4 *base = reinterpret_cast<uint4 *>(d - dm);
+      for (int g = tid; g * E < dm + n; g += NT) {
+        if (g * E >= dm && (g + 1) * E <= dm + n) {
+          base[g] = uint4{0, 0, 0, 0};
+        } else {
+          for (int j = 0; j < E; ++j) {
+            const int e = g * E + j - dm;
+            if (e >= 0 && e < n) d[e] = from_f<T>(0.0f);
+          }
+        }
       }
     }
-    const float ym = block_reduce<OpMax>(y, buf);
-    if (ym == -kInf) {  // no entries: a padded row
-      if (tid == 0) loss[row] = 0.0f;
-      if (d)
-        for (int v = tid; v < a.classes; v += kThreads) d[v] = from_f<T>(0.0f);
-      continue;
+    return;  // all CTAs of the cluster alike
+  }
+  if (C > 1) cluster_arrive();  // waited for before the first peer store
+
+  // ---- the slab
+  const T *x = static_cast<const T *>(a.x) + (int64_t)row * a.stride + first;
+  const int mis = (int)((uintptr_t)x & 15) / (int)sizeof(T);
+  const int G = n > 0 ? (mis + n + E - 1) / E : 0;
+  uint4 *slab = reinterpret_cast<uint4 *>(smem);
+  T *sx = reinterpret_cast<T *>(smem) + mis;  // sx[e] = x[e]
+  {
+    const uint4 *src = reinterpret_cast<const uint4 *>(x - mis);
+    for (int g = tid; g < G; g += NT) {
+      if (g * E >= mis && (g + 1) * E <= mis + n) {
+        copy16(slab + g, src + g);
+      } else {
+        for (int j = 0; j < E; ++j) {
+          const int e = g * E + j - mis;
+          sx[e] = e >= 0 && e < n ? x[e] : from_f<T>(-kInf);
+        }
+      }
     }
-    const float ty = (y - ym) * a.inv_t;
-    const float ey = id >= 0 ? expf(ty) : 0.0f;
-    const float ys = block_reduce<OpAdd>(ey, buf);
+  }
+  [[maybe_unused]] float xk[4], tok_x = 0.0f;
+  if constexpr (MODE == kLoss || MODE == kLossGrad) {
+    // meanwhile the teacher's softmax, and the logits of its entries (read
+    // before any CTA of the row writes its gradient: the exchange below is a
+    // barrier of them all)
+    float ys = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      xk[i] = 0.0f;
+      ty[i] = tid_[i] >= 0 ? (ty[i] - ym) * a.inv_t : -kInf;
+      tq[i] = expf(ty[i]);
+      ys += tq[i];
+      if (leader && warp == 0 && tid_[i] >= 0)
+        xk[i] = to_f((x - first)[tid_[i]]);
+    }
+    for (int o = 16; o; o >>= 1) ys += __shfl_xor_sync(~0u, ys, o);
+    ln_ys = logf(ys);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      tq[i] = tq[i] / ys;
+      const int k = lane + 32 * i;
+      if (MODE == kLossGrad && warp == 0 && k < p.te.k) {
+        sq[k] = tq[i];
+        sid[k] = tid_[i];
+      }
+    }
+  } else {
+    if (leader && tid == 0 && p.o.logprob && tok < a.classes)
+      tok_x = to_f(x[tok]);
+  }
+  copies_done();
+
+  // ---- statistics of the thread's granules, the team's
+  GranuleMax<T> gm;
+  gm.clear();
+  for (int g = tid; g < G; g += NT) gm.add(slab[g]);
+  Stat st;
+  st.m = gm.get();
+  [[maybe_unused]] const float mine = st.m;
+  {
+    const float m0 = st.m == -kInf ? 0.0f : st.m;
+    const uint64_t nm = f2(-m0, -m0), c2 = f2(a.c, a.c);
+    uint64_t s2 = 0, u2 = 0;
+    for (int g = tid; g < G; g += NT)
+      accumulate<T, MODE <= kReadTop>(slab[g], nm, c2, s2, u2);
+    float s0, s1, u0, u1;
+    f2_split(s2, s0, s1);
+    f2_split(u2, u0, u1);
+    st.s = s0 + s1;
+    st.u = u0 + u1;
+  }
+  st = warp_combine(st, a.c);
+  uint32_t *gmax = reinterpret_cast<uint32_t *>(smem + p.l.gmax);
+  uint32_t *misc = reinterpret_cast<uint32_t *>(smem + p.l.misc);
+  // maxima of groups of threads (4 lanes each when that leaves enough groups)
+  [[maybe_unused]] const bool quads = NT >= 128 && p.top_k <= NT / 8;
+  [[maybe_unused]] const int groups = quads ? NT / 4 : NT;
+  if constexpr (MODE == kReadTop) {
+    uint32_t o = st.m < kInf ? order_of(mine) : 0;
+    if (quads) {
+      o = max(o, __shfl_xor_sync(~0u, o, 1));
+      o = max(o, __shfl_xor_sync(~0u, o, 2));
+      if ((tid & 3) == 0) gmax[tid >> 2] = o;
+    } else {
+      gmax[tid] = o;
+    }
+    if (tid == 0) misc[0] = 0;  // candidates
+  }
+  if constexpr (!kWarp) {
+    float *part = reinterpret_cast<float *>(smem + p.l.stats);
+    const int mine_at = ((int)rank * kWarps + warp) * 4;
+    if (C > 1) {
+      cluster_wait();
+      if (lane < (int)C) {
+        const uint32_t to = peer_addr(part + mine_at, lane);
+        peer_store(to, st.m);
+        peer_store(to + 4, st.s);
+        peer_store(to + 8, st.u);
+      }
+      cluster_arrive();
+      cluster_wait();
+    } else {
+      if (lane == 0) {
+        part[mine_at] = st.m;
+        part[mine_at + 1] = st.s;
+        part[mine_at + 2] = st.u;
+      }
+      __syncthreads();
+    }
+    // every warp adds the same parts in the same order
+    const int parts = (int)C * kWarps;
     float m = -kInf;
-    for (int v = tid; v < a.classes; v += kThreads) m = max_nan(m, to_f(x[v]));
-    m = block_reduce<OpMax>(m, buf);
-    const bool bad = !(m < kInf) || !(ym < kInf);
-    const bool empty = m == -kInf;
-    float s = 0.0f;
-    if (!bad && !empty)
-      for (int v = tid; v < a.classes; v += kThreads)
-        s += ex2((to_f(x[v]) - m) * a.c);
-    s = block_reduce<OpAdd>(s, buf);
-    const float ln_s = logf(s), q = ey / ys;
-    float l = 0.0f;
-    if (q > 0.0f)
-      l = empty ? kInf
-                : q * ((ty - logf(ys)) - ((to_f(x[id]) - m) * a.inv_t - ln_s));
-    l = block_reduce<OpAdd>(l, buf);
-    if (tid == 0) loss[row] = bad ? nan : a.t * a.t * l;
-    if (!d) continue;
-    const float w = (row_weight ? row_weight[row] : weight) * a.t;
-    if (tid < te.k) {
-      sq[tid] = q;
-      sid[tid] = id;
+    for (int i = lane; i < parts; i += 32) m = max_nan(m, part[i * 4]);
+    st = Stat{m, 0.0f, 0.0f};
+    for (int i = lane; i < parts; i += 32) {
+      Stat v{part[i * 4], part[i * 4 + 1], part[i * 4 + 2]};
+      rescale(v, m, a.c);
+      st.s += v.s;
+      st.u += v.u;
     }
-    __syncthreads();
-    // x is read before dx of the same element is written (they may be one)
-    float own = 0.0f;
-    if (!bad && !empty && tid < te.k && id >= 0) {
-      float both = 0.0f;  // entries of one class add up
-      for (int j = 0; j < te.k; ++j) both += sid[j] == id ? sq[j] : 0.0f;
-      own = w * (ex2((to_f(x[id]) - m) * a.c) / s - both);
+    st = warp_combine(st, a.c);
+  } else {
+    __syncwarp();
+  }
+  const float m = st.m, s = st.s;
+  const bool bad = !(m < kInf) || (MODE >= kLoss && !(ym < kInf));
+  const bool empty = m == -kInf;
+  const float ln_s = logf(s);
+
+  if constexpr (MODE == kRead || MODE == kReadTop) {
+    if (leader && tid == 0) {
+      const float h = bad ? nan : empty ? 0.0f : ln_s - kLn2 * st.u / s;
+      if (p.o.entropy) p.o.entropy[row] = h;
+      if (p.o.logprob) {
+        float lp = nan;
+        if (!bad && tok < a.classes)
+          lp = empty ? -kInf : (tok_x - m) * a.inv_t - ln_s;
+        p.o.logprob[row] = lp;
+      }
+      if (p.o.stats) {
+        float *so = p.o.stats + (int64_t)row * 3;
+        so[0] = bad ? nan : m;
+        so[1] = bad ? nan : empty ? 0.0f : s;
+        so[2] = h;
+      }
     }
-    __syncthreads();
-    const float ws = w / s;
-    for (int v = tid; v < a.classes; v += kThreads) {
-      const float r =
-          bad ? nan : empty ? 0.0f : ex2((to_f(x[v]) - m) * a.c) * ws;
-      d[v] = from_f<T>(r);
+  }
+
+  if constexpr (MODE == kReadTop) {
+    // ---- alternatives.  The K-th largest of the groups' maxima is a lower
+    // bound of the slab's K-th largest logit, and few logits lie above it.
+    const int K = p.top_k;
+    int32_t *ids = p.o.top_ids + (int64_t)row * K;
+    float *lps = p.o.top_logprobs + (int64_t)row * K;
+    auto put = [&](int at, uint64_t key) {
+      ids[at] = key ? class_of(key) : -1;
+      lps[at] = bad   ? nan
+                : key ? (value_of((uint32_t)(key >> 32)) - m) * a.inv_t - ln_s
+                      : -kInf;
+    };
+    if (bad || empty) {  // the same in all CTAs of the row
+      if (leader)
+        for (int k = tid; k < K; k += NT) put(k, 0);
+      return;
     }
-    __syncthreads();
-    if (!bad && !empty && tid < te.k && id >= 0) d[id] = from_f<T>(own);
-    __syncthreads();
+    uint64_t *cand = reinterpret_cast<uint64_t *>(smem + p.l.cand);
+    if (tid < groups) {
+      const uint32_t v = gmax[tid];
+      int r = 0;
+      for (int j = 0; j < groups; j += 4) {
+        const uint4 q = *reinterpret_cast<const uint4 *>(gmax + j);
+        r += q.x > v || (q.x == v && j < tid);
+        r += q.y > v || (q.y == v && j + 1 < tid);
+        r += q.z > v || (q.z == v && j + 2 < tid);
+        r += q.w > v || (q.w == v && j + 3 < tid);
+      }
+      if (r == K - 1) misc[1] = max(v, kLowestOrder);
+    }
+    team_sync();
+    const uint32_t tau = misc[1];
+    const uint32_t my_order = order_of(mine);
+    // keys at or above `least` into cand (those that fit); their number
+    auto collect = [&](uint64_t least) {
+      if ((((uint64_t)my_order << 32) | 0xFFFFFFFFu) >= least) {
+        const float floor = value_of((uint32_t)(least >> 32));
+        for (int g = tid; g < G; g += NT) {
+          const uint4 q = slab[g];
+          GranuleMax<T> t;
+          t.clear();
+          t.add(q);
+          if (!(t.get() >= floor)) continue;
+#pragma unroll
+          for (int i = 0; i < E; ++i) {
+            float f[2];
+            f2_split(pair_of<T>(q, i >> 1), f[0], f[1]);
+            const float v = f[i & 1];
+            if (v >= floor) {
+              const uint64_t key = key_of(v, first + g * E + i - mis);
+              if (key >= least) {
+                const uint32_t at = atomicAdd(misc, 1u);
+                if (at < (uint32_t)p.l.cap) cand[at] = key;
+              }
+            }
+          }
+        }
+      }
+      team_sync();
+      const int count = (int)misc[0];
+      team_sync();
+      return count;
+    };
+    int M = collect((uint64_t)tau << 32);
+    // Rows with thousands of equal or regularly placed values overflow the
+    // buffer: halve the interval of keys (which are distinct) until between K
+    // and `cap` of them are left.
+    // (64 halvings use the interval up.)
+    uint64_t lo = (uint64_t)tau << 32, hi = ~0ull;
+    for (int i = 0, c = M; i < 64 && (c > p.l.cap || c < K) && M > p.l.cap; ++i) {
+      const uint64_t mid = lo + ((hi - lo) >> 1);
+      if (tid == 0) misc[0] = 0;
+      team_sync();
+      c = collect(mid);
+      (c < K ? hi : lo) = mid;
+      if (c >= K) M = c;
+    }
+    M = min(M, p.l.cap);
+    uint64_t *merge = reinterpret_cast<uint64_t *>(smem + p.l.merge);
+    auto keep = [&](int at, uint64_t key) {
+      if (C > 1)
+        peer_store(peer_addr(merge + rank * K + at, 0), key);
+      else
+        put(at, key);
+    };
+    for (int i = tid; i < M; i += NT) {
+      const uint64_t key = cand[i];
+      int r = 0;
+      for (int j = 0; j < M; ++j) r += cand[j] > key;
+      if (r < K) keep(r, key);
+    }
+    for (int k = M + tid; k < K; k += NT) keep(k, 0);
+    if (C > 1) {
+      cluster_arrive();
+      cluster_wait();
+      if (!leader) return;
+      const int all = (int)C * K;
+      for (int i = tid; i < all; i += NT) {
+        const uint64_t key = merge[i];
+        int r = 0;
+        for (int j = 0; j < all; ++j) {
+          const uint64_t q = merge[j];
+          r += q > key || (q == key && j < i);  // 0 may be there many times
+        }
+        if (r < K) put(r, key);
+      }
+    }
+  }
+
+  if constexpr (MODE == kLoss || MODE == kLossGrad) {
+    if (leader && warp == 0) {
+      float l = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (tq[i] > 0.0f)
+          l += empty ? kInf
+                     : tq[i] * ((ty[i] - ln_ys) - ((xk[i] - m) * a.inv_t - ln_s));
+      for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
+      if (lane == 0) p.loss[row] = bad ? nan : a.t * a.t * l;
+    }
+  }
+  if constexpr (MODE == kLossGrad) {
+    const float w = (p.row_weight ? p.row_weight[row] : p.weight) * a.t;
+    const float ws = bad ? nan : empty ? 0.0f : w / s;
+    // an empty row: 0 * 0 (its logits at -inf give e = 0 against m = 0)
+    const float m0 = empty ? 0.0f : m;
+    const uint64_t nm = f2(-m0, -m0), c2 = f2(a.c, a.c), w2 = f2(ws, ws);
+    const int dm = (int)((uintptr_t)d & 15) / (int)sizeof(T);
+    if (dm == mis) {
+      uint4 *dst = reinterpret_cast<uint4 *>(d - dm);
+      for (int g = tid; g < G; g += NT) {
+        const uint4 q = slab[g];
+        float r[E];
+#pragma unroll
+        for (int i = 0; i < E / 2; ++i) {
+          float u, v;
+          f2_split(f2_mul(f2_add(pair_of<T>(q, i), nm), c2), u, v);
+          f2_split(f2_mul(f2(ex2(u), ex2(v)), w2), r[2 * i], r[2 * i + 1]);
+        }
+        if (g * E >= mis && (g + 1) * E <= mis + n) {
+          uint4 out;
+          if constexpr (sizeof(T) == 4) {
+            out = uint4{__float_as_uint(r[0]), __float_as_uint(r[1]),
+                        __float_as_uint(r[2]), __float_as_uint(r[3])};
+          } else {
+            out = uint4{pack2<T>(r[0], r[1]), pack2<T>(r[2], r[3]),
+                        pack2<T>(r[4], r[5]), pack2<T>(r[6], r[7])};
+          }
+          dst[g] = out;
+        } else {
+#pragma unroll
+          for (int j = 0; j < E; ++j) {
+            const int e = g * E + j - mis;
+            if (e >= 0 && e < n) d[e] = from_f<T>(r[j]);
+          }
+        }
+      }
+    } else {
+      // rows of another alignment: element by element, lanes side by side
+      // (the copies of other threads are visible since the exchange)
+#pragma unroll 4
+      for (int e = tid; e < n; e += NT)
+        d[e] = from_f<T>(ex2((to_f(sx[e]) - m0) * a.c) * ws);
+    }
+    team_sync();  // an entry's element is written again, after its first value
+    if (!bad && !empty) {
+      for (int k = tid; k < p.te.k; k += NT) {
+        const int id = sid[k] - first;
+        if (sid[k] < 0 || id < 0 || id >= n) continue;
+        float both = 0.0f;  // entries of one class add up
+        for (int j = 0; j < p.te.k; ++j)
+          both += sid[j] == sid[k] ? sq[j] : 0.0f;
+        d[id] = from_f<T>(w * (ex2((to_f(sx[id]) - m) * a.c) / s - both));
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------ backward
+// Element by element from the saved statistics; a warp takes a run of 32 x
+// kRun granules of one row.  Bound by the memory: the logits in, the gradient
+// out.
+constexpr int kRun = 8;
+
+template <class T>
+__global__ void __launch_bounds__(256)
+    k_backward(RowArgs a, const void *tokens, int itype, const float *stats,
+               const float *d_logprob, const float *d_entropy, T *dx,
+               int64_t d_stride, uint32_t runs) {
+  constexpr int E = kElems<T>;
+  const int lane = threadIdx.x & 31;
+  const uint64_t unit = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const uint32_t row = (uint32_t)(unit / runs);
+  if (row >= a.rows) return;
+  const int run = (int)(unit % runs);
+  const T *x = static_cast<const T *>(a.x) + (int64_t)row * a.stride;
+  T *d = dx + (int64_t)row * d_stride;
+  const int64_t tok = tokens ? load_index(tokens, row, itype) : -1;
+  const float m = stats[(int64_t)row * 3], s = stats[(int64_t)row * 3 + 1],
+              h = stats[(int64_t)row * 3 + 2];
+  float g = d_logprob ? d_logprob[row] * a.inv_t : 0.0f;
+  const float b = d_entropy ? d_entropy[row] * a.inv_t : 0.0f;
+  if (tokens && tok >= a.classes) g = __int_as_float(0x7FFFFFFF);
+  const bool idle = s == 0.0f || (tokens && tok < 0);
+  const float inv_s = 1.0f / s;
+  // d = -p (g + b (t ln 2 - ln s + H)) = p (k0 + k1 t), t in units of log2(e)
+  const float k1 = -b * kLn2 * inv_s;
+  const float k0 = -(g + b * (h - logf(s))) * inv_s;
+  const bool plain = b == 0.0f;  // no 0 * inf from t = -inf then
+  auto grad = [&](float v, int e) {
+    const float t = (v - m) * a.c;
+    const float p = ex2(t);
+    float r = p * (plain ? k0 : k0 + k1 * fmaxf(t, -1e4f));
+    if (e == tok) r += g;
+    return idle ? 0.0f : r;
+  };
+  const int mis = (int)((uintptr_t)x & 15) / (int)sizeof(T);
+  const int dm = (int)((uintptr_t)d & 15) / (int)sizeof(T);
+  const int V = a.classes;
+  if (mis == dm) {
+    const uint4 *src = reinterpret_cast<const uint4 *>(x - mis);
+    uint4 *dst = reinterpret_cast<uint4 *>(d - dm);
+    const int g0 = run * 32 * kRun + lane;
+    uint4 q[kRun];
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      const int gi = g0 + 32 * i;
+      q[i] = uint4{0, 0, 0, 0};
+      if (!idle && gi * E >= mis && (gi + 1) * E <= mis + V) q[i] = src[gi];
+    }
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+      const int gi = g0 + 32 * i;
+      const int e0 = gi * E - mis;
+      if (e0 >= 0 && e0 + E <= V) {
+        float r[E];
+#pragma unroll
+        for (int j = 0; j < E / 2; ++j) {
+          float u, v;
+          f2_split(pair_of<T>(q[i], j), u, v);
+          r[2 * j] = grad(u, e0 + 2 * j);
+          r[2 * j + 1] = grad(v, e0 + 2 * j + 1);
+        }
+        uint4 out;
+        if constexpr (sizeof(T) == 4) {
+          out = uint4{__float_as_uint(r[0]), __float_as_uint(r[1]),
+                      __float_as_uint(r[2]), __float_as_uint(r[3])};
+        } else {
+          out = uint4{pack2<T>(r[0], r[1]), pack2<T>(r[2], r[3]),
+                      pack2<T>(r[4], r[5]), pack2<T>(r[6], r[7])};
+        }
+        dst[gi] = out;
+      } else {
+        for (int j = 0; j < E; ++j) {
+          const int e = e0 + j;
+          if (e >= 0 && e < V)
+            d[e] = from_f<T>(idle ? 0.0f : grad(to_f(x[e]), e));
+        }
+      }
+    }
+  } else {
+    const int e0 = run * 32 * kRun * E + lane;
+#pragma unroll 8
+    for (int i = 0; i < kRun * E; ++i) {
+      const int e = e0 + 32 * i;
+      if (e < V) d[e] = from_f<T>(idle ? 0.0f : grad(to_f(x[e]), e));
+    }
   }
 }
 
@@ -403,8 +932,6 @@ void check_grad(const char *who, const tmnn_logits &x, const void *d,
     bad(std::string(who) + ": d_logits overlaps the logits in part");
 }
 
-uint32_t row_grid(uint32_t rows) { return rows < (1u << 20) ? rows : 1u << 20; }
-
 #define BY_DTYPE(dtype, ...)                 \
   do {                                       \
     if ((dtype) == TMNN_DTYPE_F32) {         \
@@ -418,6 +945,102 @@ uint32_t row_grid(uint32_t rows) { return rows < (1u << 20) ? rows : 1u << 20; }
       __VA_ARGS__;                           \
     }                                        \
   } while (0)
+
+constexpr int kMaxDevices = 64;
+int sm_count() {
+  static std::atomic<int> known[kMaxDevices];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= kMaxDevices) return 148;
+  int n = known[dev].load(std::memory_order_relaxed);
+  if (!n) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) !=
+        cudaSuccess)
+      return 148;
+    known[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
+// Shared memory above 48 KB and clusters above 8 CTAs are asked for once a
+// kernel and device.
+template <class K>
+void allow(K kernel, std::atomic<uint64_t> &done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_acquire) & bit) return;
+  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                       227 * 1024);
+  cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  done.fetch_or(bit, std::memory_order_release);
+}
+
+template <class T, int NT, int MODE>
+void launch_team_of(TeamArgs &p, cudaStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  auto kernel = k_team<T, NT, MODE>;
+  allow(kernel, done);
+  constexpr int teams = NT == 32 ? 4 : 1;
+  const int granules = p.slab / kElems<T> + 1;
+  p.l = team_layout(MODE, NT, p.cluster, MODE >= kLoss ? p.te.k : p.top_k,
+                    granules);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((p.a.rows + teams - 1) / teams * p.cluster);
+  cfg.blockDim = dim3(NT * teams);
+  cfg.dynamicSmemBytes = (size_t)p.l.total * teams;
+  cfg.stream = st;
+  cudaLaunchAttribute at;
+  if (p.cluster > 1) {
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = p.cluster;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+  }
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+  if (e != cudaSuccess)
+    throw std::runtime_error(std::string("class-logit kernel: ") +
+                             cudaGetErrorString(e));
+}
+
+// Threads and CTAs of a row.  Slabs of up to 64 KB leave three CTAs on an SM,
+// so that two of them load while one computes; with too few rows to fill the
+// SMs a row is split further.
+template <class T, int MODE>
+void launch_team(TeamArgs &p, cudaStream_t st) {
+  constexpr int E = kElems<T>;
+  const int64_t bytes = (int64_t)p.a.classes * (int)sizeof(T);
+  const int sms = sm_count();
+  const int k = MODE == kReadTop ? p.top_k : 0;
+  int c = 1;
+  while (c < 8 && bytes > (int64_t)c * 64 * 1024) c *= 2;
+  while (c < 8 && bytes >= (int64_t)c * 16 * 1024 &&
+         (int64_t)p.a.rows * c < 2 * sms)
+    c *= 2;
+  if (bytes > 8 * 128 * 1024) c = 16;
+  p.cluster = c;
+  p.slab = ((p.a.classes + c - 1) / c + E - 1) / E * E;
+  const int granules = p.slab / E + 1;
+  if (c == 1 && granules <= 256 && k <= 32)
+    launch_team_of<T, 32, MODE>(p, st);
+  else if (granules <= 1024)
+    launch_team_of<T, 128, MODE>(p, st);
+  else
+    launch_team_of<T, 256, MODE>(p, st);
+}
+
+// Launches for rows [i, i + n) of all, n small enough for a grid.
+template <class F>
+int in_parts(uint32_t rows, F &&f) {
+  constexpr uint32_t most = 1u << 26;
+  int launches = 0;
+  for (uint64_t i = 0; i < rows; i += most, ++launches)
+    f((uint32_t)i, (uint32_t)(rows - i < most ? rows - i : most));
+  return launches;
+}
+const void *at(const void *p, int64_t bytes) {
+  return p ? static_cast<const unsigned char *>(p) + bytes : nullptr;
+}
 
 }  // namespace
 
@@ -442,10 +1065,24 @@ int launch_token_logprobs(const tmnn_logits &x, const void *tokens,
     check_ptr(who, "top_ids", o.top_ids, 4);
     check_ptr(who, "top_logprobs", o.top_logprobs, 4);
   }
-  BY_DTYPE(x.dtype, (k_logprobs<T><<<row_grid(x.rows), kThreads, 0, st>>>(
-                        a, tokens, index_type, (int)top_k, o)));
-  launched(who);
-  return 1;
+  return in_parts(x.rows, [&](uint32_t i, uint32_t n) {
+    TeamArgs p{};
+    p.a = a;
+    p.a.x = at(x.data, (int64_t)i * x.row_stride * elem_size(x.dtype));
+    p.a.rows = n;
+    p.tokens = at(tokens, (int64_t)i * index_size(index_type));
+    p.itype = index_type;
+    p.top_k = (int)top_k;
+    p.o.logprob = o.logprob ? o.logprob + i : nullptr;
+    p.o.entropy = o.entropy ? o.entropy + i : nullptr;
+    p.o.top_ids = top_k ? o.top_ids + (int64_t)i * top_k : nullptr;
+    p.o.top_logprobs = top_k ? o.top_logprobs + (int64_t)i * top_k : nullptr;
+    p.o.stats = o.stats ? o.stats + (int64_t)i * 3 : nullptr;
+    if (top_k)
+      BY_DTYPE(x.dtype, (launch_team<T, kReadTop>(p, st)));
+    else
+      BY_DTYPE(x.dtype, (launch_team<T, kRead>(p, st)));
+  });
 }
 
 int launch_token_logprobs_backward(const tmnn_logits &x, const void *tokens,
@@ -464,12 +1101,23 @@ int launch_token_logprobs_backward(const tmnn_logits &x, const void *tokens,
   check_opt(who, "d_logprob", d_logprob, 4);
   check_opt(who, "d_entropy", d_entropy, 4);
   check_grad(who, x, d_logits, d_stride);
-  BY_DTYPE(x.dtype,
-           (k_logprobs_backward<T><<<row_grid(x.rows), kThreads, 0, st>>>(
-               a, tokens, index_type, stats, d_logprob, d_entropy,
-               static_cast<T *>(d_logits), d_stride)));
-  launched(who);
-  return 1;
+  const int size = elem_size(x.dtype), per_run = 32 * kRun * (16 / size);
+  // one granule more than the row's bytes hold: rows may start inside one
+  const uint32_t runs = (x.classes + 16 / size + per_run - 1) / per_run;
+  return in_parts(x.rows, [&](uint32_t i, uint32_t n) {
+    RowArgs b = a;
+    b.x = at(x.data, (int64_t)i * x.row_stride * size);
+    b.rows = n;
+    const void *d = at(d_logits, (int64_t)i * d_stride * size);
+    const uint32_t grid = (uint32_t)(((uint64_t)n * runs + 7) / 8);
+    BY_DTYPE(x.dtype,
+             (k_backward<T><<<grid, 256, 0, st>>>(
+                 b, at(tokens, (int64_t)i * index_size(index_type)), index_type,
+                 stats + (int64_t)i * 3, d_logprob ? d_logprob + i : nullptr,
+                 d_entropy ? d_entropy + i : nullptr,
+                 static_cast<T *>(const_cast<void *>(d)), d_stride, runs)));
+    launched(who);
+  });
 }
 
 int launch_distill(const tmnn_logits &x, const void *ids, int index_type,
@@ -487,12 +1135,25 @@ int launch_distill(const tmnn_logits &x, const void *ids, int index_type,
   check_opt(who, "row_weight", row_weight, 4);
   check_ptr(who, "loss", loss, 4);
   if (d_logits) check_grad(who, x, d_logits, d_stride);
-  const Teacher te{ids, teacher, index_type, teacher_dtype, (int)k};
-  BY_DTYPE(x.dtype, (k_distill<T><<<row_grid(x.rows), kThreads, 0, st>>>(
-                        a, te, row_weight, weight, loss,
-                        static_cast<T *>(d_logits), d_stride)));
-  launched(who);
-  return 1;
+  const int size = elem_size(x.dtype);
+  return in_parts(x.rows, [&](uint32_t i, uint32_t n) {
+    TeamArgs p{};
+    p.a = a;
+    p.a.x = at(x.data, (int64_t)i * x.row_stride * size);
+    p.a.rows = n;
+    p.te = {at(ids, (int64_t)i * k * index_size(index_type)),
+            at(teacher, (int64_t)i * k * elem_size(teacher_dtype)), index_type,
+            teacher_dtype, (int)k};
+    p.row_weight = row_weight ? row_weight + i : nullptr;
+    p.weight = weight;
+    p.loss = loss + i;
+    p.dx = const_cast<void *>(at(d_logits, (int64_t)i * d_stride * size));
+    p.d_stride = d_stride;
+    if (d_logits)
+      BY_DTYPE(x.dtype, (launch_team<T, kLossGrad>(p, st)));
+    else
+      BY_DTYPE(x.dtype, (launch_team<T, kLoss>(p, st)));
+  });
 }
 
 void launch_row_sum(const float *values, uint32_t n, double *sum,
