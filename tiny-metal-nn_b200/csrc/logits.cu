@@ -280,24 +280,80 @@ struct Teacher {
   int itype, dtype, k;
 };
 
+// the granule whose every element is -inf
+template <class T>
+__device__ __forceinline__ uint4 no_logits() {
+  const uint32_t w = sizeof(T) == 4                   ? 0xFF800000u
+                     : std::is_same<T, __half>::value ? 0xFC00FC00u
+                                                      : 0xFF80FF80u;
+  return uint4{w, w, w, w};
+}
+template <class T>
+__device__ __forceinline__ uint4 pack_granule(const float *r) {
+  if constexpr (sizeof(T) == 4)
+    return uint4{__float_as_uint(r[0]), __float_as_uint(r[1]),
+                 __float_as_uint(r[2]), __float_as_uint(r[3])};
+  else
+    return uint4{pack2<T>(r[0], r[1]), pack2<T>(r[2], r[3]),
+                 pack2<T>(r[4], r[5]), pack2<T>(r[6], r[7])};
+}
+
+// What one row's reads give, from its statistics.
+struct RowEnd {
+  float m, s, u, inv_t, ln_s;
+  bool bad, empty;
+  __device__ __forceinline__ RowEnd(const Stat &v, float inv_t_)
+      : m(v.m), s(v.s), u(v.u), inv_t(inv_t_), ln_s(logf(v.s)),
+        bad(!(v.m < kInf)), empty(v.m == -kInf) {}
+  __device__ __forceinline__ float logp(float x) const {
+    return (x - m) * inv_t - ln_s;
+  }
+};
+__device__ __forceinline__ float not_a_number() {
+  return __int_as_float(0x7FFFFFFF);
+}
+__device__ __forceinline__ void write_read(const LogprobOut &o, uint32_t row,
+                                           const RowEnd &r, float tok_x,
+                                           bool tok_ok) {
+  const float nan = not_a_number();
+  const float h = r.bad ? nan : r.empty ? 0.0f : r.ln_s - kLn2 * r.u / r.s;
+  if (o.entropy) o.entropy[row] = h;
+  if (o.logprob)
+    o.logprob[row] = r.bad || !tok_ok ? nan : r.empty ? -kInf : r.logp(tok_x);
+  if (o.stats) {
+    float *so = o.stats + (int64_t)row * 3;
+    so[0] = r.bad ? nan : r.m;
+    so[1] = r.bad ? nan : r.empty ? 0.0f : r.s;
+    so[2] = h;
+  }
+}
+__device__ __forceinline__ void write_read_padding(const LogprobOut &o,
+                                                   uint32_t row) {
+  if (o.logprob) o.logprob[row] = 0.0f;
+  if (o.entropy) o.entropy[row] = 0.0f;
+  if (o.stats)
+    for (int i = 0; i < 3; ++i) o.stats[(int64_t)row * 3 + i] = 0.0f;
+}
+
 // ------------------------------------------------------------ a team a row
-// A team -- a warp, a CTA, or a cluster of CTAs each holding a part ("slab")
-// of the row in its shared memory -- reads a row once.  Every thread copies
-// its own granules (cp.async) and works on the same ones in each pass, so the
-// passes need no barrier between them: maximum, sums relative to the thread's
-// maximum, one exchange of (m, s, u) over the team, and then the alternatives
-// or the gradient from the slab.  Memory traffic is that of the operator
+// A team -- a CTA, or a cluster of CTAs each holding a part ("slab") of the
+// row in its shared memory -- reads a row once.  Every thread copies its own
+// granules (cp.async) and sums over the same ones, so there is no barrier
+// before the one exchange of (m, s, u) over the team; then the alternatives or
+// the gradient come from the slab.  Memory traffic is that of the operator
 // itself: the row once in, results or gradient once out.
-enum Mode { kRead = 0, kReadTop = 1, kLoss = 2, kLossGrad = 3 };
+enum Mode { kRead = 0, kReadTop = 1, kLoss = 2, kLossGrad = 3, kBack = 4 };
 
 constexpr int kMaxCluster = 16;
 constexpr uint32_t kLowestOrder = 0x00800000u;  // order of the lowest finite
+constexpr int kMaxGroups = 256;
 
-// Shared memory of a team, in bytes from its base: the slab, the exchange of
-// statistics, and what the mode needs.
+// Shared memory of a CTA of a team, in bytes from its base: the slab, the
+// exchange of statistics, and what the mode needs.
 struct TeamLayout {
-  int stats, teacher, gmax, cand, merge, misc, total;
-  int cap;  // candidates for the alternatives
+  int stats, teacher, misc, gmax, cand, total;
+  int cap;     // candidates a CTA may hold
+  int groups;  // groups of threads over the team, each with its maximum
 };
 __host__ __device__ inline TeamLayout team_layout(int mode, int threads,
                                                   int cluster, int k,
@@ -310,14 +366,14 @@ __host__ __device__ inline TeamLayout team_layout(int mode, int threads,
   if (mode >= kLoss) off += (k * 8 + 15) / 16 * 16;
   l.misc = off;
   if (mode == kReadTop) {
-    off += 16;
+    off += 16 + 2 * kMaxCluster * 4;  // count, threshold; counts of the CTAs
     l.gmax = off;
-    off += threads * 4;
-    l.cap = 4 * k > 256 ? 4 * k : 256;
+    l.groups = cluster * threads;
+    while (l.groups > kMaxGroups) l.groups /= 2;
+    off += l.groups * 4;
+    l.cap = 2 * k > 128 ? 2 * k : 128;
     l.cand = off;
-    off += l.cap * 8;
-    l.merge = off;
-    if (cluster > 1) off += cluster * k * 8;
+    off += cluster * l.cap * 8;  // in the first CTA those of all
   }
   l.total = (off + 15) / 16 * 16;
   return l;
@@ -336,33 +392,48 @@ struct TeamArgs {
   int64_t d_stride;
   int cluster;  // CTAs a row
   int slab;     // elements a CTA, a multiple of the granule
+  int eager;    // copy the slab before it is known whether the row is padding
   TeamLayout l;
 };
 
 template <class T, int NT, int MODE>
-__global__ void __launch_bounds__(NT == 32 ? 128 : NT) k_team(TeamArgs p) {
-  extern __shared__ __align__(16) unsigned char smem_all[];
+__global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
+  extern __shared__ __align__(16) unsigned char smem[];
   constexpr int E = kElems<T>;
-  constexpr bool kWarp = NT == 32;
-  constexpr int kTeams = kWarp ? 4 : 1;
   constexpr int kWarps = NT / 32;
+  constexpr bool kReads = MODE == kRead || MODE == kReadTop;
   const RowArgs &a = p.a;
-  const int tid = kWarp ? threadIdx.x & 31 : threadIdx.x;
-  const int lane = threadIdx.x & 31, warp = kWarp ? 0 : threadIdx.x >> 5;
-  const int team = kWarp ? threadIdx.x >> 5 : 0;
-  const uint32_t C = kWarp ? 1 : p.cluster;
-  const uint32_t rank = kWarp ? 0 : blockIdx.x % C;
-  const uint32_t row = blockIdx.x / C * kTeams + team;
-  if (row >= a.rows) return;  // whole warps; CTA teams cover the rows exactly
-  unsigned char *smem = smem_all + team * p.l.total;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t C = p.cluster, rank = blockIdx.x % C, row = blockIdx.x / C;
   const bool leader = rank == 0;
-  const float nan = __int_as_float(0x7FFFFFFF);
-  auto team_sync = [&] {
-    if constexpr (kWarp)
-      __syncwarp();
-    else
-      __syncthreads();
+  const float nan = not_a_number();
+
+  // ---- the slab: x[first .. first + n) of the row
+  const int first = (int)rank * p.slab;
+  const int n = max(0, min(p.slab, a.classes - first));
+  const T *x = static_cast<const T *>(a.x) + (int64_t)row * a.stride + first;
+  const int mis = (int)((uintptr_t)x & 15) / (int)sizeof(T);
+  const int G = n > 0 ? (mis + n + E - 1) / E : 0;
+  uint4 *slab = reinterpret_cast<uint4 *>(smem);
+  T *sx = reinterpret_cast<T *>(smem) + mis;  // sx[e] = x[e]
+  auto load = [&] {
+    const uint4 *src = reinterpret_cast<const uint4 *>(x - mis);
+    const int lo = mis ? 1 : 0, hi = (mis + n) / E;  // whole granules
+    for (int g = tid; g < hi; g += NT)
+      if (g >= lo) copy16(slab + g, src + g);
+    // the first and last one, by the threads they belong to
+    if ((lo && tid == 0) || (G > hi && tid == hi % NT)) {
+      for (int i = 0; i < 2; ++i) {
+        const int g = i ? hi : 0;
+        if ((i ? G > hi : lo) && tid == g % NT)
+          for (int j = 0; j < E; ++j) {
+            const int e = g * E + j - mis;
+            sx[e] = e >= 0 && e < n ? x[e] : from_f<T>(-kInf);
+          }
+      }
+    }
   };
+  if (p.eager) load();
 
   // ---- is the row padding?
   int64_t tok = 0;
@@ -371,16 +442,11 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT) k_team(TeamArgs p) {
   [[maybe_unused]] float ty[4], tq[4], ln_ys = 0.0f, ym = 0.0f;
   [[maybe_unused]] int32_t tid_[4];
   bool idle;
-  if constexpr (MODE == kRead || MODE == kReadTop) {
+  if constexpr (kReads) {
     if (p.tokens) tok = load_index(p.tokens, row, p.itype);
     idle = tok < 0;
     if (idle && leader) {
-      if (tid == 0) {
-        if (p.o.logprob) p.o.logprob[row] = 0.0f;
-        if (p.o.entropy) p.o.entropy[row] = 0.0f;
-        if (p.o.stats)
-          for (int i = 0; i < 3; ++i) p.o.stats[(int64_t)row * 3 + i] = 0.0f;
-      }
+      if (tid == 0) write_read_padding(p.o, row);
       if constexpr (MODE == kReadTop)
         for (int k = tid; k < p.top_k; k += NT) {
           p.o.top_ids[(int64_t)row * p.top_k + k] = -1;
@@ -408,8 +474,6 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT) k_team(TeamArgs p) {
     idle = ym == -kInf;
     if (idle && leader && tid == 0) p.loss[row] = 0.0f;
   }
-  const int first = (int)rank * p.slab;
-  const int n = min(p.slab, a.classes - first);  // may be below 1
   T *d = MODE == kLossGrad
              ? static_cast<T *>(p.dx) + (int64_t)row * p.d_stride + first
              : nullptr;
@@ -429,31 +493,14 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT) k_team(TeamArgs p) {
         }
       }
     }
+    copies_done();
     return;  // all CTAs of the cluster alike
   }
   if (C > 1) cluster_arrive();  // waited for before the first peer store
+  if (!p.eager) load();
 
-  // ---- the slab
-  const T *x = static_cast<const T *>(a.x) + (int64_t)row * a.stride + first;
-  const int mis = (int)((uintptr_t)x & 15) / (int)sizeof(T);
-  const int G = n > 0 ? (mis + n + E - 1) / E : 0;
-  uint4 *slab = reinterpret_cast<uint4 *>(smem);
-  T *sx = reinterpret_cast<T *>(smem) + mis;  // sx[e] = x[e]
-  {
-    const uint4 *src = reinterpret_cast<const uint4 *>(x - mis);
-    for (int g = tid; g < G; g += NT) {
-      if (g * E >= mis && (g + 1) * E <= mis + n) {
-        copy16(slab + g, src + g);
-      } else {
-        for (int j = 0; j < E; ++j) {
-          const int e = g * E + j - mis;
-          sx[e] = e >= 0 && e < n ? x[e] : from_f<T>(-kInf);
-        }
-      }
-    }
-  }
   [[maybe_unused]] float xk[4], tok_x = 0.0f;
-  if constexpr (MODE == kLoss || MODE == kLossGrad) {
+  if constexpr (!kReads) {
     // meanwhile the teacher's softmax, and the logits of its entries (read
     // before any CTA of the row writes its gradient: the exchange below is a
     // barrier of them all)
@@ -484,47 +531,68 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT) k_team(TeamArgs p) {
   }
   copies_done();
 
-  // ---- statistics of the thread's granules, the team's
-  GranuleMax<T> gm;
-  gm.clear();
-  for (int g = tid; g < G; g += NT) gm.add(slab[g]);
+  // ---- statistics of the thread's granules, four at a time: their maximum,
+  // the sums brought to it, their terms
+  constexpr int kBatch = 4;
+  float mine = -kInf;
   Stat st;
-  st.m = gm.get();
-  [[maybe_unused]] const float mine = st.m;
   {
-    const float m0 = st.m == -kInf ? 0.0f : st.m;
-    const uint64_t nm = f2(-m0, -m0), c2 = f2(a.c, a.c);
+    const uint64_t c2 = f2(a.c, a.c);
     uint64_t s2 = 0, u2 = 0;
-    for (int g = tid; g < G; g += NT)
-      accumulate<T, MODE <= kReadTop>(slab[g], nm, c2, s2, u2);
+    for (int g0 = tid; g0 < G; g0 += kBatch * NT) {
+      uint4 q[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        q[i] = g0 + i * NT < G ? slab[g0 + i * NT] : no_logits<T>();
+      GranuleMax<T> gm;
+      gm.clear();
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) gm.add(q[i]);
+      const float m = max_nan(mine, gm.get());
+      const float m0 = m == -kInf ? 0.0f : m;
+      const float dm = (mine - m0) * a.c, f = ex2(dm);
+      mine = m;
+      s2 = f2_mul(s2, f2(f, f));
+      if (kReads) {
+        const float dd = fmaxf(dm, -1e4f);
+        u2 = f2_fma(u2, f2(f, f), f2_mul(s2, f2(dd, dd)));
+      }
+      const uint64_t nm = f2(-m0, -m0);
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        accumulate<T, kReads>(q[i], nm, c2, s2, u2);
+    }
     float s0, s1, u0, u1;
     f2_split(s2, s0, s1);
     f2_split(u2, u0, u1);
-    st.s = s0 + s1;
-    st.u = u0 + u1;
+    st = Stat{mine, s0 + s1, u0 + u1};
   }
   st = warp_combine(st, a.c);
   uint32_t *gmax = reinterpret_cast<uint32_t *>(smem + p.l.gmax);
   uint32_t *misc = reinterpret_cast<uint32_t *>(smem + p.l.misc);
-  // maxima of groups of threads (4 lanes each when that leaves enough groups)
-  [[maybe_unused]] const bool quads = NT >= 128 && p.top_k <= NT / 8;
-  [[maybe_unused]] const int groups = quads ? NT / 4 : NT;
   if constexpr (MODE == kReadTop) {
-    uint32_t o = st.m < kInf ? order_of(mine) : 0;
-    if (quads) {
-      o = max(o, __shfl_xor_sync(~0u, o, 1));
-      o = max(o, __shfl_xor_sync(~0u, o, 2));
-      if ((tid & 3) == 0) gmax[tid >> 2] = o;
-    } else {
-      gmax[tid] = o;
+    // the largest logits of groups of neighbouring threads, to all CTAs
+    uint32_t o = order_of(mine);
+    const int size = (int)C * NT / p.l.groups;
+    for (int i = 1; i < size; i *= 2)
+      o = max(o, __shfl_xor_sync(~0u, o, i));
+    if (C > 1) cluster_wait();
+    if (tid % size == 0) {
+      uint32_t *to = gmax + ((int)rank * NT + tid) / size;
+      if (C > 1) {
+        for (uint32_t r = 0; r < C; ++r)
+          peer_store(peer_addr(to, r), __uint_as_float(o));
+      } else {
+        *to = o;
+      }
     }
     if (tid == 0) misc[0] = 0;  // candidates
   }
-  if constexpr (!kWarp) {
+  {
     float *part = reinterpret_cast<float *>(smem + p.l.stats);
     const int mine_at = ((int)rank * kWarps + warp) * 4;
     if (C > 1) {
-      cluster_wait();
+      if (MODE != kReadTop) cluster_wait();
       if (lane < (int)C) {
         const uint32_t to = peer_addr(part + mine_at, lane);
         peer_store(to, st.m);
@@ -553,150 +621,154 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT) k_team(TeamArgs p) {
       st.u += v.u;
     }
     st = warp_combine(st, a.c);
-  } else {
-    __syncwarp();
   }
-  const float m = st.m, s = st.s;
-  const bool bad = !(m < kInf) || (MODE >= kLoss && !(ym < kInf));
-  const bool empty = m == -kInf;
-  const float ln_s = logf(s);
+  RowEnd end(st, a.inv_t);
+  if (!kReads) end.bad |= !(ym < kInf);
+  const float m = end.m, s = end.s;
+  const bool bad = end.bad, empty = end.empty;
 
-  if constexpr (MODE == kRead || MODE == kReadTop) {
-    if (leader && tid == 0) {
-      const float h = bad ? nan : empty ? 0.0f : ln_s - kLn2 * st.u / s;
-      if (p.o.entropy) p.o.entropy[row] = h;
-      if (p.o.logprob) {
-        float lp = nan;
-        if (!bad && tok < a.classes)
-          lp = empty ? -kInf : (tok_x - m) * a.inv_t - ln_s;
-        p.o.logprob[row] = lp;
-      }
-      if (p.o.stats) {
-        float *so = p.o.stats + (int64_t)row * 3;
-        so[0] = bad ? nan : m;
-        so[1] = bad ? nan : empty ? 0.0f : s;
-        so[2] = h;
-      }
-    }
-  }
+  if constexpr (kReads)
+    if (leader && tid == 0) write_read(p.o, row, end, tok_x, tok < a.classes);
 
   if constexpr (MODE == kReadTop) {
-    // ---- alternatives.  The K-th largest of the groups' maxima is a lower
-    // bound of the slab's K-th largest logit, and few logits lie above it.
+    // ---- alternatives.  A value that at least K groups' maxima reach is a
+    // lower bound of the K-th largest logit, and few logits lie above it.
     const int K = p.top_k;
     int32_t *ids = p.o.top_ids + (int64_t)row * K;
     float *lps = p.o.top_logprobs + (int64_t)row * K;
     auto put = [&](int at, uint64_t key) {
       ids[at] = key ? class_of(key) : -1;
-      lps[at] = bad   ? nan
-                : key ? (value_of((uint32_t)(key >> 32)) - m) * a.inv_t - ln_s
-                      : -kInf;
+      lps[at] = bad ? nan : key ? end.logp(value_of((uint32_t)(key >> 32))) : -kInf;
     };
     if (bad || empty) {  // the same in all CTAs of the row
       if (leader)
         for (int k = tid; k < K; k += NT) put(k, 0);
       return;
     }
-    uint64_t *cand = reinterpret_cast<uint64_t *>(smem + p.l.cand);
-    if (tid < groups) {
-      const uint32_t v = gmax[tid];
-      int r = 0;
-      for (int j = 0; j < groups; j += 4) {
-        const uint4 q = *reinterpret_cast<const uint4 *>(gmax + j);
-        r += q.x > v || (q.x == v && j < tid);
-        r += q.y > v || (q.y == v && j + 1 < tid);
-        r += q.z > v || (q.z == v && j + 2 < tid);
-        r += q.w > v || (q.w == v && j + 3 < tid);
-      }
-      if (r == K - 1) misc[1] = max(v, kLowestOrder);
-    }
-    team_sync();
-    const uint32_t tau = misc[1];
-    const uint32_t my_order = order_of(mine);
-    // keys at or above `least` into cand (those that fit); their number
-    auto collect = [&](uint64_t least) {
-      if ((((uint64_t)my_order << 32) | 0xFFFFFFFFu) >= least) {
-        const float floor = value_of((uint32_t)(least >> 32));
-        for (int g = tid; g < G; g += NT) {
-          const uint4 q = slab[g];
-          GranuleMax<T> t;
-          t.clear();
-          t.add(q);
-          if (!(t.get() >= floor)) continue;
+    if (warp == 0) {
+      // the largest such value with its low 16 bits zero (all there is to a
+      // 16-bit logit), by halving; each lane holds 8 of the maxima
+      uint32_t v[kMaxGroups / 32], t = 0;
 #pragma unroll
-          for (int i = 0; i < E; ++i) {
+      for (int i = 0; i < kMaxGroups / 32; ++i)
+        v[i] = lane + 32 * i < p.l.groups ? gmax[lane + 32 * i] : 0;
+      for (uint32_t b = 1u << 31; b >= 1u << 16; b >>= 1) {
+        const uint32_t up = t | b;
+        uint32_t c = 0;
+#pragma unroll
+        for (int i = 0; i < kMaxGroups / 32; ++i) c += v[i] >= up;
+        if (__reduce_add_sync(~0u, c) >= (uint32_t)K) t = up;
+      }
+      if (lane == 0) misc[1] = max(t, kLowestOrder);
+    }
+    __syncthreads();
+    const uint32_t tau = misc[1];
+    uint64_t *cand = reinterpret_cast<uint64_t *>(smem + p.l.cand);
+    uint32_t *counts = misc + 4;
+    const uint32_t my_order = order_of(mine);
+    // Keys at or above `least`: those that fit go to this CTA's part of the
+    // first CTA's buffer; returns their number over the team, or a large number
+    // if a part overflowed.
+    int round = 0;
+    auto collect = [&](uint64_t least) {
+      const float floor = value_of((uint32_t)(least >> 32));
+      uint64_t *part = cand + (int)rank * p.l.cap;
+      const uint32_t to = C > 1 ? peer_addr(part, 0) : smem_addr(part);
+      // The warp goes together through the granules of each thread that has
+      // such a key: lanes 2 i and 2 i + 1 take the halves of granule i.
+      uint32_t have = __ballot_sync(
+          ~0u, (((uint64_t)my_order << 32) | 0xFFFFFFFFu) >= least);
+      while (have) {
+        const int src = __ffs(have) - 1;
+        have &= have - 1;
+        for (int g = warp * 32 + src + NT * (lane >> 1); g < G; g += NT * 16) {
+          const uint2 q = reinterpret_cast<const uint2 *>(slab + g)[lane & 1];
+          const uint4 q4{q.x, q.y, 0, 0};
+#pragma unroll
+          for (int i = 0; i < E / 2; ++i) {
             float f[2];
-            f2_split(pair_of<T>(q, i >> 1), f[0], f[1]);
+            f2_split(pair_of<T>(q4, i >> 1), f[0], f[1]);
             const float v = f[i & 1];
             if (v >= floor) {
-              const uint64_t key = key_of(v, first + g * E + i - mis);
+              const uint64_t key =
+                  key_of(v, first + g * E + (lane & 1) * (E / 2) + i - mis);
               if (key >= least) {
                 const uint32_t at = atomicAdd(misc, 1u);
-                if (at < (uint32_t)p.l.cap) cand[at] = key;
+                if (at < (uint32_t)p.l.cap) {
+                  if (C > 1)
+                    peer_store(to + at * 8, key);
+                  else
+                    part[at] = key;
+                }
               }
             }
           }
         }
       }
-      team_sync();
-      const int count = (int)misc[0];
-      team_sync();
-      return count;
-    };
-    int M = collect((uint64_t)tau << 32);
-    // Rows with thousands of equal or regularly placed values overflow the
-    // buffer: halve the interval of keys (which are distinct) until between K
-    // and `cap` of them are left.
-    // (64 halvings use the interval up.)
-    uint64_t lo = (uint64_t)tau << 32, hi = ~0ull;
-    for (int i = 0, c = M; i < 64 && (c > p.l.cap || c < K) && M > p.l.cap; ++i) {
-      const uint64_t mid = lo + ((hi - lo) >> 1);
+      __syncthreads();
+      if (C == 1) {
+        const int M = (int)misc[0];
+        counts[0] = M;
+        __syncthreads();
+        if (tid == 0) misc[0] = 0;
+        return M;
+      }
+      // two sets of counts in turn: one is written while the other is read
+      uint32_t *now = counts + (round++ & 1) * kMaxCluster;
+      if (tid < (int)C)
+        peer_store(peer_addr(now + rank, tid), __uint_as_float(misc[0]));
+      cluster_arrive();
+      cluster_wait();
       if (tid == 0) misc[0] = 0;
-      team_sync();
-      c = collect(mid);
+      int M = 0, most = 0;
+      for (uint32_t r = 0; r < C; ++r) {
+        M += (int)now[r];
+        most = max(most, (int)now[r]);
+      }
+      return most > p.l.cap ? 0x7FFFFFFF : M;
+    };
+    const int limit = C > 1 ? p.l.cap * 2 : p.l.cap;  // the first CTA ranks them
+    int M = collect((uint64_t)tau << 32);
+    // Rows with many equal or regularly placed values overflow the buffers:
+    // halve the interval of keys (which are distinct) until few enough, but K
+    // at least, are left.  64 halvings use the interval up.
+    uint64_t lo = (uint64_t)tau << 32, hi = ~0ull;
+    for (int i = 0; i < 64 && M > limit; ++i) {
+      const uint64_t mid = lo + ((hi - lo) >> 1);
+      __syncthreads();
+      const int c = collect(mid);
       (c < K ? hi : lo) = mid;
       if (c >= K) M = c;
     }
-    M = min(M, p.l.cap);
-    uint64_t *merge = reinterpret_cast<uint64_t *>(smem + p.l.merge);
-    auto keep = [&](int at, uint64_t key) {
-      if (C > 1)
-        peer_store(peer_addr(merge + rank * K + at, 0), key);
-      else
-        put(at, key);
-    };
-    for (int i = tid; i < M; i += NT) {
-      const uint64_t key = cand[i];
-      int r = 0;
-      for (int j = 0; j < M; ++j) r += cand[j] > key;
-      if (r < K) keep(r, key);
-    }
-    for (int k = M + tid; k < K; k += NT) keep(k, 0);
-    if (C > 1) {
-      cluster_arrive();
-      cluster_wait();
-      if (!leader) return;
-      const int all = (int)C * K;
-      for (int i = tid; i < all; i += NT) {
-        const uint64_t key = merge[i];
-        int r = 0;
-        for (int j = 0; j < all; ++j) {
-          const uint64_t q = merge[j];
-          r += q > key || (q == key && j < i);  // 0 may be there many times
-        }
-        if (r < K) put(r, key);
+    if (!leader) return;  // nothing of this CTA is read from here on
+    const uint32_t *now = counts + ((round - 1) & 1) * kMaxCluster;
+    if (C == 1) now = counts;
+    auto held = [&](uint32_t r) { return min((int)now[r], p.l.cap); };
+    int all = 0;
+    for (uint32_t r = 0; r < C; ++r) all += held(r);
+    for (int i = tid; i < all; i += NT) {
+      int at = i;
+      uint32_t r = 0;
+      for (; at >= held(r); ++r) at -= held(r);
+      const uint64_t key = cand[(int)r * p.l.cap + at];
+      int above = 0;
+      for (uint32_t q = 0; q < C; ++q) {
+        const uint64_t *of = cand + (int)q * p.l.cap;
+        const int many = held(q);
+        for (int j = 0; j < many; ++j) above += of[j] > key;
       }
+      if (above < K) put(above, key);
     }
+    for (int k = all + tid; k < K; k += NT) put(k, 0);
   }
 
-  if constexpr (MODE == kLoss || MODE == kLossGrad) {
+  if constexpr (!kReads) {
     if (leader && warp == 0) {
       float l = 0.0f;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (tq[i] > 0.0f)
-          l += empty ? kInf
-                     : tq[i] * ((ty[i] - ln_ys) - ((xk[i] - m) * a.inv_t - ln_s));
+          l += empty ? kInf : tq[i] * ((ty[i] - ln_ys) - end.logp(xk[i]));
       for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
       if (lane == 0) p.loss[row] = bad ? nan : a.t * a.t * l;
     }
@@ -710,6 +782,7 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT) k_team(TeamArgs p) {
     const int dm = (int)((uintptr_t)d & 15) / (int)sizeof(T);
     if (dm == mis) {
       uint4 *dst = reinterpret_cast<uint4 *>(d - dm);
+#pragma unroll 2
       for (int g = tid; g < G; g += NT) {
         const uint4 q = slab[g];
         float r[E];
@@ -720,15 +793,7 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT) k_team(TeamArgs p) {
           f2_split(f2_mul(f2(ex2(u), ex2(v)), w2), r[2 * i], r[2 * i + 1]);
         }
         if (g * E >= mis && (g + 1) * E <= mis + n) {
-          uint4 out;
-          if constexpr (sizeof(T) == 4) {
-            out = uint4{__float_as_uint(r[0]), __float_as_uint(r[1]),
-                        __float_as_uint(r[2]), __float_as_uint(r[3])};
-          } else {
-            out = uint4{pack2<T>(r[0], r[1]), pack2<T>(r[2], r[3]),
-                        pack2<T>(r[4], r[5]), pack2<T>(r[6], r[7])};
-          }
-          dst[g] = out;
+          dst[g] = pack_granule<T>(r);
         } else {
 #pragma unroll
           for (int j = 0; j < E; ++j) {
@@ -744,7 +809,7 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT) k_team(TeamArgs p) {
       for (int e = tid; e < n; e += NT)
         d[e] = from_f<T>(ex2((to_f(sx[e]) - m0) * a.c) * ws);
     }
-    team_sync();  // an entry's element is written again, after its first value
+    __syncthreads();  // an entry's element is written again, after its first value
     if (!bad && !empty) {
       for (int k = tid; k < p.te.k; k += NT) {
         const int id = sid[k] - first;
@@ -758,10 +823,326 @@ __global__ void __launch_bounds__(NT == 32 ? 128 : NT) k_team(TeamArgs p) {
   }
 }
 
+// ------------------------------------------------------------ gradient terms
+// d = -p (g + b (log p + H)) + g at the token
+//   = e^t (k0 + k1 t log2(e)) with t = (x - m) / T
+struct BackRow {
+  float m, g, k0, k1;
+  int tok;
+  bool idle;
+  __device__ __forceinline__ BackRow(const RowArgs &a, const void *tokens,
+                                     int itype, const float *stats,
+                                     const float *d_logprob,
+                                     const float *d_entropy, uint32_t row) {
+    const float *st = stats + (int64_t)row * 3;
+    const int64_t t = tokens ? load_index(tokens, row, itype) : 0;
+    m = st[0];
+    const float s = st[1], h = st[2];
+    g = d_logprob ? d_logprob[row] * a.inv_t : 0.0f;
+    const float b = d_entropy ? d_entropy[row] * a.inv_t : 0.0f;
+    idle = s == 0.0f || t < 0;
+    if (t >= a.classes) g = not_a_number();
+    tok = tokens && t < a.classes ? (int)t : -1;
+    const float inv_s = 1.0f / s;
+    k1 = -b * kLn2 * inv_s;
+    k0 = -(b == 0.0f ? g : g + b * (h - logf(s))) * inv_s;
+  }
+  // element e of value v
+  __device__ __forceinline__ float at(float v, int e, float c) const {
+    const float t = (v - m) * c;
+    // where t is -inf e^t is 0: a finite t keeps 0 * t from being NaN
+    const float r = ex2(t) * fmaf(k1, fmaxf(t, -1e4f), k0);
+    return idle ? 0.0f : e == tok ? r + g : r;
+  }
+};
+
+// ------------------------------------------------------------ lanes a row
+// Narrow rows: 1 to 32 neighbouring lanes hold a row in registers, NG granules
+// each (granule lane + lanes * j), and reduce over one another with shuffles.
+// There is no shared memory but for a teacher's entries, and nothing is read
+// or written twice.
+struct NarrowArgs {
+  RowArgs a;
+  const void *tokens;
+  int itype, top_k;
+  LogprobOut o;
+  const float *stats, *d_logprob, *d_entropy;  // backward
+  Teacher te;
+  const float *row_weight;
+  float weight;
+  float *loss;
+  void *dx;
+  int64_t d_stride;
+  int lanes;
+  // the logits' memory, inside which a whole granule may be read although it
+  // holds elements of other rows (null where those may be written meanwhile)
+  const void *lo, *hi;
+};
+
+template <class T, int NG, int MODE>
+__global__ void __launch_bounds__(128) k_narrow(NarrowArgs p) {
+  extern __shared__ float entries[];
+  constexpr int E = kElems<T>;
+  constexpr bool kReads = MODE == kRead || MODE == kReadTop;
+  constexpr bool kTeacher = MODE == kLoss || MODE == kLossGrad;
+  const RowArgs &a = p.a;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int L = p.lanes, l = lane & (L - 1), V = a.classes;
+  const uint32_t want = (blockIdx.x * 4 + warp) * (32 / L) + lane / L;
+  const bool on = want < a.rows;  // lanes of no row repeat the last one
+  const uint32_t row = on ? want : a.rows - 1;
+  const float nan = not_a_number();
+  auto group_max = [&](float v) {
+    for (int o = 1; o < L; o *= 2) v = max_nan(v, __shfl_xor_sync(~0u, v, o));
+    return v;
+  };
+  auto group_sum = [&](float v) {
+    for (int o = 1; o < L; o *= 2) v += __shfl_xor_sync(~0u, v, o);
+    return v;
+  };
+
+  // ---- the row
+  const T *x = static_cast<const T *>(a.x) + (int64_t)row * a.stride;
+  const int mis = (int)((uintptr_t)x & 15) / (int)sizeof(T);
+  uint4 q[NG];
+  {
+    const uint4 *src = reinterpret_cast<const uint4 *>(x - mis);
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      const int g = l + L * j, e0 = g * E - mis;
+      q[j] = no_logits<T>();
+      if (e0 >= V) continue;
+      if ((e0 >= 0 && e0 + E <= V) ||
+          (p.lo && src + g >= p.lo && src + g + 1 <= p.hi)) {
+        q[j] = src[g];
+      } else {
+        T v[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+          v[i] = e0 + i >= 0 && e0 + i < V ? x[e0 + i] : from_f<T>(-kInf);
+        q[j] = *reinterpret_cast<const uint4 *>(v);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      const int e0 = (l + L * j) * E - mis;
+      if (e0 >= V || (e0 >= 0 && e0 + E <= V)) continue;
+      T v[E];
+      *reinterpret_cast<uint4 *>(v) = q[j];
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (e0 + i < 0 || e0 + i >= V) v[i] = from_f<T>(-kInf);
+      q[j] = *reinterpret_cast<const uint4 *>(v);
+    }
+  }
+  T *d = MODE == kLossGrad || MODE == kBack
+             ? static_cast<T *>(p.dx) + (int64_t)row * p.d_stride
+             : nullptr;
+  // writes f(value, element) of every element
+  auto write_rows = [&](auto &&f) {
+    const int dm = (int)((uintptr_t)d & 15) / (int)sizeof(T);
+    uint4 *dst = reinterpret_cast<uint4 *>(d - dm);
+    if (!on) return;
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      const int g = l + L * j, e0 = g * E - mis;
+      if (e0 >= V) continue;
+      float r[E];
+#pragma unroll
+      for (int i = 0; i < E / 2; ++i) {
+        float u, v;
+        f2_split(pair_of<T>(q[j], i), u, v);
+        r[2 * i] = f(u, e0 + 2 * i);
+        r[2 * i + 1] = f(v, e0 + 2 * i + 1);
+      }
+      if (dm == mis && e0 >= 0 && e0 + E <= V) {
+        dst[g] = pack_granule<T>(r);
+      } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+          if (e0 + i >= 0 && e0 + i < V) d[e0 + i] = from_f<T>(r[i]);
+      }
+    }
+  };
+
+  if constexpr (MODE == kBack) {
+    const BackRow b(a, p.tokens, p.itype, p.stats, p.d_logprob, p.d_entropy, row);
+    write_rows([&](float v, int e) { return b.at(v, e, a.c); });
+    return;
+  }
+
+  // ---- the teacher's entries, entry l + lanes * i of a row by lane l
+  const int K = kTeacher ? p.te.k : 0;
+  float *sq = entries + (warp * (32 / L) + lane / L) * K * 3;  // e^(y - max)
+  float *sy = sq + K;                                          // y, then own d
+  int32_t *sid = reinterpret_cast<int32_t *>(sy + K);
+  float ym = 0.0f, ys = 1.0f;
+  int64_t tok = 0;
+  bool idle = false;
+  float tok_x = 0.0f;
+  if constexpr (kTeacher) {
+    ym = -kInf;
+    for (int k = l; k < K; k += L) {
+      const int64_t at = (int64_t)row * K + k;
+      const int64_t id = load_index(p.te.ids, at, p.te.itype);
+      float y = load_value(p.te.logits, at, p.te.dtype);
+      const bool out = id < 0 || y == -kInf;  // left out
+      if (!out && id >= V) y = nan;
+      sid[k] = out ? -1 : id < V ? (int32_t)id : 0;
+      sy[k] = out ? -kInf : y;
+      ym = max_nan(ym, sy[k]);
+    }
+    ym = group_max(ym);
+    idle = ym == -kInf;
+    ys = 0.0f;
+    for (int k = l; k < K; k += L) {
+      const float y = sid[k] >= 0 ? (sy[k] - ym) * a.inv_t : -kInf;
+      sy[k] = y;
+      sq[k] = expf(y);
+      ys += sq[k];
+    }
+    ys = group_sum(ys);
+  } else {
+    if (p.tokens) tok = load_index(p.tokens, row, p.itype);
+    idle = tok < 0;
+    if (l == 0 && p.o.logprob && !idle && tok < V) tok_x = to_f(x[tok]);
+  }
+
+  // ---- statistics
+  GranuleMax<T> gm;
+  gm.clear();
+#pragma unroll
+  for (int j = 0; j < NG; ++j) gm.add(q[j]);
+  Stat st;
+  st.m = group_max(gm.get());
+  {
+    const float m0 = st.m == -kInf ? 0.0f : st.m;
+    const uint64_t nm = f2(-m0, -m0), c2 = f2(a.c, a.c);
+    uint64_t s2 = 0, u2 = 0;
+#pragma unroll
+    for (int j = 0; j < NG; ++j)
+      if (l + L * j < (mis + V + E - 1) / E)
+        accumulate<T, kReads>(q[j], nm, c2, s2, u2);
+    float s0, s1, u0, u1;
+    f2_split(s2, s0, s1);
+    f2_split(u2, u0, u1);
+    st.s = group_sum(s0 + s1);
+    st.u = kReads ? group_sum(u0 + u1) : 0.0f;
+  }
+  RowEnd end(st, a.inv_t);
+  if (kTeacher) end.bad |= !(ym < kInf);
+
+  if constexpr (kReads) {
+    if (l == 0 && on) {
+      if (idle)
+        write_read_padding(p.o, row);
+      else
+        write_read(p.o, row, end, tok_x, tok < V);
+    }
+  }
+  if constexpr (MODE == kReadTop) {
+    // one alternative after the other: the largest value, of the lowest class
+    int32_t *ids = p.o.top_ids + (int64_t)row * p.top_k;
+    float *lps = p.o.top_logprobs + (int64_t)row * p.top_k;
+    float best[NG];  // maximum of each granule
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      GranuleMax<T> t;
+      t.clear();
+      t.add(q[j]);
+      best[j] = end.bad || idle ? -kInf : t.get();
+    }
+    for (int k = 0; k < p.top_k; ++k) {
+      float v = best[0];
+      uint4 w = q[0];
+      int at = 0;
+#pragma unroll
+      for (int j = 1; j < NG; ++j)
+        if (best[j] > v) {
+          v = best[j];
+          w = q[j];
+          at = j;
+        }
+      const float top = group_max(v);
+      int cls = 0x7FFFFFFF, where = 0;
+      if (v == top && top > -kInf) {
+#pragma unroll
+        for (int i = E - 1; i >= 0; --i) {
+          float f[2];
+          f2_split(pair_of<T>(w, i >> 1), f[0], f[1]);
+          if (f[i & 1] == v) where = i;
+        }
+        cls = (l + L * at) * E + where - mis;
+      }
+      int first = cls;
+      for (int o = 1; o < L; o *= 2)
+        first = min(first, __shfl_xor_sync(~0u, first, o));
+      if (cls == first && top > -kInf) {  // taken: the granule without it
+        T t[E];
+        *reinterpret_cast<uint4 *>(t) = w;
+        float rest = -kInf;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          if (i == where) t[i] = from_f<T>(-kInf);
+          rest = fmaxf(rest, to_f(t[i]));
+        }
+        w = *reinterpret_cast<const uint4 *>(t);
+#pragma unroll
+        for (int j = 0; j < NG; ++j)
+          if (j == at) {
+            q[j] = w;
+            best[j] = rest;
+          }
+      }
+      if (l == 0 && on) {
+        const bool some = top > -kInf;
+        ids[k] = some ? first : -1;
+        lps[k] = some ? end.logp(top) : end.bad && !idle ? nan : -kInf;
+      }
+    }
+  }
+  if constexpr (kTeacher) {
+    const float ln_ys = logf(ys), inv_ys = 1.0f / ys;
+    const float w = (p.row_weight ? p.row_weight[row] : p.weight) * a.t;
+    float loss = 0.0f;
+    __syncwarp();
+    if (!idle)
+      for (int k = l; k < K; k += L) {
+        const float e = sq[k];
+        if (sid[k] < 0) continue;
+        const float xv = to_f(x[sid[k]]);
+        if (e > 0.0f)
+          loss += end.empty ? kInf
+                            : e / ys * ((sy[k] - ln_ys) - end.logp(xv));
+        if constexpr (MODE == kLossGrad) {
+          float both = 0.0f;  // entries of one class add up
+          for (int j = 0; j < K; ++j) both += sid[j] == sid[k] ? sq[j] : 0.0f;
+          sy[k] = w * (ex2((xv - end.m) * a.c) / end.s - both * inv_ys);
+        }
+      }
+    loss = group_sum(loss);
+    if (l == 0 && on)
+      p.loss[row] = idle ? 0.0f : end.bad ? nan : a.t * a.t * loss;
+    if constexpr (MODE == kLossGrad) {
+      const bool zero = idle || (end.empty && !end.bad);
+      const float ws = zero ? 0.0f : end.bad ? nan : w / end.s;
+      const float m0 = zero ? 0.0f : end.m;
+      __syncwarp();  // every lane has read what the row's lanes now write
+      write_rows([&](float v, int) {
+        return zero ? 0.0f : ex2((v - m0) * a.c) * ws;
+      });
+      __syncwarp();  // an entry's element is written again
+      if (on && !zero && !end.bad)
+        for (int k = l; k < K; k += L)
+          if (sid[k] >= 0) d[sid[k]] = from_f<T>(sy[k]);
+    }
+  }
+}
+
 // ------------------------------------------------------------ backward
-// Element by element from the saved statistics; a warp takes a run of 32 x
-// kRun granules of one row.  Bound by the memory: the logits in, the gradient
-// out.
+// Wide rows, element by element from the saved statistics; a warp takes a run
+// of 32 x kRun granules of one row.  Bound by the memory: the logits in, the
+// gradient out.
 constexpr int kRun = 8;
 
 template <class T>
@@ -771,31 +1152,13 @@ __global__ void __launch_bounds__(256)
                int64_t d_stride, uint32_t runs) {
   constexpr int E = kElems<T>;
   const int lane = threadIdx.x & 31;
-  const uint64_t unit = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const uint32_t row = (uint32_t)(unit / runs);
+  const uint32_t unit = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const uint32_t row = unit / runs;
   if (row >= a.rows) return;
-  const int run = (int)(unit % runs);
+  const int run = (int)(unit - row * runs);
   const T *x = static_cast<const T *>(a.x) + (int64_t)row * a.stride;
   T *d = dx + (int64_t)row * d_stride;
-  const int64_t tok = tokens ? load_index(tokens, row, itype) : -1;
-  const float m = stats[(int64_t)row * 3], s = stats[(int64_t)row * 3 + 1],
-              h = stats[(int64_t)row * 3 + 2];
-  float g = d_logprob ? d_logprob[row] * a.inv_t : 0.0f;
-  const float b = d_entropy ? d_entropy[row] * a.inv_t : 0.0f;
-  if (tokens && tok >= a.classes) g = __int_as_float(0x7FFFFFFF);
-  const bool idle = s == 0.0f || (tokens && tok < 0);
-  const float inv_s = 1.0f / s;
-  // d = -p (g + b (t ln 2 - ln s + H)) = p (k0 + k1 t), t in units of log2(e)
-  const float k1 = -b * kLn2 * inv_s;
-  const float k0 = -(g + b * (h - logf(s))) * inv_s;
-  const bool plain = b == 0.0f;  // no 0 * inf from t = -inf then
-  auto grad = [&](float v, int e) {
-    const float t = (v - m) * a.c;
-    const float p = ex2(t);
-    float r = p * (plain ? k0 : k0 + k1 * fmaxf(t, -1e4f));
-    if (e == tok) r += g;
-    return idle ? 0.0f : r;
-  };
+  const BackRow b(a, tokens, itype, stats, d_logprob, d_entropy, row);
   const int mis = (int)((uintptr_t)x & 15) / (int)sizeof(T);
   const int dm = (int)((uintptr_t)d & 15) / (int)sizeof(T);
   const int V = a.classes;
@@ -806,37 +1169,28 @@ __global__ void __launch_bounds__(256)
     uint4 q[kRun];
 #pragma unroll
     for (int i = 0; i < kRun; ++i) {
-      const int gi = g0 + 32 * i;
+      const int g = g0 + 32 * i;
       q[i] = uint4{0, 0, 0, 0};
-      if (!idle && gi * E >= mis && (gi + 1) * E <= mis + V) q[i] = src[gi];
+      if (!b.idle && g * E >= mis && (g + 1) * E <= mis + V) q[i] = src[g];
     }
 #pragma unroll
     for (int i = 0; i < kRun; ++i) {
-      const int gi = g0 + 32 * i;
-      const int e0 = gi * E - mis;
+      const int g = g0 + 32 * i, e0 = g * E - mis;
       if (e0 >= 0 && e0 + E <= V) {
         float r[E];
 #pragma unroll
         for (int j = 0; j < E / 2; ++j) {
           float u, v;
           f2_split(pair_of<T>(q[i], j), u, v);
-          r[2 * j] = grad(u, e0 + 2 * j);
-          r[2 * j + 1] = grad(v, e0 + 2 * j + 1);
+          r[2 * j] = b.at(u, e0 + 2 * j, a.c);
+          r[2 * j + 1] = b.at(v, e0 + 2 * j + 1, a.c);
         }
-        uint4 out;
-        if constexpr (sizeof(T) == 4) {
-          out = uint4{__float_as_uint(r[0]), __float_as_uint(r[1]),
-                      __float_as_uint(r[2]), __float_as_uint(r[3])};
-        } else {
-          out = uint4{pack2<T>(r[0], r[1]), pack2<T>(r[2], r[3]),
-                      pack2<T>(r[4], r[5]), pack2<T>(r[6], r[7])};
-        }
-        dst[gi] = out;
+        dst[g] = pack_granule<T>(r);
       } else {
         for (int j = 0; j < E; ++j) {
           const int e = e0 + j;
           if (e >= 0 && e < V)
-            d[e] = from_f<T>(idle ? 0.0f : grad(to_f(x[e]), e));
+            d[e] = from_f<T>(b.idle ? 0.0f : b.at(to_f(x[e]), e, a.c));
         }
       }
     }
@@ -845,7 +1199,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll 8
     for (int i = 0; i < kRun * E; ++i) {
       const int e = e0 + 32 * i;
-      if (e < V) d[e] = from_f<T>(idle ? 0.0f : grad(to_f(x[e]), e));
+      if (e < V) d[e] = from_f<T>(b.idle ? 0.0f : b.at(to_f(x[e]), e, a.c));
     }
   }
 }
@@ -975,19 +1329,24 @@ void allow(K kernel, std::atomic<uint64_t> &done) {
   done.fetch_or(bit, std::memory_order_release);
 }
 
+void check_launch(cudaError_t e) {
+  if (e != cudaSuccess)
+    throw std::runtime_error(std::string("class-logit kernel: ") +
+                             cudaGetErrorString(e));
+}
+
 template <class T, int NT, int MODE>
 void launch_team_of(TeamArgs &p, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
   auto kernel = k_team<T, NT, MODE>;
   allow(kernel, done);
-  constexpr int teams = NT == 32 ? 4 : 1;
   const int granules = p.slab / kElems<T> + 1;
   p.l = team_layout(MODE, NT, p.cluster, MODE >= kLoss ? p.te.k : p.top_k,
                     granules);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((p.a.rows + teams - 1) / teams * p.cluster);
-  cfg.blockDim = dim3(NT * teams);
-  cfg.dynamicSmemBytes = (size_t)p.l.total * teams;
+  cfg.gridDim = dim3(p.a.rows * (uint32_t)p.cluster);
+  cfg.blockDim = dim3(NT);
+  cfg.dynamicSmemBytes = (size_t)p.l.total;
   cfg.stream = st;
   cudaLaunchAttribute at;
   if (p.cluster > 1) {
@@ -997,10 +1356,7 @@ void launch_team_of(TeamArgs &p, cudaStream_t st) {
     cfg.attrs = &at;
     cfg.numAttrs = 1;
   }
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
-  if (e != cudaSuccess)
-    throw std::runtime_error(std::string("class-logit kernel: ") +
-                             cudaGetErrorString(e));
+  check_launch(cudaLaunchKernelEx(&cfg, kernel, p));
 }
 
 // Threads and CTAs of a row.  Slabs of up to 64 KB leave three CTAs on an SM,
@@ -1011,7 +1367,6 @@ void launch_team(TeamArgs &p, cudaStream_t st) {
   constexpr int E = kElems<T>;
   const int64_t bytes = (int64_t)p.a.classes * (int)sizeof(T);
   const int sms = sm_count();
-  const int k = MODE == kReadTop ? p.top_k : 0;
   int c = 1;
   while (c < 8 && bytes > (int64_t)c * 64 * 1024) c *= 2;
   while (c < 8 && bytes >= (int64_t)c * 16 * 1024 &&
@@ -1020,13 +1375,52 @@ void launch_team(TeamArgs &p, cudaStream_t st) {
   if (bytes > 8 * 128 * 1024) c = 16;
   p.cluster = c;
   p.slab = ((p.a.classes + c - 1) / c + E - 1) / E * E;
+  p.eager = (int64_t)p.a.rows * c <= 2 * sms;
   const int granules = p.slab / E + 1;
-  if (c == 1 && granules <= 256 && k <= 32)
-    launch_team_of<T, 32, MODE>(p, st);
-  else if (granules <= 1024)
+  if (granules <= 1024 && (MODE != kReadTop || p.top_k <= 64))
     launch_team_of<T, 128, MODE>(p, st);
   else
     launch_team_of<T, 256, MODE>(p, st);
+}
+
+// Granules of the widest row when rows may start anywhere inside one.
+int granules_of(const RowArgs &a, int dtype) {
+  const int size = elem_size(dtype), e = 16 / size;
+  const bool aligned =
+      (uintptr_t)a.x % 16 == 0 && (a.rows == 1 || a.stride % e == 0);
+  return (a.classes + (aligned ? 0 : e - 1) + e - 1) / e;
+}
+constexpr int kNarrow = 256;  // granules of a narrow row
+
+template <class T, int NG, int MODE>
+void launch_narrow_of(NarrowArgs &p, cudaStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  auto kernel = k_narrow<T, NG, MODE>;
+  size_t smem = 0;
+  if (MODE == kLoss || MODE == kLossGrad) {
+    allow(kernel, done);
+    smem = (size_t)(128 / p.lanes) * p.te.k * 12;
+  }
+  const uint32_t rows = 128 / p.lanes;
+  kernel<<<(p.a.rows + rows - 1) / rows, 128, smem, st>>>(p);
+  check_launch(cudaGetLastError());
+}
+
+// Four granules a lane keep enough loads in flight and few lanes idle; eight
+// only where 32 lanes are not enough.
+template <class T, int MODE>
+void launch_narrow(NarrowArgs &p, int dtype, cudaStream_t st) {
+  const int g = granules_of(p.a, dtype);
+  p.lanes = 1;
+  while (p.lanes < 32 && p.lanes * 4 < g) p.lanes *= 2;
+  const bool in_place = p.dx == p.a.x;
+  p.lo = in_place ? nullptr : p.a.x;
+  p.hi = static_cast<const T *>(p.a.x) +
+         ((int64_t)(p.a.rows - 1) * p.a.stride + p.a.classes);
+  if (p.lanes * 4 >= g)
+    launch_narrow_of<T, 4, MODE>(p, st);
+  else
+    launch_narrow_of<T, 8, MODE>(p, st);
 }
 
 // Launches for rows [i, i + n) of all, n small enough for a grid.
@@ -1078,10 +1472,22 @@ int launch_token_logprobs(const tmnn_logits &x, const void *tokens,
     p.o.top_ids = top_k ? o.top_ids + (int64_t)i * top_k : nullptr;
     p.o.top_logprobs = top_k ? o.top_logprobs + (int64_t)i * top_k : nullptr;
     p.o.stats = o.stats ? o.stats + (int64_t)i * 3 : nullptr;
-    if (top_k)
+    if (granules_of(p.a, x.dtype) <= kNarrow) {
+      NarrowArgs q{};
+      q.a = p.a;
+      q.tokens = p.tokens;
+      q.itype = p.itype;
+      q.top_k = p.top_k;
+      q.o = p.o;
+      if (top_k)
+        BY_DTYPE(x.dtype, (launch_narrow<T, kReadTop>(q, x.dtype, st)));
+      else
+        BY_DTYPE(x.dtype, (launch_narrow<T, kRead>(q, x.dtype, st)));
+    } else if (top_k) {
       BY_DTYPE(x.dtype, (launch_team<T, kReadTop>(p, st)));
-    else
+    } else {
       BY_DTYPE(x.dtype, (launch_team<T, kRead>(p, st)));
+    }
   });
 }
 
@@ -1109,6 +1515,19 @@ int launch_token_logprobs_backward(const tmnn_logits &x, const void *tokens,
     b.x = at(x.data, (int64_t)i * x.row_stride * size);
     b.rows = n;
     const void *d = at(d_logits, (int64_t)i * d_stride * size);
+    if (granules_of(b, x.dtype) <= kNarrow) {
+      NarrowArgs q{};
+      q.a = b;
+      q.tokens = at(tokens, (int64_t)i * index_size(index_type));
+      q.itype = index_type;
+      q.stats = stats + (int64_t)i * 3;
+      q.d_logprob = d_logprob ? d_logprob + i : nullptr;
+      q.d_entropy = d_entropy ? d_entropy + i : nullptr;
+      q.dx = const_cast<void *>(d);
+      q.d_stride = d_stride;
+      BY_DTYPE(x.dtype, (launch_narrow<T, kBack>(q, x.dtype, st)));
+      return;
+    }
     const uint32_t grid = (uint32_t)(((uint64_t)n * runs + 7) / 8);
     BY_DTYPE(x.dtype,
              (k_backward<T><<<grid, 256, 0, st>>>(
@@ -1149,10 +1568,24 @@ int launch_distill(const tmnn_logits &x, const void *ids, int index_type,
     p.loss = loss + i;
     p.dx = const_cast<void *>(at(d_logits, (int64_t)i * d_stride * size));
     p.d_stride = d_stride;
-    if (d_logits)
+    if (granules_of(p.a, x.dtype) <= kNarrow) {
+      NarrowArgs q{};
+      q.a = p.a;
+      q.te = p.te;
+      q.row_weight = p.row_weight;
+      q.weight = weight;
+      q.loss = p.loss;
+      q.dx = p.dx;
+      q.d_stride = d_stride;
+      if (d_logits)
+        BY_DTYPE(x.dtype, (launch_narrow<T, kLossGrad>(q, x.dtype, st)));
+      else
+        BY_DTYPE(x.dtype, (launch_narrow<T, kLoss>(q, x.dtype, st)));
+    } else if (d_logits) {
       BY_DTYPE(x.dtype, (launch_team<T, kLossGrad>(p, st)));
-    else
+    } else {
       BY_DTYPE(x.dtype, (launch_team<T, kLoss>(p, st)));
+    }
   });
 }
 
