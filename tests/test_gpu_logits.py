@@ -65,11 +65,12 @@ def make_tokens(n, V, seed, dtype="int64"):
     return torch.from_numpy(tok).to("cuda").to(getattr(torch, dtype)), tok
 
 
+# 300 rows and more: wide rows in numbers that fill the SMs
 SIZES = [(1, 1), (3, 2), (40, 3), (13, 19), (70000, 5), (33, 31), (300, 64),
          (12, 65), (50, 127), (11, 257), (64, 1000), (5, 1023), (17, 1024),
          (17, 1025), (10, 2047), (12, 2311), (10, 4097), (21, 8192), (2, 32768),
          (11, 32003), (300, 5000), (1, 131072), (10, 50021), (3, 262143),
-         (12, 131071), (1, 524288)]
+         (12, 131071), (1, 524288), (320, 9001), (305, 33000), (600, 2500)]
 DTYPES = ["f32", "bf16", "fp16"]
 
 
@@ -127,7 +128,7 @@ def test_many_alternatives(V, k):
     import torch
     import tmnn_b200 as t
     rng = np.random.default_rng(V + k)
-    x = np.zeros((9, V))
+    x = np.zeros((11, V))
     x[0] = rng.integers(0, 4, V)
     x[1] = np.arange(V) % 2048
     x[2] = rng.normal(size=V)
@@ -140,16 +141,25 @@ def test_many_alternatives(V, k):
     x[6, rng.permutation(V)[:max(1, k // 2)]] = 2.5
     x[7] = np.arange(V) / 64.0
     x[8, : V // 2] = rng.normal(size=V // 2) + 9
+    x[9] = -np.inf
+    x[9, V // 2:] = LOWEST["f32"]
+    x[10] = 0.5
     for dtype in DTYPES:
+        x[9, V // 2:] = LOWEST[dtype]
         c = torch.from_numpy(x).to("cuda").to(_t(dtype))
         xd = c.double().cpu().numpy()
         r = t.token_logprobs(c, top_k=k)
         _, _, ids, top, _, rows = ref.token_logprobs(xd, 1.0, None, k)
+        # the same rows in numbers that fill the SMs
+        many = t.token_logprobs(c.repeat(60, 1), top_k=k)
+        assert torch.equal(many.top_ids, r.top_ids.repeat(60, 1))
         assert np.array_equal(r.top_ids.cpu().numpy(), ids), dtype
         dk = np.take_along_axis(rows.d, np.clip(ids, 0, V - 1), 1)
         tol = 1.1 * (ref.U * 3 * dk + rows.tol_ln[:, None] + 2 * ref.U *
                      np.abs(np.where(np.isfinite(top), top, 0))) + 1e-37
         ref.assert_close(r.top_logprobs.cpu(), top, tol, dtype)
+        ref.assert_close(many.top_logprobs.cpu(), np.tile(top, (60, 1)),
+                         np.tile(tol, (60, 1)), dtype)
 
 
 def _round(d, tol, dtype):

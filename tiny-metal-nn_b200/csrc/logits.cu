@@ -23,7 +23,7 @@ using namespace tmnn;
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
+
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kInf = __builtin_huge_valf();
 
@@ -258,6 +258,11 @@ __device__ __forceinline__ void copies_done() {
 }
 __device__ __forceinline__ void cluster_arrive() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+// Says that this CTA runs; its peers may write to it when all have said so.
+// Orders no memory (that costs a fence).
+__device__ __forceinline__ void cluster_arrive_started() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void cluster_wait() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -496,7 +501,7 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
     copies_done();
     return;  // all CTAs of the cluster alike
   }
-  if (C > 1) cluster_arrive();  // waited for before the first peer store
+  if (C > 1) cluster_arrive_started();
   if (!p.eager) load();
 
   [[maybe_unused]] float xk[4], tok_x = 0.0f;
@@ -820,6 +825,303 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
         d[id] = from_f<T>(w * (ex2((to_f(sx[id]) - m) * a.c) / s - both));
       }
     }
+  }
+}
+
+// ------------------------------------------------------------ a CTA a row
+// Enough wide rows to fill the SMs, and no gradient: a CTA streams its row
+// through registers, four granules a thread at a time with the next four in
+// flight, and nothing of the row is kept.  One exchange at the end.
+//
+// For the alternatives each thread notes the maximum of every run of granules
+// it read.  The K-th largest of the threads' maxima is a lower bound of the
+// row's K-th largest logit; the few runs that reach it are read once more (out
+// of the L2) and their logits above it ranked.
+constexpr int kRuns = 16;             // runs a thread
+constexpr int kPicked = 4 * kMaxTop;  // runs read again, logits ranked
+
+struct StreamArgs {
+  RowArgs a;
+  const void *tokens;
+  int itype, top_k;
+  LogprobOut o;
+  Teacher te;
+  float *loss;
+};
+
+// The largest value, of those with the low 16 bits zero (all there is to a
+// 16-bit logit), that at least K of N orders reach; with none, the order of the
+// lowest logit.  One warp; halving from the top bit.
+template <int N>
+__device__ __forceinline__ uint32_t reached_by(int K, const uint32_t *values) {
+  uint32_t v[N / 32], t = 0;
+#pragma unroll
+  for (int i = 0; i < N / 32; ++i) v[i] = values[(threadIdx.x & 31) + 32 * i];
+  for (uint32_t b = 1u << 31; b >= 1u << 16; b >>= 1) {
+    const uint32_t up = t | b;
+    uint32_t c = 0;
+#pragma unroll
+    for (int i = 0; i < N / 32; ++i) c += v[i] >= up;
+    if (__reduce_add_sync(~0u, c) >= (uint32_t)K) t = up;
+  }
+  return max(t, kLowestOrder);
+}
+template <class T, int NT, int MODE>
+__global__ void __launch_bounds__(NT) k_stream(StreamArgs p) {
+  constexpr int E = kElems<T>, kBatch = 4, kWarps = NT / 32;
+  constexpr bool kReads = MODE == kRead || MODE == kReadTop;
+  constexpr bool kTop = MODE == kReadTop;
+  __shared__ float part[kWarps * 3];
+  __shared__ float run_max[kTop ? kRuns * NT : 1];
+  __shared__ uint32_t gmax[kTop ? NT : 1], runs[kTop ? kPicked : 1];
+  __shared__ uint64_t picked[kTop ? kPicked : 1];
+  __shared__ uint32_t misc[4];  // runs to read, tau, logits picked
+  const RowArgs &a = p.a;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t row = blockIdx.x;
+  const int V = a.classes;
+  const float nan = not_a_number();
+
+  // ---- `head` elements up to a 16-byte boundary, whole granules, the rest
+  const T *x = static_cast<const T *>(a.x) + (int64_t)row * a.stride;
+  const int mis = (int)((uintptr_t)x & 15) / (int)sizeof(T);
+  const int head = min(mis ? E - mis : 0, V), F = (V - head) / E;
+  const uint4 *src = reinterpret_cast<const uint4 *>(x + head);
+  uint4 q[kBatch], next[kBatch];
+  auto load = [&](uint4 *to, int f0) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      to[i] = f0 + i * NT + tid < F ? src[f0 + i * NT + tid] : no_logits<T>();
+  };
+  load(q, 0);
+  // the elements outside whole granules, one a lane of the first warp
+  float odd = -kInf;
+  int odd_class = 0;
+  if (warp == 0 && lane < 16) {
+    odd_class = lane < 8 ? lane : head + F * E + lane - 8;
+    if (lane < 8 ? lane < head : odd_class < V) odd = to_f(x[odd_class]);
+  }
+
+  // ---- is the row padding?
+  int64_t tok = 0;
+  float tok_x = 0.0f;
+  [[maybe_unused]] float ty[4], xk[4], ym = -kInf;
+  if constexpr (kReads) {
+    if (p.tokens) tok = load_index(p.tokens, row, p.itype);
+    if (tok < 0) {
+      if (tid == 0) write_read_padding(p.o, row);
+      if constexpr (kTop)
+        for (int k = tid; k < p.top_k; k += NT) {
+          p.o.top_ids[(int64_t)row * p.top_k + k] = -1;
+          p.o.top_logprobs[(int64_t)row * p.top_k + k] = -kInf;
+        }
+      return;
+    }
+    if (tid == 0 && p.o.logprob && tok < V) tok_x = to_f(x[tok]);
+  } else {
+    // entry lane + 32 i in register i (every warp: all of them must know)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      ty[i] = -kInf;
+      xk[i] = 0.0f;
+      const int k = lane + 32 * i;
+      if (k >= p.te.k) continue;
+      const int64_t at = (int64_t)row * p.te.k + k;
+      const int64_t id = load_index(p.te.ids, at, p.te.itype);
+      const float y = load_value(p.te.logits, at, p.te.dtype);
+      if (id < 0 || y == -kInf) continue;  // left out
+      ty[i] = id < V ? y : nan;
+      if (warp == 0 && id < V) xk[i] = to_f(x[id]);
+      ym = max_nan(ym, ty[i]);
+    }
+    for (int o = 16; o; o >>= 1) ym = max_nan(ym, __shfl_xor_sync(~0u, ym, o));
+    if (ym == -kInf) {
+      if (tid == 0) p.loss[row] = 0.0f;
+      return;
+    }
+  }
+  if (kTop && tid == 0) misc[0] = misc[2] = 0;
+
+  // ---- the stream
+  Stat st{-kInf, 0.0f, 0.0f};
+  uint64_t s2 = 0, u2 = 0;
+  const uint64_t c2 = f2(a.c, a.c);
+  // a run is `per` batches
+  const int per = (F + kBatch * NT * kRuns - 1) / (kBatch * NT * kRuns);
+  int run = 0, in_run = 0;
+  float run_of = -kInf;
+  for (int f0 = 0; f0 < F || f0 == 0; f0 += kBatch * NT) {
+    load(next, f0 + kBatch * NT);
+    GranuleMax<T> gm;
+    gm.clear();
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) gm.add(q[i]);
+    float bm = gm.get();
+    const float batch = bm;
+    if (f0 == 0 && warp == 0) bm = max_nan(bm, odd);
+    const float m = max_nan(st.m, bm), m0 = m == -kInf ? 0.0f : m;
+    const float dm = (st.m - m0) * a.c, f = ex2(dm);
+    st.m = m;
+    s2 = f2_mul(s2, f2(f, f));
+    if (kReads) {
+      const float dd = fmaxf(dm, -1e4f);
+      u2 = f2_fma(u2, f2(f, f), f2_mul(s2, f2(dd, dd)));
+    }
+    const uint64_t nm = f2(-m0, -m0);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) accumulate<T, kReads>(q[i], nm, c2, s2, u2);
+    if (f0 == 0 && warp == 0) {
+      const float t = (odd - m0) * a.c, e = ex2(t);
+      s2 = f2_add(s2, f2(e, 0.0f));
+      u2 = f2_fma(f2(e, 0.0f), f2(fmaxf(t, -1e4f), 0.0f), u2);
+    }
+    if constexpr (kTop) {
+      run_of = fmaxf(run_of, batch);
+      if (++in_run == per) {
+        run_max[run++ * NT + tid] = run_of;
+        run_of = -kInf;
+        in_run = 0;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) q[i] = next[i];
+  }
+  {
+    float s0, s1, u0, u1;
+    f2_split(s2, s0, s1);
+    f2_split(u2, u0, u1);
+    st.s = s0 + s1;
+    st.u = u0 + u1;
+  }
+  if constexpr (kTop) {
+    if (in_run) run_max[run++ * NT + tid] = run_of;
+    gmax[tid] = order_of(st.m);
+  }
+  st = warp_combine(st, a.c);
+  if (lane == 0) {
+    part[warp * 3] = st.m;
+    part[warp * 3 + 1] = st.s;
+    part[warp * 3 + 2] = st.u;
+  }
+  __syncthreads();
+  if (!kTop && warp) return;
+  st = Stat{-kInf, 0.0f, 0.0f};
+  if (lane < kWarps)
+    st = Stat{part[lane * 3], part[lane * 3 + 1], part[lane * 3 + 2]};
+  st = warp_combine(st, a.c);
+  RowEnd end(st, a.inv_t);
+
+  if constexpr (kReads) {
+    if (tid == 0) write_read(p.o, row, end, tok_x, tok < V);
+  } else {
+    end.bad |= !(ym < kInf);
+    float tq[4], ys = 0.0f, l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool in = !(ty[i] == -kInf);
+      ty[i] = (ty[i] - ym) * a.inv_t;
+      tq[i] = in ? expf(ty[i]) : 0.0f;
+      ys += tq[i];
+    }
+    for (int o = 16; o; o >>= 1) ys += __shfl_xor_sync(~0u, ys, o);
+    const float ln_ys = logf(ys);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (tq[i] > 0.0f)
+        l += end.empty ? kInf
+                       : tq[i] / ys * ((ty[i] - ln_ys) - end.logp(xk[i]));
+    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
+    if (lane == 0) p.loss[row] = end.bad ? nan : a.t * a.t * l;
+  }
+  if constexpr (kTop) {
+    const int K = p.top_k;
+    int32_t *ids = p.o.top_ids + (int64_t)row * K;
+    float *lps = p.o.top_logprobs + (int64_t)row * K;
+    auto put = [&](int at, uint64_t key) {
+      ids[at] = key ? class_of(key) : -1;
+      lps[at] =
+          end.bad ? nan : key ? end.logp(value_of((uint32_t)(key >> 32))) : -kInf;
+    };
+    if (end.bad || end.empty) {
+      for (int k = tid; k < K; k += NT) put(k, 0);
+      return;
+    }
+    if (warp == 0) {
+      const uint32_t t = reached_by<NT>(K, gmax);
+      if (lane == 0) misc[1] = t;
+    }
+    __syncthreads();
+    const uint32_t tau = misc[1];
+    const float floor = value_of(tau);
+    for (int r = 0; r < run; ++r)
+      if (run_max[r * NT + tid] >= floor) {
+        const uint32_t at = atomicAdd(misc, 1u);
+        if (at < kPicked) runs[at] = (uint32_t)(r << 16 | tid);
+      }
+    __syncthreads();
+    const bool over = misc[0] > kPicked;
+    const int todo = over ? 0 : (int)misc[0], of = per * kBatch;
+    // f(key, place) of every logit of those runs, or of the row if there were
+    // too many, and of the logits outside whole granules
+    auto each = [&](auto &&f) {
+      auto granule = [&](int g) {
+        const uint4 w = src[g];
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          float v[2];
+          f2_split(pair_of<T>(w, j >> 1), v[0], v[1]);
+          if (v[j & 1] >= floor) f(key_of(v[j & 1], head + g * E + j));
+        }
+      };
+      for (int i = tid; i < todo * of; i += NT) {
+        const uint32_t r = runs[i / of];
+        const int g = ((int)(r >> 16) * of + i % of) * NT + (int)(r & 0xFFFF);
+        if (g < F) granule(g);
+      }
+      if (over)
+        for (int g = tid; g < F; g += NT) granule(g);
+      if (odd >= floor) f(key_of(odd, odd_class));
+    };
+    auto pick = [&](uint64_t least) {
+      each([&](uint64_t key) {
+        if (key >= least) {
+          const uint32_t at = atomicAdd(misc + 2, 1u);
+          if (at < kPicked) picked[at] = key;
+        }
+      });
+      __syncthreads();
+      return (int)misc[2];
+    };
+    uint64_t lo = (uint64_t)tau << 32, hi = ((uint64_t)order_of(end.m) + 1) << 32;
+    int M = over ? kPicked + 1 : pick(lo);
+    if (M > kPicked) {
+      // Many equal logits: halve the interval of keys, which are distinct,
+      // until K of them at least are left, but few enough.  64 halvings use
+      // the interval up.
+      for (int i = 0; i < 64; ++i) {
+        const uint64_t mid = lo + ((hi - lo) >> 1);
+        int c = 0;
+        each([&](uint64_t key) { c += key >= mid; });
+        c = __reduce_add_sync(~0u, c);
+        __syncthreads();
+        if (lane == 0) gmax[warp] = (uint32_t)c;
+        if (tid == 0) misc[2] = 0;
+        __syncthreads();
+        int all = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) all += (int)gmax[w];
+        (all >= K ? lo : hi) = mid;
+        if (all >= K && all <= kPicked) break;
+      }
+      M = min(pick(lo), kPicked);
+    }
+    for (int i = tid; i < M; i += NT) {
+      const uint64_t key = picked[i];
+      int above = 0;
+      for (int j = 0; j < M; ++j) above += picked[j] > key;
+      if (above < K) put(above, key);
+    }
+    for (int k = M + tid; k < K; k += NT) put(k, 0);
   }
 }
 
@@ -1383,6 +1685,23 @@ void launch_team(TeamArgs &p, cudaStream_t st) {
     launch_team_of<T, 256, MODE>(p, st);
 }
 
+// Whether rows of a kernel without gradients are streamed by one CTA each: when
+// there are enough of them to keep every SM loading.
+bool streams(const RowArgs &a) {
+  return (int64_t)a.rows >= 2 * (int64_t)sm_count();
+}
+template <class T, int MODE>
+void launch_stream(const TeamArgs &p, cudaStream_t st) {
+  const StreamArgs q{p.a, p.tokens, p.itype, p.top_k, p.o, p.te, p.loss};
+  // a few batches a thread at least, and maxima well above the alternatives in
+  // number
+  if (p.a.classes <= 4 * 4 * 256 * kElems<T> && (MODE != kReadTop || p.top_k <= 32))
+    k_stream<T, 128, MODE><<<p.a.rows, 128, 0, st>>>(q);
+  else
+    k_stream<T, 256, MODE><<<p.a.rows, 256, 0, st>>>(q);
+  check_launch(cudaGetLastError());
+}
+
 // Granules of the widest row when rows may start anywhere inside one.
 int granules_of(const RowArgs &a, int dtype) {
   const int size = elem_size(dtype), e = 16 / size;
@@ -1483,6 +1802,11 @@ int launch_token_logprobs(const tmnn_logits &x, const void *tokens,
         BY_DTYPE(x.dtype, (launch_narrow<T, kReadTop>(q, x.dtype, st)));
       else
         BY_DTYPE(x.dtype, (launch_narrow<T, kRead>(q, x.dtype, st)));
+    } else if (streams(p.a)) {
+      if (top_k)
+        BY_DTYPE(x.dtype, (launch_stream<T, kReadTop>(p, st)));
+      else
+        BY_DTYPE(x.dtype, (launch_stream<T, kRead>(p, st)));
     } else if (top_k) {
       BY_DTYPE(x.dtype, (launch_team<T, kReadTop>(p, st)));
     } else {
@@ -1581,6 +1905,8 @@ int launch_distill(const tmnn_logits &x, const void *ids, int index_type,
         BY_DTYPE(x.dtype, (launch_narrow<T, kLossGrad>(q, x.dtype, st)));
       else
         BY_DTYPE(x.dtype, (launch_narrow<T, kLoss>(q, x.dtype, st)));
+    } else if (!d_logits && streams(p.a)) {
+      BY_DTYPE(x.dtype, (launch_stream<T, kLoss>(p, st)));
     } else if (d_logits) {
       BY_DTYPE(x.dtype, (launch_team<T, kLossGrad>(p, st)));
     } else {
