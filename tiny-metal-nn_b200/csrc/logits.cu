@@ -1158,6 +1158,309 @@ struct BackRow {
   }
 };
 
+// ------------------------------------------------------------ a thread a row
+// Rows of up to 64 classes (a field's outputs): a warp brings 32 of them into
+// shared memory as fp32, side by side as they lie in memory, and each thread
+// works through one row there.  No lane idles on a row's odd end and nothing
+// is reduced over lanes.  Rows of whole quads lie `pitch` apart, an odd number
+// of quads, so that the lanes' 16-byte reads meet different banks; other rows
+// keep their distance V (odd, or twice an odd number).
+constexpr int kTinyClasses = 64;
+
+struct TinyArgs {
+  RowArgs a;
+  const void *tokens;
+  int itype, top_k;
+  LogprobOut o;
+  const float *stats, *d_logprob, *d_entropy;  // backward
+  Teacher te;
+  const float *row_weight;
+  float weight;
+  float *loss;
+  void *dx;
+  int64_t d_stride;
+  int pitch;            // floats between rows in shared memory
+  int packed, d_packed; // rows without gaps from a 16-byte boundary on
+};
+
+template <class T, int MODE, bool QUADS>
+__global__ void __launch_bounds__(128) k_tiny(TinyArgs p) {
+  extern __shared__ __align__(16) float image_all[];
+  constexpr bool kReads = MODE == kRead || MODE == kReadTop;
+  constexpr bool kTeacher = MODE == kLoss || MODE == kLossGrad;
+  const RowArgs &a = p.a;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int V = a.classes, P = p.pitch;
+  const uint32_t row0 = (blockIdx.x * 4 + warp) * 32;
+  if (row0 >= a.rows) return;
+  const int rows = min(32u, a.rows - row0);
+  float *image = image_all + warp * ((32 * P + 3) / 4 * 4);
+  const float nan = not_a_number();
+
+  // f(element's place in the image, its place among the rows, row, class) of
+  // every element, lanes side by side
+  auto each_element = [&](auto &&f) {
+    int r = 0, c = lane;
+    while (c >= V) c -= V, ++r;
+    const int dr = 32 / V, dc = 32 - dr * V;
+    while (r < rows) {
+      f(r * P + c, r, c);
+      r += dr;
+      c += dc;
+      if (c >= V) c -= V, ++r;
+    }
+  };
+  // f(first of four places in the image, quad) of every quad of packed rows
+  auto each_quad = [&](int first, int step, int end, auto &&f) {
+    if (QUADS) {
+      const int R = V / 4;  // quads a row
+      int r = first / R, c = first - r * R;
+      const int dr = step / R, dc = step - dr * R;
+      for (int i = first; i < end; i += step) {
+        f(r * P + c * 4, i);
+        r += dr;
+        c += dc;
+        if (c >= R) c -= R, ++r;
+      }
+    } else {
+      for (int i = first; i < end; i += step) f(i * 4, i);
+    }
+  };
+
+  // ---- in
+  const T *x = static_cast<const T *>(a.x) + (int64_t)row0 * a.stride;
+  const int quads = rows * V / 4;  // whole ones
+  if (p.packed) {
+    if constexpr (sizeof(T) == 4) {
+      each_quad(lane, 32, quads, [&](int at, int i) {
+        copy16(image + at, reinterpret_cast<const uint4 *>(x) + i);
+      });
+      copies_done();
+    } else {
+      // two quads a granule; lanes 2 i and 2 i + 1 take its halves
+      each_quad(lane, 32, quads, [&](int at, int i) {
+        const uint2 w = reinterpret_cast<const uint2 *>(x)[i];
+        const uint4 g{w.x, w.y, 0, 0};
+        float4 v;
+        f2_split(pair_of<T>(g, 0), v.x, v.y);
+        f2_split(pair_of<T>(g, 1), v.z, v.w);
+        *reinterpret_cast<float4 *>(image + at) = v;
+      });
+    }
+    const int e = quads * 4 + lane;
+    if (!QUADS && e < rows * V) image[e] = to_f(x[e]);
+  } else {
+    each_element([&](int at, int r, int c) {
+      image[at] = to_f(x[(int64_t)r * a.stride + c]);
+    });
+  }
+  __syncwarp();
+
+  float *mine = image + lane * P;
+  const bool on = lane < rows;
+  const uint32_t row = row0 + (on ? lane : 0);
+  // f(first class, four values) of the thread's row; -inf behind its end
+  auto each = [&](auto &&f) {
+    if (QUADS) {
+#pragma unroll 4
+      for (int c = 0; c < V; c += 4)
+        f(c, *reinterpret_cast<const float4 *>(mine + c));
+    } else {
+      int c = 0;
+#pragma unroll 2
+      for (; c + 4 <= V; c += 4)
+        f(c, float4{mine[c], mine[c + 1], mine[c + 2], mine[c + 3]});
+      if (c < V)
+        f(c, float4{mine[c], c + 1 < V ? mine[c + 1] : -kInf,
+                    c + 2 < V ? mine[c + 2] : -kInf, -kInf});
+    }
+  };
+  // v becomes element c + i of the thread's row
+  auto write4 = [&](int c, const float4 &v) {
+    if (QUADS) {
+      *reinterpret_cast<float4 *>(mine + c) = v;
+    } else {
+      mine[c] = v.x;
+      if (c + 1 < V) mine[c + 1] = v.y;
+      if (c + 2 < V) mine[c + 2] = v.z;
+      if (c + 3 < V) mine[c + 3] = v.w;
+    }
+  };
+
+  if (on) {
+    int64_t tok = 0;
+    float ym = 0.0f;
+    bool idle = false;
+    const int64_t entry0 = (int64_t)row * p.te.k;
+    // the teacher's entry k: its id, -1 if left out, and logit
+    auto entry = [&](int k, float &y) {
+      const int64_t id = load_index(p.te.ids, entry0 + k, p.te.itype);
+      y = load_value(p.te.logits, entry0 + k, p.te.dtype);
+      if (id < 0 || y == -kInf) return -1;
+      if (id >= V) {
+        y = nan;
+        return 0;
+      }
+      return (int)id;
+    };
+    if constexpr (kReads) {
+      if (p.tokens) tok = load_index(p.tokens, row, p.itype);
+      idle = tok < 0;
+    }
+    if constexpr (kTeacher) {
+      ym = -kInf;
+      for (int k = 0; k < p.te.k; ++k) {
+        float y;
+        if (entry(k, y) >= 0) ym = max_nan(ym, y);
+      }
+      idle = ym == -kInf;
+    }
+    if constexpr (MODE == kBack) {
+      const BackRow b(a, p.tokens, p.itype, p.stats, p.d_logprob, p.d_entropy,
+                      row);
+      each([&](int c, const float4 &v) {
+        write4(c, float4{b.at(v.x, c, a.c), b.at(v.y, c + 1, a.c),
+                         b.at(v.z, c + 2, a.c), b.at(v.w, c + 3, a.c)});
+      });
+    } else {
+      Stat st{-kInf, 0.0f, 0.0f};
+      each([&](int, const float4 &v) {
+        st.m = max_nan(max_nan(st.m, max_nan(v.x, v.y)), max_nan(v.z, v.w));
+      });
+      const float m0 = st.m == -kInf ? 0.0f : st.m;
+      const uint64_t nm = f2(-m0, -m0), c2 = f2(a.c, a.c);
+      {
+        uint64_t s2 = 0, u2 = 0;
+        each([&](int, const float4 &v) {
+          const uint4 g{__float_as_uint(v.x), __float_as_uint(v.y),
+                        __float_as_uint(v.z), __float_as_uint(v.w)};
+          accumulate<float, kReads>(g, nm, c2, s2, u2);
+        });
+        float s0, s1, u0, u1;
+        f2_split(s2, s0, s1);
+        f2_split(u2, u0, u1);
+        st.s = s0 + s1;
+        st.u = u0 + u1;
+      }
+      RowEnd end(st, a.inv_t);
+      if (kTeacher) end.bad |= !(ym < kInf);
+      if constexpr (kReads) {
+        if (idle)
+          write_read_padding(p.o, row);
+        else
+          write_read(p.o, row, end, tok < V ? mine[tok] : 0.0f, tok < V);
+      }
+      if constexpr (MODE == kReadTop) {
+        // the maxima of eight classes each; the largest of them, its class,
+        // and the eight without it, again and again
+        constexpr int kEights = kTinyClasses / 8;
+        float best[kEights];
+#pragma unroll
+        for (int j = 0; j < kEights; ++j) {
+          float v = -kInf;
+          if (!end.bad && !idle)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (j * 8 + i < V) v = fmaxf(v, mine[j * 8 + i]);
+          best[j] = v;
+        }
+        int32_t *ids = p.o.top_ids + (int64_t)row * p.top_k;
+        float *lps = p.o.top_logprobs + (int64_t)row * p.top_k;
+        for (int k = 0; k < p.top_k; ++k) {
+          float v = best[0];
+          int at = 0;
+#pragma unroll
+          for (int j = 1; j < kEights; ++j)
+            if (best[j] > v) {
+              v = best[j];
+              at = j;
+            }
+          const bool some = v > -kInf;
+          int cls = -1;
+          float rest = -kInf;
+          if (some) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int c = at * 8 + i;
+              const float w = c < V ? mine[c] : -kInf;
+              if (cls < 0 && w == v)
+                cls = c;
+              else
+                rest = fmaxf(rest, w);
+            }
+            mine[cls] = -kInf;
+#pragma unroll
+            for (int j = 0; j < kEights; ++j)
+              if (j == at) best[j] = rest;
+          }
+          ids[k] = cls;
+          lps[k] = some ? end.logp(v) : end.bad && !idle ? nan : -kInf;
+        }
+      }
+      if constexpr (kTeacher) {
+        const float w = (p.row_weight ? p.row_weight[row] : p.weight) * a.t;
+        const bool zero = idle || (end.empty && !end.bad);
+        float ys = 0.0f, loss = 0.0f;
+        for (int k = 0; k < p.te.k; ++k) {
+          float y;
+          if (entry(k, y) >= 0) ys += expf((y - ym) * a.inv_t);
+        }
+        const float ln_ys = logf(ys), inv_ys = 1.0f / ys;
+        for (int k = 0; k < p.te.k; ++k) {
+          float y;
+          const int id = entry(k, y);
+          const float ty = (y - ym) * a.inv_t;
+          const float q = id >= 0 ? expf(ty) * inv_ys : 0.0f;
+          if (q > 0.0f)
+            loss += end.empty ? kInf
+                              : q * ((ty - ln_ys) - end.logp(mine[id]));
+        }
+        p.loss[row] = idle ? 0.0f : end.bad ? nan : a.t * a.t * loss;
+        if constexpr (MODE == kLossGrad) {
+          const float ws = zero ? 0.0f : end.bad ? nan : w / end.s;
+          each([&](int c, const float4 &v) {
+            float4 r;
+            float t, u;
+            f2_split(f2_mul(f2_add(f2(v.x, v.y), nm), c2), t, u);
+            f2_split(f2_mul(f2(ex2(t), ex2(u)), f2(ws, ws)), r.x, r.y);
+            f2_split(f2_mul(f2_add(f2(v.z, v.w), nm), c2), t, u);
+            f2_split(f2_mul(f2(ex2(t), ex2(u)), f2(ws, ws)), r.z, r.w);
+            write4(c, zero ? float4{0.0f, 0.0f, 0.0f, 0.0f} : r);
+          });
+          if (!zero && !end.bad)
+            for (int k = 0; k < p.te.k; ++k) {
+              float y;
+              const int id = entry(k, y);
+              if (id >= 0) mine[id] -= w * (expf((y - ym) * a.inv_t) * inv_ys);
+            }
+        }
+      }
+    }
+  }
+
+  // ---- out
+  if constexpr (MODE == kLossGrad || MODE == kBack) {
+    __syncwarp();
+    T *d = static_cast<T *>(p.dx) + (int64_t)row0 * p.d_stride;
+    if (p.d_packed) {
+      each_quad(lane, 32, quads, [&](int at, int i) {
+        const float4 v = *reinterpret_cast<const float4 *>(image + at);
+        if constexpr (sizeof(T) == 4)
+          reinterpret_cast<float4 *>(d)[i] = v;
+        else
+          reinterpret_cast<uint2 *>(d)[i] =
+              uint2{pack2<T>(v.x, v.y), pack2<T>(v.z, v.w)};
+      });
+      const int e = quads * 4 + lane;
+      if (!QUADS && e < rows * V) d[e] = from_f<T>(image[e]);
+    } else {
+      each_element([&](int at, int r, int c) {
+        d[(int64_t)r * p.d_stride + c] = from_f<T>(image[at]);
+      });
+    }
+  }
+}
+
 // ------------------------------------------------------------ lanes a row
 // Narrow rows: 1 to 32 neighbouring lanes hold a row in registers, NG granules
 // each (granule lane + lanes * j), and reduce over one another with shuffles.
@@ -1702,6 +2005,25 @@ void launch_stream(const TeamArgs &p, cudaStream_t st) {
   check_launch(cudaGetLastError());
 }
 
+template <class T, int MODE>
+void launch_tiny(TinyArgs &p, cudaStream_t st) {
+  const int V = p.a.classes;
+  const bool quads = V % 4 == 0;
+  p.pitch = quads ? (V / 4 | 1) * 4 : V;
+  auto packed = [&](const void *at, int64_t stride) {
+    return (uintptr_t)at % 16 == 0 && (stride == V || p.a.rows == 1);
+  };
+  p.packed = packed(p.a.x, p.a.stride);
+  p.d_packed = packed(p.dx, p.d_stride);
+  const size_t smem = (size_t)((32 * p.pitch + 3) / 4 * 4) * 4 * sizeof(float);
+  const uint32_t grid = (p.a.rows + 127) / 128;
+  if (quads)
+    k_tiny<T, MODE, true><<<grid, 128, smem, st>>>(p);
+  else
+    k_tiny<T, MODE, false><<<grid, 128, smem, st>>>(p);
+  check_launch(cudaGetLastError());
+}
+
 // Granules of the widest row when rows may start anywhere inside one.
 int granules_of(const RowArgs &a, int dtype) {
   const int size = elem_size(dtype), e = 16 / size;
@@ -1791,7 +2113,18 @@ int launch_token_logprobs(const tmnn_logits &x, const void *tokens,
     p.o.top_ids = top_k ? o.top_ids + (int64_t)i * top_k : nullptr;
     p.o.top_logprobs = top_k ? o.top_logprobs + (int64_t)i * top_k : nullptr;
     p.o.stats = o.stats ? o.stats + (int64_t)i * 3 : nullptr;
-    if (granules_of(p.a, x.dtype) <= kNarrow) {
+    if (x.classes <= kTinyClasses) {
+      TinyArgs q{};
+      q.a = p.a;
+      q.tokens = p.tokens;
+      q.itype = p.itype;
+      q.top_k = p.top_k;
+      q.o = p.o;
+      if (top_k)
+        BY_DTYPE(x.dtype, (launch_tiny<T, kReadTop>(q, st)));
+      else
+        BY_DTYPE(x.dtype, (launch_tiny<T, kRead>(q, st)));
+    } else if (granules_of(p.a, x.dtype) <= kNarrow) {
       NarrowArgs q{};
       q.a = p.a;
       q.tokens = p.tokens;
@@ -1839,6 +2172,19 @@ int launch_token_logprobs_backward(const tmnn_logits &x, const void *tokens,
     b.x = at(x.data, (int64_t)i * x.row_stride * size);
     b.rows = n;
     const void *d = at(d_logits, (int64_t)i * d_stride * size);
+    if (x.classes <= kTinyClasses) {
+      TinyArgs q{};
+      q.a = b;
+      q.tokens = at(tokens, (int64_t)i * index_size(index_type));
+      q.itype = index_type;
+      q.stats = stats + (int64_t)i * 3;
+      q.d_logprob = d_logprob ? d_logprob + i : nullptr;
+      q.d_entropy = d_entropy ? d_entropy + i : nullptr;
+      q.dx = const_cast<void *>(d);
+      q.d_stride = d_stride;
+      BY_DTYPE(x.dtype, (launch_tiny<T, kBack>(q, st)));
+      return;
+    }
     if (granules_of(b, x.dtype) <= kNarrow) {
       NarrowArgs q{};
       q.a = b;
@@ -1892,7 +2238,20 @@ int launch_distill(const tmnn_logits &x, const void *ids, int index_type,
     p.loss = loss + i;
     p.dx = const_cast<void *>(at(d_logits, (int64_t)i * d_stride * size));
     p.d_stride = d_stride;
-    if (granules_of(p.a, x.dtype) <= kNarrow) {
+    if (x.classes <= kTinyClasses) {
+      TinyArgs q{};
+      q.a = p.a;
+      q.te = p.te;
+      q.row_weight = p.row_weight;
+      q.weight = weight;
+      q.loss = p.loss;
+      q.dx = p.dx;
+      q.d_stride = d_stride;
+      if (d_logits)
+        BY_DTYPE(x.dtype, (launch_tiny<T, kLossGrad>(q, st)));
+      else
+        BY_DTYPE(x.dtype, (launch_tiny<T, kLoss>(q, st)));
+    } else if (granules_of(p.a, x.dtype) <= kNarrow) {
       NarrowArgs q{};
       q.a = p.a;
       q.te = p.te;
