@@ -1197,145 +1197,201 @@ __global__ void __launch_bounds__(128) k_tiny(TinyArgs p) {
   float *image = image_all + warp * ((32 * P + 3) / 4 * 4);
   const float nan = not_a_number();
 
-  // f(element's place in the image, its place among the rows, row, class) of
-  // every element, lanes side by side
-  auto each_element = [&](auto &&f) {
+  // use(row, i, load(row, i)) of every i < N of every row, lanes side by side,
+  // four loads in flight
+  auto each_of = [&](int N, auto &&load, auto &&use) {
     int r = 0, c = lane;
-    while (c >= V) c -= V, ++r;
-    const int dr = 32 / V, dc = 32 - dr * V;
-    while (r < rows) {
-      f(r * P + c, r, c);
-      r += dr;
-      c += dc;
-      if (c >= V) c -= V, ++r;
-    }
-  };
-  // f(first of four places in the image, quad) of every quad of packed rows
-  auto each_quad = [&](int first, int step, int end, auto &&f) {
-    if (QUADS) {
-      const int R = V / 4;  // quads a row
-      int r = first / R, c = first - r * R;
-      const int dr = step / R, dc = step - dr * R;
-      for (int i = first; i < end; i += step) {
-        f(r * P + c * 4, i);
+    while (c >= N) c -= N, ++r;
+    const int dr = 32 / N, dc = 32 - dr * N;
+    while (__any_sync(~0u, r < rows)) {
+      int rs[4], cs[4];
+      decltype(load(0, 0)) v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        rs[i] = r;
+        cs[i] = c;
+        if (r < rows) v[i] = load(r, c);
         r += dr;
         c += dc;
-        if (c >= R) c -= R, ++r;
+        if (c >= N) c -= N, ++r;
       }
-    } else {
-      for (int i = first; i < end; i += step) f(i * 4, i);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (rs[i] < rows) use(rs[i], cs[i], v[i]);
+    }
+  };
+  // The same of every quad of packed rows: load(quad), then use(first of its
+  // four places in the image, quad, value).
+  auto each_quad = [&](int end, auto &&load, auto &&use) {
+    const int R = QUADS ? V / 4 : 1;  // quads a row
+    int r = lane / R, c = lane - r * R;
+    const int dr = 32 / R, dc = 32 - dr * R;
+    for (int i0 = lane; i0 - lane < end; i0 += 128) {
+      int at[4];
+      decltype(load(0, 0)) v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        at[i] = QUADS ? r * P + c * 4 : (i0 + 32 * i) * 4;
+        if (i0 + 32 * i < end) v[i] = load(at[i], i0 + 32 * i);
+        if (QUADS) {
+          r += dr;
+          c += dc;
+          if (c >= R) c -= R, ++r;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i0 + 32 * i < end) use(at[i], i0 + 32 * i, v[i]);
     }
   };
 
   // ---- in
   const T *x = static_cast<const T *>(a.x) + (int64_t)row0 * a.stride;
   const int quads = rows * V / 4;  // whole ones
+  const bool on = lane < rows;
+  const uint32_t row = row0 + (on ? lane : 0);
+  int64_t tok = 0;
+  float weight = p.weight;
+  if (kReads && p.tokens) tok = load_index(p.tokens, row, p.itype);
+  if (MODE == kLossGrad && p.row_weight) weight = p.row_weight[row];
   if (p.packed) {
     if constexpr (sizeof(T) == 4) {
-      each_quad(lane, 32, quads, [&](int at, int i) {
-        copy16(image + at, reinterpret_cast<const uint4 *>(x) + i);
-      });
-      copies_done();
+      each_quad(
+          quads,
+          [&](int at, int i) {
+            copy16(image + at, reinterpret_cast<const uint4 *>(x) + i);
+            return 0;
+          },
+          [](int, int, int) {});
     } else {
-      // two quads a granule; lanes 2 i and 2 i + 1 take its halves
-      each_quad(lane, 32, quads, [&](int at, int i) {
-        const uint2 w = reinterpret_cast<const uint2 *>(x)[i];
-        const uint4 g{w.x, w.y, 0, 0};
-        float4 v;
-        f2_split(pair_of<T>(g, 0), v.x, v.y);
-        f2_split(pair_of<T>(g, 1), v.z, v.w);
-        *reinterpret_cast<float4 *>(image + at) = v;
-      });
+      each_quad(
+          quads,
+          [&](int, int i) { return reinterpret_cast<const uint2 *>(x)[i]; },
+          [&](int at, int, const uint2 &w) {
+            const uint4 g{w.x, w.y, 0, 0};
+            float4 v;
+            f2_split(pair_of<T>(g, 0), v.x, v.y);
+            f2_split(pair_of<T>(g, 1), v.z, v.w);
+            *reinterpret_cast<float4 *>(image + at) = v;
+          });
     }
     const int e = quads * 4 + lane;
     if (!QUADS && e < rows * V) image[e] = to_f(x[e]);
   } else {
-    each_element([&](int at, int r, int c) {
-      image[at] = to_f(x[(int64_t)r * a.stride + c]);
-    });
+    each_of(
+        V, [&](int r, int c) { return x[(int64_t)r * a.stride + c]; },
+        [&](int r, int c, T v) { image[r * P + c] = to_f(v); });
   }
+  // the teacher's entries: id (-1 if left out) and logit, rows an odd number
+  // apart
+  const int K = kTeacher ? p.te.k : 0, KP = K | 1;
+  float *ey = image_all + 4 * ((32 * P + 3) / 4 * 4) + warp * 64 * KP;
+  int32_t *eid = reinterpret_cast<int32_t *>(ey + 32 * KP);
+  if constexpr (kTeacher) {
+    struct Entry {
+      int64_t id;
+      float y;
+    };
+    const int64_t first = (int64_t)row0 * K;
+    each_of(
+        K,
+        [&](int r, int k) {
+          return Entry{load_index(p.te.ids, first + r * K + k, p.te.itype),
+                       load_value(p.te.logits, first + r * K + k, p.te.dtype)};
+        },
+        [&](int r, int k, const Entry &t) {
+          const bool out = t.id < 0 || t.y == -kInf;  // left out
+          ey[r * KP + k] = out ? -kInf : t.id < V ? t.y : nan;
+          eid[r * KP + k] = out ? -1 : t.id < V ? (int32_t)t.id : 0;
+        });
+    ey += lane * KP;
+    eid += lane * KP;
+  }
+  if (p.packed && sizeof(T) == 4) copies_done();
   __syncwarp();
 
   float *mine = image + lane * P;
-  const bool on = lane < rows;
-  const uint32_t row = row0 + (on ? lane : 0);
-  // f(first class, four values) of the thread's row; -inf behind its end
-  auto each = [&](auto &&f) {
+  // the j-th eight of the thread's row, -inf behind its end
+  auto eight = [&](int j, float *v) {
+    const int c = j * 8;
     if (QUADS) {
-#pragma unroll 4
-      for (int c = 0; c < V; c += 4)
-        f(c, *reinterpret_cast<const float4 *>(mine + c));
+      const float4 lo = *reinterpret_cast<const float4 *>(mine + c);
+      float4 hi{-kInf, -kInf, -kInf, -kInf};
+      if (c + 4 < V) hi = *reinterpret_cast<const float4 *>(mine + c + 4);
+      v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w;
+      v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
+    } else if (c + 8 <= V) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = mine[c + i];
     } else {
-      int c = 0;
-#pragma unroll 2
-      for (; c + 4 <= V; c += 4)
-        f(c, float4{mine[c], mine[c + 1], mine[c + 2], mine[c + 3]});
-      if (c < V)
-        f(c, float4{mine[c], c + 1 < V ? mine[c + 1] : -kInf,
-                    c + 2 < V ? mine[c + 2] : -kInf, -kInf});
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = c + i < V ? mine[c + i] : -kInf;
     }
   };
-  // v becomes element c + i of the thread's row
-  auto write4 = [&](int c, const float4 &v) {
+  auto write_eight = [&](int j, const float *v) {
+    const int c = j * 8;
     if (QUADS) {
-      *reinterpret_cast<float4 *>(mine + c) = v;
+      *reinterpret_cast<float4 *>(mine + c) = float4{v[0], v[1], v[2], v[3]};
+      if (c + 4 < V)
+        *reinterpret_cast<float4 *>(mine + c + 4) = float4{v[4], v[5], v[6], v[7]};
     } else {
-      mine[c] = v.x;
-      if (c + 1 < V) mine[c + 1] = v.y;
-      if (c + 2 < V) mine[c + 2] = v.z;
-      if (c + 3 < V) mine[c + 3] = v.w;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c + i < V) mine[c + i] = v[i];
     }
   };
+  auto max8 = [](const float *v) {
+    return max_nan(max_nan(max_nan(v[0], v[1]), max_nan(v[2], v[3])),
+                   max_nan(max_nan(v[4], v[5]), max_nan(v[6], v[7])));
+  };
+  constexpr int kEights = kTinyClasses / 8;
+  const int eights = (V + 7) / 8;
 
   if (on) {
-    int64_t tok = 0;
-    float ym = 0.0f;
-    bool idle = false;
-    const int64_t entry0 = (int64_t)row * p.te.k;
-    // the teacher's entry k: its id, -1 if left out, and logit
-    auto entry = [&](int k, float &y) {
-      const int64_t id = load_index(p.te.ids, entry0 + k, p.te.itype);
-      y = load_value(p.te.logits, entry0 + k, p.te.dtype);
-      if (id < 0 || y == -kInf) return -1;
-      if (id >= V) {
-        y = nan;
-        return 0;
-      }
-      return (int)id;
-    };
-    if constexpr (kReads) {
-      if (p.tokens) tok = load_index(p.tokens, row, p.itype);
-      idle = tok < 0;
-    }
-    if constexpr (kTeacher) {
-      ym = -kInf;
-      for (int k = 0; k < p.te.k; ++k) {
-        float y;
-        if (entry(k, y) >= 0) ym = max_nan(ym, y);
-      }
-      idle = ym == -kInf;
-    }
     if constexpr (MODE == kBack) {
       const BackRow b(a, p.tokens, p.itype, p.stats, p.d_logprob, p.d_entropy,
                       row);
-      each([&](int c, const float4 &v) {
-        write4(c, float4{b.at(v.x, c, a.c), b.at(v.y, c + 1, a.c),
-                         b.at(v.z, c + 2, a.c), b.at(v.w, c + 3, a.c)});
-      });
+#pragma unroll 2
+      for (int j = 0; j < eights; ++j) {
+        float v[8];
+        eight(j, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = b.at(v[i], j * 8 + i, a.c);
+        write_eight(j, v);
+      }
     } else {
-      Stat st{-kInf, 0.0f, 0.0f};
-      each([&](int, const float4 &v) {
-        st.m = max_nan(max_nan(st.m, max_nan(v.x, v.y)), max_nan(v.z, v.w));
-      });
+      float ym = -kInf;
+      bool idle = tok < 0;
+      if constexpr (kTeacher) {
+        for (int k = 0; k < K; ++k) ym = max_nan(ym, ey[k]);
+        idle = ym == -kInf;
+      }
+      float best[kEights];  // maxima of the eights
+#pragma unroll
+      for (int j = 0; j < kEights; ++j) {
+        best[j] = -kInf;
+        if (j < eights) {
+          float v[8];
+          eight(j, v);
+          best[j] = max8(v);
+        }
+      }
+      Stat st{max8(best), 0.0f, 0.0f};
       const float m0 = st.m == -kInf ? 0.0f : st.m;
       const uint64_t nm = f2(-m0, -m0), c2 = f2(a.c, a.c);
       {
         uint64_t s2 = 0, u2 = 0;
-        each([&](int, const float4 &v) {
-          const uint4 g{__float_as_uint(v.x), __float_as_uint(v.y),
-                        __float_as_uint(v.z), __float_as_uint(v.w)};
-          accumulate<float, kReads>(g, nm, c2, s2, u2);
-        });
+#pragma unroll 2
+        for (int j = 0; j < eights; ++j) {
+          float v[8];
+          eight(j, v);
+#pragma unroll
+          for (int i = 0; i < 8; i += 4)
+            accumulate<float, kReads>(
+                uint4{__float_as_uint(v[i]), __float_as_uint(v[i + 1]),
+                      __float_as_uint(v[i + 2]), __float_as_uint(v[i + 3])},
+                nm, c2, s2, u2);
+        }
         float s0, s1, u0, u1;
         f2_split(s2, s0, s1);
         f2_split(u2, u0, u1);
@@ -1351,88 +1407,100 @@ __global__ void __launch_bounds__(128) k_tiny(TinyArgs p) {
           write_read(p.o, row, end, tok < V ? mine[tok] : 0.0f, tok < V);
       }
       if constexpr (MODE == kReadTop) {
-        // the maxima of eight classes each; the largest of them, its class,
-        // and the eight without it, again and again
-        constexpr int kEights = kTinyClasses / 8;
-        float best[kEights];
-#pragma unroll
-        for (int j = 0; j < kEights; ++j) {
-          float v = -kInf;
-          if (!end.bad && !idle)
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (j * 8 + i < V) v = fmaxf(v, mine[j * 8 + i]);
-          best[j] = v;
-        }
+        // the largest of the eights' maxima, its class, and that eight without
+        // it, again and again; four alternatives are written together
+        const bool none = end.bad || idle;
         int32_t *ids = p.o.top_ids + (int64_t)row * p.top_k;
         float *lps = p.o.top_logprobs + (int64_t)row * p.top_k;
-        for (int k = 0; k < p.top_k; ++k) {
-          float v = best[0];
-          int at = 0;
+        const bool fours = p.top_k % 4 == 0 && (uintptr_t)p.o.top_ids % 16 == 0 &&
+                           (uintptr_t)p.o.top_logprobs % 16 == 0;
+        for (int k0 = 0; k0 < p.top_k; k0 += 4) {
+          int32_t id[4];
+          float lp[4];
 #pragma unroll
-          for (int j = 1; j < kEights; ++j)
-            if (best[j] > v) {
-              v = best[j];
-              at = j;
+          for (int k = 0; k < 4; ++k) {
+            float v = best[0];
+            int at = 0;
+#pragma unroll
+            for (int j = 1; j < kEights; ++j)
+              if (best[j] > v) {
+                v = best[j];
+                at = j;
+              }
+            const bool some = v > -kInf && !none && k0 + k < p.top_k;
+            id[k] = -1;
+            lp[k] = end.bad && !idle ? nan : -kInf;
+            if (some) {
+              float w[8];
+              eight(at, w);
+              int i = 7;
+#pragma unroll
+              for (int e = 6; e >= 0; --e)
+                if (w[e] == v) i = e;
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                if (e == i) w[e] = -kInf;
+              const float rest = max8(w);
+              id[k] = at * 8 + i;
+              lp[k] = end.logp(v);
+              mine[id[k]] = -kInf;
+#pragma unroll
+              for (int j = 0; j < kEights; ++j)
+                if (j == at) best[j] = rest;
             }
-          const bool some = v > -kInf;
-          int cls = -1;
-          float rest = -kInf;
-          if (some) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int c = at * 8 + i;
-              const float w = c < V ? mine[c] : -kInf;
-              if (cls < 0 && w == v)
-                cls = c;
-              else
-                rest = fmaxf(rest, w);
-            }
-            mine[cls] = -kInf;
-#pragma unroll
-            for (int j = 0; j < kEights; ++j)
-              if (j == at) best[j] = rest;
           }
-          ids[k] = cls;
-          lps[k] = some ? end.logp(v) : end.bad && !idle ? nan : -kInf;
+          if (fours) {
+            *reinterpret_cast<int4 *>(ids + k0) = int4{id[0], id[1], id[2], id[3]};
+            *reinterpret_cast<float4 *>(lps + k0) =
+                float4{lp[0], lp[1], lp[2], lp[3]};
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (k0 + k < p.top_k) {
+                ids[k0 + k] = id[k];
+                lps[k0 + k] = lp[k];
+              }
+          }
         }
       }
       if constexpr (kTeacher) {
-        const float w = (p.row_weight ? p.row_weight[row] : p.weight) * a.t;
+        // loss = sum q (log q - log p) = (sum e (y - log p)) / sum e
+        //        - log sum e  with e = e^y, y = (teacher - max) / T
+        const float w = weight * a.t;
         const bool zero = idle || (end.empty && !end.bad);
         float ys = 0.0f, loss = 0.0f;
-        for (int k = 0; k < p.te.k; ++k) {
-          float y;
-          if (entry(k, y) >= 0) ys += expf((y - ym) * a.inv_t);
+        for (int k = 0; k < K; ++k) {
+          const float y = (ey[k] - ym) * a.inv_t, e = eid[k] >= 0 ? expf(y) : 0.0f;
+          ys += e;
+          if (e > 0.0f)
+            loss += end.empty ? kInf : e * (y - end.logp(mine[eid[k]]));
+          if (MODE == kLossGrad) ey[k] = e;
         }
-        const float ln_ys = logf(ys), inv_ys = 1.0f / ys;
-        for (int k = 0; k < p.te.k; ++k) {
-          float y;
-          const int id = entry(k, y);
-          const float ty = (y - ym) * a.inv_t;
-          const float q = id >= 0 ? expf(ty) * inv_ys : 0.0f;
-          if (q > 0.0f)
-            loss += end.empty ? kInf
-                              : q * ((ty - ln_ys) - end.logp(mine[id]));
-        }
-        p.loss[row] = idle ? 0.0f : end.bad ? nan : a.t * a.t * loss;
+        const float inv_ys = 1.0f / ys;
+        p.loss[row] = idle      ? 0.0f
+                      : end.bad ? nan
+                                : a.t * a.t * (loss * inv_ys - logf(ys));
         if constexpr (MODE == kLossGrad) {
           const float ws = zero ? 0.0f : end.bad ? nan : w / end.s;
-          each([&](int c, const float4 &v) {
-            float4 r;
-            float t, u;
-            f2_split(f2_mul(f2_add(f2(v.x, v.y), nm), c2), t, u);
-            f2_split(f2_mul(f2(ex2(t), ex2(u)), f2(ws, ws)), r.x, r.y);
-            f2_split(f2_mul(f2_add(f2(v.z, v.w), nm), c2), t, u);
-            f2_split(f2_mul(f2(ex2(t), ex2(u)), f2(ws, ws)), r.z, r.w);
-            write4(c, zero ? float4{0.0f, 0.0f, 0.0f, 0.0f} : r);
-          });
-          if (!zero && !end.bad)
-            for (int k = 0; k < p.te.k; ++k) {
-              float y;
-              const int id = entry(k, y);
-              if (id >= 0) mine[id] -= w * (expf((y - ym) * a.inv_t) * inv_ys);
+          const uint64_t w2 = f2(ws, ws);
+#pragma unroll 2
+          for (int j = 0; j < eights; ++j) {
+            float v[8];
+            eight(j, v);
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+              float t, u;
+              f2_split(f2_mul(f2_add(f2(v[i], v[i + 1]), nm), c2), t, u);
+              f2_split(f2_mul(f2(ex2(t), ex2(u)), w2), v[i], v[i + 1]);
+              if (zero) v[i] = v[i + 1] = 0.0f;
             }
+            write_eight(j, v);
+          }
+          if (!zero && !end.bad) {
+            const float wq = w * inv_ys;
+            for (int k = 0; k < K; ++k)
+              if (eid[k] >= 0) mine[eid[k]] -= wq * ey[k];
+          }
         }
       }
     }
@@ -1443,20 +1511,24 @@ __global__ void __launch_bounds__(128) k_tiny(TinyArgs p) {
     __syncwarp();
     T *d = static_cast<T *>(p.dx) + (int64_t)row0 * p.d_stride;
     if (p.d_packed) {
-      each_quad(lane, 32, quads, [&](int at, int i) {
-        const float4 v = *reinterpret_cast<const float4 *>(image + at);
-        if constexpr (sizeof(T) == 4)
-          reinterpret_cast<float4 *>(d)[i] = v;
-        else
-          reinterpret_cast<uint2 *>(d)[i] =
-              uint2{pack2<T>(v.x, v.y), pack2<T>(v.z, v.w)};
-      });
+      each_quad(
+          quads,
+          [&](int at, int) { return *reinterpret_cast<const float4 *>(image + at); },
+          [&](int, int i, const float4 &v) {
+            if constexpr (sizeof(T) == 4)
+              reinterpret_cast<float4 *>(d)[i] = v;
+            else
+              reinterpret_cast<uint2 *>(d)[i] =
+                  uint2{pack2<T>(v.x, v.y), pack2<T>(v.z, v.w)};
+          });
       const int e = quads * 4 + lane;
       if (!QUADS && e < rows * V) d[e] = from_f<T>(image[e]);
     } else {
-      each_element([&](int at, int r, int c) {
-        d[(int64_t)r * p.d_stride + c] = from_f<T>(image[at]);
-      });
+      each_of(
+          V, [&](int r, int c) { return image[r * P + c]; },
+          [&](int r, int c, float v) {
+            d[(int64_t)r * p.d_stride + c] = from_f<T>(v);
+          });
     }
   }
 }
@@ -2015,7 +2087,13 @@ void launch_tiny(TinyArgs &p, cudaStream_t st) {
   };
   p.packed = packed(p.a.x, p.a.stride);
   p.d_packed = packed(p.dx, p.d_stride);
-  const size_t smem = (size_t)((32 * p.pitch + 3) / 4 * 4) * 4 * sizeof(float);
+  static std::atomic<uint64_t> done[2] = {};
+  size_t smem = (size_t)((32 * p.pitch + 3) / 4 * 4) * 4 * sizeof(float);
+  if (MODE == kLoss || MODE == kLossGrad) {
+    allow(k_tiny<T, MODE, true>, done[0]);
+    allow(k_tiny<T, MODE, false>, done[1]);
+    smem += (size_t)4 * 64 * (p.te.k | 1) * sizeof(float);
+  }
   const uint32_t grid = (p.a.rows + 127) / 128;
   if (quads)
     k_tiny<T, MODE, true><<<grid, 128, smem, st>>>(p);
