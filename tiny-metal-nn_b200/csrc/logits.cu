@@ -106,28 +106,12 @@ __device__ __forceinline__ float load_value(const void *p, int64_t i,
 template <class T>
 constexpr int kElems = 16 / (int)sizeof(T);
 
-__device__ __forceinline__ uint64_t f2(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
+__device__ __forceinline__ float2 f2(float a, float b) {
+  return make_float2(a, b);
 }
-__device__ __forceinline__ void f2_split(uint64_t v, float &a, float &b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
+__device__ __forceinline__ void split(float2 v, float &a, float &b) {
+  a = v.x;
+  b = v.y;
 }
 
 __device__ __forceinline__ uint32_t word(const uint4 &g, int i) {
@@ -135,19 +119,19 @@ __device__ __forceinline__ uint32_t word(const uint4 &g, int i) {
 }
 // the i-th pair of a granule's values
 template <class T>
-__device__ __forceinline__ uint64_t pair_of(const uint4 &g, int i);
+__device__ __forceinline__ float2 pair_of(const uint4 &g, int i);
 template <>
-__device__ __forceinline__ uint64_t pair_of<float>(const uint4 &g, int i) {
+__device__ __forceinline__ float2 pair_of<float>(const uint4 &g, int i) {
   return f2(__uint_as_float(word(g, 2 * i)), __uint_as_float(word(g, 2 * i + 1)));
 }
 template <>
-__device__ __forceinline__ uint64_t pair_of<__half>(const uint4 &g, int i) {
+__device__ __forceinline__ float2 pair_of<__half>(const uint4 &g, int i) {
   const uint32_t w = word(g, i);
   const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
-  return f2(f.x, f.y);
+  return f;
 }
 template <>
-__device__ __forceinline__ uint64_t pair_of<__nv_bfloat16>(const uint4 &g,
+__device__ __forceinline__ float2 pair_of<__nv_bfloat16>(const uint4 &g,
                                                            int i) {
   const uint32_t w = word(g, i);
   return f2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
@@ -196,7 +180,7 @@ struct GranuleMax {
     const uint4 g{two(two(m[0], m[1]), two(m[2], m[3])), 0, 0, 0};
     if constexpr (sizeof(T) == 4) return __uint_as_float(g.x);
     float a, b;
-    f2_split(pair_of<T>(g, 0), a, b);
+    split(pair_of<T>(g, 0), a, b);
     return max_nan(a, b);
   }
 };
@@ -204,18 +188,18 @@ struct GranuleMax {
 // s += sum e^t and, if U, u += sum e^t t log2(e) over a granule, in two lanes;
 // nm = -max and c = log2(e) / T twice
 template <class T, bool U>
-__device__ __forceinline__ void accumulate(const uint4 &g, uint64_t nm,
-                                           uint64_t c, uint64_t &s,
-                                           uint64_t &u) {
+__device__ __forceinline__ void accumulate(const uint4 &g, float2 nm,
+                                           float2 c, float2 &s,
+                                           float2 &u) {
 #pragma unroll
   for (int i = 0; i < kElems<T> / 2; ++i) {
-    const uint64_t t = f2_mul(f2_add(pair_of<T>(g, i), nm), c);
+    const float2 t = __fmul2_rn(__fadd2_rn(pair_of<T>(g, i), nm), c);
     float a, b;
-    f2_split(t, a, b);
-    const uint64_t e = f2(ex2(a), ex2(b));
-    s = f2_add(s, e);
+    split(t, a, b);
+    const float2 e = f2(ex2(a), ex2(b));
+    s = __fadd2_rn(s, e);
     // where t is -inf e is 0: a finite t keeps 0 * t from being NaN
-    if (U) u = f2_fma(e, f2(fmaxf(a, -1e4f), fmaxf(b, -1e4f)), u);
+    if (U) u = __ffma2_rn(e, f2(fmaxf(a, -1e4f), fmaxf(b, -1e4f)), u);
   }
 }
 
@@ -338,6 +322,24 @@ __device__ __forceinline__ void write_read_padding(const LogprobOut &o,
   if (o.entropy) o.entropy[row] = 0.0f;
   if (o.stats)
     for (int i = 0; i < 3; ++i) o.stats[(int64_t)row * 3 + i] = 0.0f;
+}
+
+// zeros in a row's gradient, in granules of its own alignment; by all threads
+template <class T, int NT>
+__device__ __forceinline__ void write_zeros(T *d, int n) {
+  constexpr int E = kElems<T>;
+  const int dm = (int)((uintptr_t)d & 15) / (int)sizeof(T);
+  uint4 *base = reinterpret_cast<uint4 *>(d - dm);
+  for (int g = threadIdx.x; g * E < dm + n; g += NT) {
+    if (g * E >= dm && (g + 1) * E <= dm + n) {
+      base[g] = uint4{0, 0, 0, 0};
+    } else {
+      for (int j = 0; j < E; ++j) {
+        const int e = g * E + j - dm;
+        if (e >= 0 && e < n) d[e] = from_f<T>(0.0f);
+      }
+    }
+  }
 }
 
 // ------------------------------------------------------------ a team a row
@@ -483,21 +485,7 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
              ? static_cast<T *>(p.dx) + (int64_t)row * p.d_stride + first
              : nullptr;
   if (idle) {
-    if constexpr (MODE == kLossGrad) {
-      // zeros in granules of the gradient's own alignment
-      const int dm = (int)((uintptr_t)d & 15) / (int)sizeof(T);
-      uint4 *base = reinterpret_cast<uint4 *>(d - dm);
-      for (int g = tid; g * E < dm + n; g += NT) {
-        if (g * E >= dm && (g + 1) * E <= dm + n) {
-          base[g] = uint4{0, 0, 0, 0};
-        } else {
-          for (int j = 0; j < E; ++j) {
-            const int e = g * E + j - dm;
-            if (e >= 0 && e < n) d[e] = from_f<T>(0.0f);
-          }
-        }
-      }
-    }
+    if constexpr (MODE == kLossGrad) write_zeros<T, NT>(d, n);
     copies_done();
     return;  // all CTAs of the cluster alike
   }
@@ -542,8 +530,8 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
   float mine = -kInf;
   Stat st;
   {
-    const uint64_t c2 = f2(a.c, a.c);
-    uint64_t s2 = 0, u2 = 0;
+    const float2 c2 = f2(a.c, a.c);
+    float2 s2 = f2(0.0f, 0.0f), u2 = s2;
     for (int g0 = tid; g0 < G; g0 += kBatch * NT) {
       uint4 q[kBatch];
 #pragma unroll
@@ -557,19 +545,19 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
       const float m0 = m == -kInf ? 0.0f : m;
       const float dm = (mine - m0) * a.c, f = ex2(dm);
       mine = m;
-      s2 = f2_mul(s2, f2(f, f));
+      s2 = __fmul2_rn(s2, f2(f, f));
       if (kReads) {
         const float dd = fmaxf(dm, -1e4f);
-        u2 = f2_fma(u2, f2(f, f), f2_mul(s2, f2(dd, dd)));
+        u2 = __ffma2_rn(u2, f2(f, f), __fmul2_rn(s2, f2(dd, dd)));
       }
-      const uint64_t nm = f2(-m0, -m0);
+      const float2 nm = f2(-m0, -m0);
 #pragma unroll
       for (int i = 0; i < kBatch; ++i)
         accumulate<T, kReads>(q[i], nm, c2, s2, u2);
     }
     float s0, s1, u0, u1;
-    f2_split(s2, s0, s1);
-    f2_split(u2, u0, u1);
+    split(s2, s0, s1);
+    split(u2, u0, u1);
     st = Stat{mine, s0 + s1, u0 + u1};
   }
   st = warp_combine(st, a.c);
@@ -692,7 +680,7 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
 #pragma unroll
           for (int i = 0; i < E / 2; ++i) {
             float f[2];
-            f2_split(pair_of<T>(q4, i >> 1), f[0], f[1]);
+            split(pair_of<T>(q4, i >> 1), f[0], f[1]);
             const float v = f[i & 1];
             if (v >= floor) {
               const uint64_t key =
@@ -783,7 +771,7 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
     const float ws = bad ? nan : empty ? 0.0f : w / s;
     // an empty row: 0 * 0 (its logits at -inf give e = 0 against m = 0)
     const float m0 = empty ? 0.0f : m;
-    const uint64_t nm = f2(-m0, -m0), c2 = f2(a.c, a.c), w2 = f2(ws, ws);
+    const float2 nm = f2(-m0, -m0), c2 = f2(a.c, a.c), w2 = f2(ws, ws);
     const int dm = (int)((uintptr_t)d & 15) / (int)sizeof(T);
     if (dm == mis) {
       uint4 *dst = reinterpret_cast<uint4 *>(d - dm);
@@ -794,8 +782,8 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
 #pragma unroll
         for (int i = 0; i < E / 2; ++i) {
           float u, v;
-          f2_split(f2_mul(f2_add(pair_of<T>(q, i), nm), c2), u, v);
-          f2_split(f2_mul(f2(ex2(u), ex2(v)), w2), r[2 * i], r[2 * i + 1]);
+          split(__fmul2_rn(__fadd2_rn(pair_of<T>(q, i), nm), c2), u, v);
+          split(__fmul2_rn(f2(ex2(u), ex2(v)), w2), r[2 * i], r[2 * i + 1]);
         }
         if (g * E >= mis && (g + 1) * E <= mis + n) {
           dst[g] = pack_granule<T>(r);
@@ -846,7 +834,11 @@ struct StreamArgs {
   int itype, top_k;
   LogprobOut o;
   Teacher te;
+  const float *row_weight;
+  float weight;
   float *loss;
+  void *dx;
+  int64_t d_stride;
 };
 
 // The largest value, of those with the low 16 bits zero (all there is to a
@@ -872,10 +864,13 @@ __global__ void __launch_bounds__(NT) k_stream(StreamArgs p) {
   constexpr bool kReads = MODE == kRead || MODE == kReadTop;
   constexpr bool kTop = MODE == kReadTop;
   __shared__ float part[kWarps * 3];
-  __shared__ float run_max[kTop ? kRuns * NT : 1];
+  __shared__ float run_max[kTop ? (kRuns + 1) * NT : 1];
   __shared__ uint32_t gmax[kTop ? NT : 1], runs[kTop ? kPicked : 1];
   __shared__ uint64_t picked[kTop ? kPicked : 1];
   __shared__ uint32_t misc[4];  // runs to read, tau, logits picked
+  constexpr bool kGrad = MODE == kLossGrad;
+  __shared__ float sq[kGrad ? kMaxTop : 1];
+  __shared__ int32_t sid[kGrad ? kMaxTop : 1];
   const RowArgs &a = p.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t row = blockIdx.x;
@@ -887,13 +882,45 @@ __global__ void __launch_bounds__(NT) k_stream(StreamArgs p) {
   const int mis = (int)((uintptr_t)x & 15) / (int)sizeof(T);
   const int head = min(mis ? E - mis : 0, V), F = (V - head) / E;
   const uint4 *src = reinterpret_cast<const uint4 *>(x + head);
-  uint4 q[kBatch], next[kBatch];
-  auto load = [&](uint4 *to, int f0) {
+  T *d = kGrad ? static_cast<T *>(p.dx) + (int64_t)row * p.d_stride : nullptr;
+  // The row in batches, body(granules, first one): the last, short one first,
+  // then the whole ones, each loaded while the one before is worked on.
+  constexpr bool kAhead = MODE == kRead && NT > 128;
+  const int whole = F / (kBatch * NT);
+  const bool rest = F > whole * kBatch * NT;
+  auto load = [&](uint4 *to, int b) {
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i)
-      to[i] = f0 + i * NT + tid < F ? src[f0 + i * NT + tid] : no_logits<T>();
+    for (int i = 0; i < kBatch; ++i) to[i] = src[(b * kBatch + i) * NT + tid];
   };
-  load(q, 0);
+  auto load_last = [&](uint4 *to) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int f = (whole * kBatch + i) * NT + tid;
+      to[i] = f < F ? src[f] : no_logits<T>();
+    }
+  };
+  auto sweep = [&](uint4 *one, auto &&body) {  // one: the last batch
+    if constexpr (!kAhead) {
+      if (rest) body(one, whole);
+      for (int b = 0; b < whole; ++b) {
+        load(one, b);
+        body(one, b);
+      }
+      return;
+    }
+    uint4 two[kBatch];
+    if (whole) load(two, 0);
+    if (rest) body(one, whole);
+    for (int b = 0; b < whole;) {
+      if (b + 1 < whole) load(one, b + 1);
+      body(two, b++);
+      if (b == whole) break;
+      if (b + 1 < whole) load(two, b + 1);
+      body(one, b++);
+    }
+  };
+  uint4 q[kBatch];
+  if (rest) load_last(q);
   // the elements outside whole granules, one a lane of the first warp
   float odd = -kInf;
   int odd_class = 0;
@@ -906,6 +933,7 @@ __global__ void __launch_bounds__(NT) k_stream(StreamArgs p) {
   int64_t tok = 0;
   float tok_x = 0.0f;
   [[maybe_unused]] float ty[4], xk[4], ym = -kInf;
+  [[maybe_unused]] int32_t tid_[4];
   if constexpr (kReads) {
     if (p.tokens) tok = load_index(p.tokens, row, p.itype);
     if (tok < 0) {
@@ -924,6 +952,7 @@ __global__ void __launch_bounds__(NT) k_stream(StreamArgs p) {
     for (int i = 0; i < 4; ++i) {
       ty[i] = -kInf;
       xk[i] = 0.0f;
+      tid_[i] = -1;
       const int k = lane + 32 * i;
       if (k >= p.te.k) continue;
       const int64_t at = (int64_t)row * p.te.k + k;
@@ -931,12 +960,14 @@ __global__ void __launch_bounds__(NT) k_stream(StreamArgs p) {
       const float y = load_value(p.te.logits, at, p.te.dtype);
       if (id < 0 || y == -kInf) continue;  // left out
       ty[i] = id < V ? y : nan;
+      tid_[i] = id < V ? (int32_t)id : 0;
       if (warp == 0 && id < V) xk[i] = to_f(x[id]);
       ym = max_nan(ym, ty[i]);
     }
     for (int o = 16; o; o >>= 1) ym = max_nan(ym, __shfl_xor_sync(~0u, ym, o));
     if (ym == -kInf) {
       if (tid == 0) p.loss[row] = 0.0f;
+      if constexpr (kGrad) write_zeros<T, NT>(d, V);
       return;
     }
   }
@@ -944,52 +975,53 @@ __global__ void __launch_bounds__(NT) k_stream(StreamArgs p) {
 
   // ---- the stream
   Stat st{-kInf, 0.0f, 0.0f};
-  uint64_t s2 = 0, u2 = 0;
-  const uint64_t c2 = f2(a.c, a.c);
-  // a run is `per` batches
-  const int per = (F + kBatch * NT * kRuns - 1) / (kBatch * NT * kRuns);
+  float2 s2 = f2(0.0f, 0.0f), u2 = s2;
+  const float2 c2 = f2(a.c, a.c);
+  // a run is `per` batches, the last batch one of its own
+  const int per = max(1, (whole + kRuns - 1) / kRuns);
   int run = 0, in_run = 0;
   float run_of = -kInf;
-  for (int f0 = 0; f0 < F || f0 == 0; f0 += kBatch * NT) {
-    load(next, f0 + kBatch * NT);
+  // the logits outside whole granules, first of all
+  if (warp == 0) {
+    const float m0 = odd == -kInf ? 0.0f : odd;
+    const float t = (odd - m0) * a.c, e = ex2(t);
+    st.m = odd;
+    s2 = f2(e, 0.0f);
+  }
+  sweep(q, [&](const uint4 *g, int b) {
     GranuleMax<T> gm;
     gm.clear();
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) gm.add(q[i]);
-    float bm = gm.get();
-    const float batch = bm;
-    if (f0 == 0 && warp == 0) bm = max_nan(bm, odd);
-    const float m = max_nan(st.m, bm), m0 = m == -kInf ? 0.0f : m;
+    for (int i = 0; i < kBatch; ++i) gm.add(g[i]);
+    const float batch = gm.get();
+    const float m = max_nan(st.m, batch), m0 = m == -kInf ? 0.0f : m;
     const float dm = (st.m - m0) * a.c, f = ex2(dm);
     st.m = m;
-    s2 = f2_mul(s2, f2(f, f));
+    s2 = __fmul2_rn(s2, f2(f, f));
     if (kReads) {
       const float dd = fmaxf(dm, -1e4f);
-      u2 = f2_fma(u2, f2(f, f), f2_mul(s2, f2(dd, dd)));
+      u2 = __ffma2_rn(u2, f2(f, f), __fmul2_rn(s2, f2(dd, dd)));
     }
-    const uint64_t nm = f2(-m0, -m0);
+    const float2 nm = f2(-m0, -m0);
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) accumulate<T, kReads>(q[i], nm, c2, s2, u2);
-    if (f0 == 0 && warp == 0) {
-      const float t = (odd - m0) * a.c, e = ex2(t);
-      s2 = f2_add(s2, f2(e, 0.0f));
-      u2 = f2_fma(f2(e, 0.0f), f2(fmaxf(t, -1e4f), 0.0f), u2);
-    }
+    for (int i = 0; i < kBatch; ++i) accumulate<T, kReads>(g[i], nm, c2, s2, u2);
     if constexpr (kTop) {
-      run_of = fmaxf(run_of, batch);
-      if (++in_run == per) {
-        run_max[run++ * NT + tid] = run_of;
-        run_of = -kInf;
-        in_run = 0;
+      if (b == whole) {
+        run_max[kRuns * NT + tid] = batch;
+      } else {
+        run_of = fmaxf(run_of, batch);
+        if (++in_run == per) {
+          run_max[run++ * NT + tid] = run_of;
+          run_of = -kInf;
+          in_run = 0;
+        }
       }
     }
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) q[i] = next[i];
-  }
+  });
   {
     float s0, s1, u0, u1;
-    f2_split(s2, s0, s1);
-    f2_split(u2, u0, u1);
+    split(s2, s0, s1);
+    split(u2, u0, u1);
     st.s = s0 + s1;
     st.u = u0 + u1;
   }
@@ -1004,7 +1036,7 @@ __global__ void __launch_bounds__(NT) k_stream(StreamArgs p) {
     part[warp * 3 + 2] = st.u;
   }
   __syncthreads();
-  if (!kTop && warp) return;
+  if (!kTop && !kGrad && warp) return;
   st = Stat{-kInf, 0.0f, 0.0f};
   if (lane < kWarps)
     st = Stat{part[lane * 3], part[lane * 3 + 1], part[lane * 3 + 2]};
@@ -1015,6 +1047,8 @@ __global__ void __launch_bounds__(NT) k_stream(StreamArgs p) {
     if (tid == 0) write_read(p.o, row, end, tok_x, tok < V);
   } else {
     end.bad |= !(ym < kInf);
+  }
+  if (!kReads && warp == 0) {
     float tq[4], ys = 0.0f, l = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -1032,6 +1066,58 @@ __global__ void __launch_bounds__(NT) k_stream(StreamArgs p) {
                        : tq[i] / ys * ((ty[i] - ln_ys) - end.logp(xk[i]));
     for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
     if (lane == 0) p.loss[row] = end.bad ? nan : a.t * a.t * l;
+    if constexpr (kGrad) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = lane + 32 * i;
+        if (k < p.te.k) {
+          sq[k] = tq[i] / ys;
+          sid[k] = tid_[i];
+        }
+      }
+    }
+  }
+  if constexpr (kGrad) {
+    const float w = (p.row_weight ? p.row_weight[row] : p.weight) * a.t;
+    const float ws = end.bad ? nan : end.empty ? 0.0f : w / end.s;
+    // an empty row: 0 * 0 (its logits at -inf give e = 0 against m = 0)
+    const float m0 = end.empty ? 0.0f : end.m;
+    const float2 nm = f2(-m0, -m0), w2 = f2(ws, ws);
+    if ((int)((uintptr_t)d & 15) == mis * (int)sizeof(T)) {
+      uint4 *dst = reinterpret_cast<uint4 *>(d + head);
+      if (rest) load_last(q);
+      sweep(q, [&](const uint4 *g, int b) {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          float r[E];
+#pragma unroll
+          for (int j = 0; j < E / 2; ++j) {
+            const float2 t = __fmul2_rn(__fadd2_rn(pair_of<T>(g[i], j), nm), c2);
+            split(__fmul2_rn(f2(ex2(t.x), ex2(t.y)), w2), r[2 * j], r[2 * j + 1]);
+          }
+          const int f = (b * kBatch + i) * NT + tid;
+          if (b < whole || f < F) dst[f] = pack_granule<T>(r);
+        }
+      });
+      if (warp == 0 && lane < 16 && (lane < 8 ? lane < head : odd_class < V))
+        d[odd_class] = from_f<T>(ex2((odd - m0) * a.c) * ws);
+    } else {
+      // rows of another alignment: element by element, lanes side by side
+#pragma unroll 8
+      for (int e = tid; e < V; e += NT)
+        d[e] = from_f<T>(ex2((to_f(x[e]) - m0) * a.c) * ws);
+    }
+    __syncthreads();  // an entry's element is written again, after its first value
+    if (warp == 0 && !end.bad && !end.empty) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (tid_[i] < 0) continue;
+        float both = 0.0f;  // entries of one class add up
+        for (int j = 0; j < p.te.k; ++j) both += sid[j] == tid_[i] ? sq[j] : 0.0f;
+        d[tid_[i]] =
+            from_f<T>(w * (ex2((xk[i] - end.m) * a.c) / end.s - both));
+      }
+    }
   }
   if constexpr (kTop) {
     const int K = p.top_k;
@@ -1053,8 +1139,8 @@ __global__ void __launch_bounds__(NT) k_stream(StreamArgs p) {
     __syncthreads();
     const uint32_t tau = misc[1];
     const float floor = value_of(tau);
-    for (int r = 0; r < run; ++r)
-      if (run_max[r * NT + tid] >= floor) {
+    for (int r = 0; r <= kRuns; ++r)
+      if ((r < run || (r == kRuns && rest)) && run_max[r * NT + tid] >= floor) {
         const uint32_t at = atomicAdd(misc, 1u);
         if (at < kPicked) runs[at] = (uint32_t)(r << 16 | tid);
       }
@@ -1069,14 +1155,16 @@ __global__ void __launch_bounds__(NT) k_stream(StreamArgs p) {
 #pragma unroll
         for (int j = 0; j < E; ++j) {
           float v[2];
-          f2_split(pair_of<T>(w, j >> 1), v[0], v[1]);
+          split(pair_of<T>(w, j >> 1), v[0], v[1]);
           if (v[j & 1] >= floor) f(key_of(v[j & 1], head + g * E + j));
         }
       };
       for (int i = tid; i < todo * of; i += NT) {
         const uint32_t r = runs[i / of];
-        const int g = ((int)(r >> 16) * of + i % of) * NT + (int)(r & 0xFFFF);
-        if (g < F) granule(g);
+        const bool end_run = r >> 16 == kRuns;
+        const int at = (end_run ? whole * kBatch : (int)(r >> 16) * of) + i % of;
+        const int g = at * NT + (int)(r & 0xFFFF);
+        if (end_run ? g < F : at < whole * kBatch) granule(g);
       }
       if (over)
         for (int g = tid; g < F; g += NT) granule(g);
@@ -1270,8 +1358,8 @@ __global__ void __launch_bounds__(128) k_tiny(TinyArgs p) {
           [&](int at, int, const uint2 &w) {
             const uint4 g{w.x, w.y, 0, 0};
             float4 v;
-            f2_split(pair_of<T>(g, 0), v.x, v.y);
-            f2_split(pair_of<T>(g, 1), v.z, v.w);
+            split(pair_of<T>(g, 0), v.x, v.y);
+            split(pair_of<T>(g, 1), v.z, v.w);
             *reinterpret_cast<float4 *>(image + at) = v;
           });
     }
@@ -1378,9 +1466,9 @@ __global__ void __launch_bounds__(128) k_tiny(TinyArgs p) {
       }
       Stat st{max8(best), 0.0f, 0.0f};
       const float m0 = st.m == -kInf ? 0.0f : st.m;
-      const uint64_t nm = f2(-m0, -m0), c2 = f2(a.c, a.c);
+      const float2 nm = f2(-m0, -m0), c2 = f2(a.c, a.c);
       {
-        uint64_t s2 = 0, u2 = 0;
+        float2 s2 = f2(0.0f, 0.0f), u2 = s2;
 #pragma unroll 2
         for (int j = 0; j < eights; ++j) {
           float v[8];
@@ -1393,8 +1481,8 @@ __global__ void __launch_bounds__(128) k_tiny(TinyArgs p) {
                 nm, c2, s2, u2);
         }
         float s0, s1, u0, u1;
-        f2_split(s2, s0, s1);
-        f2_split(u2, u0, u1);
+        split(s2, s0, s1);
+        split(u2, u0, u1);
         st.s = s0 + s1;
         st.u = u0 + u1;
       }
@@ -1482,7 +1570,7 @@ __global__ void __launch_bounds__(128) k_tiny(TinyArgs p) {
                                 : a.t * a.t * (loss * inv_ys - logf(ys));
         if constexpr (MODE == kLossGrad) {
           const float ws = zero ? 0.0f : end.bad ? nan : w / end.s;
-          const uint64_t w2 = f2(ws, ws);
+          const float2 w2 = f2(ws, ws);
 #pragma unroll 2
           for (int j = 0; j < eights; ++j) {
             float v[8];
@@ -1490,8 +1578,8 @@ __global__ void __launch_bounds__(128) k_tiny(TinyArgs p) {
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
               float t, u;
-              f2_split(f2_mul(f2_add(f2(v[i], v[i + 1]), nm), c2), t, u);
-              f2_split(f2_mul(f2(ex2(t), ex2(u)), w2), v[i], v[i + 1]);
+              split(__fmul2_rn(__fadd2_rn(f2(v[i], v[i + 1]), nm), c2), t, u);
+              split(__fmul2_rn(f2(ex2(t), ex2(u)), w2), v[i], v[i + 1]);
               if (zero) v[i] = v[i + 1] = 0.0f;
             }
             write_eight(j, v);
@@ -1628,7 +1716,7 @@ __global__ void __launch_bounds__(128) k_narrow(NarrowArgs p) {
 #pragma unroll
       for (int i = 0; i < E / 2; ++i) {
         float u, v;
-        f2_split(pair_of<T>(q[j], i), u, v);
+        split(pair_of<T>(q[j], i), u, v);
         r[2 * i] = f(u, e0 + 2 * i);
         r[2 * i + 1] = f(v, e0 + 2 * i + 1);
       }
@@ -1694,15 +1782,15 @@ __global__ void __launch_bounds__(128) k_narrow(NarrowArgs p) {
   st.m = group_max(gm.get());
   {
     const float m0 = st.m == -kInf ? 0.0f : st.m;
-    const uint64_t nm = f2(-m0, -m0), c2 = f2(a.c, a.c);
-    uint64_t s2 = 0, u2 = 0;
+    const float2 nm = f2(-m0, -m0), c2 = f2(a.c, a.c);
+    float2 s2 = f2(0.0f, 0.0f), u2 = s2;
 #pragma unroll
     for (int j = 0; j < NG; ++j)
       if (l + L * j < (mis + V + E - 1) / E)
         accumulate<T, kReads>(q[j], nm, c2, s2, u2);
     float s0, s1, u0, u1;
-    f2_split(s2, s0, s1);
-    f2_split(u2, u0, u1);
+    split(s2, s0, s1);
+    split(u2, u0, u1);
     st.s = group_sum(s0 + s1);
     st.u = kReads ? group_sum(u0 + u1) : 0.0f;
   }
@@ -1746,7 +1834,7 @@ __global__ void __launch_bounds__(128) k_narrow(NarrowArgs p) {
 #pragma unroll
         for (int i = E - 1; i >= 0; --i) {
           float f[2];
-          f2_split(pair_of<T>(w, i >> 1), f[0], f[1]);
+          split(pair_of<T>(w, i >> 1), f[0], f[1]);
           if (f[i & 1] == v) where = i;
         }
         cls = (l + L * at) * E + where - mis;
@@ -1858,7 +1946,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
         for (int j = 0; j < E / 2; ++j) {
           float u, v;
-          f2_split(pair_of<T>(q[i], j), u, v);
+          split(pair_of<T>(q[i], j), u, v);
           r[2 * j] = b.at(u, e0 + 2 * j, a.c);
           r[2 * j + 1] = b.at(v, e0 + 2 * j + 1, a.c);
         }
@@ -2067,7 +2155,15 @@ bool streams(const RowArgs &a) {
 }
 template <class T, int MODE>
 void launch_stream(const TeamArgs &p, cudaStream_t st) {
-  const StreamArgs q{p.a, p.tokens, p.itype, p.top_k, p.o, p.te, p.loss};
+  const StreamArgs q{p.a,  p.tokens,     p.itype,  p.top_k, p.o,       p.te,
+                     p.row_weight, p.weight, p.loss, p.dx, p.d_stride};
+  if constexpr (MODE == kLossGrad) {
+    if ((int64_t)p.a.classes * (int)sizeof(T) > 128 * 1024) {
+      k_stream<T, 1024, MODE><<<p.a.rows, 1024, 0, st>>>(q);
+      check_launch(cudaGetLastError());
+      return;
+    }
+  }
   // a few batches a thread at least, and maxima well above the alternatives in
   // number
   if (p.a.classes <= 4 * 4 * 256 * kElems<T> && (MODE != kReadTop || p.top_k <= 32))
@@ -2344,6 +2440,8 @@ int launch_distill(const tmnn_logits &x, const void *ids, int index_type,
         BY_DTYPE(x.dtype, (launch_narrow<T, kLoss>(q, x.dtype, st)));
     } else if (!d_logits && streams(p.a)) {
       BY_DTYPE(x.dtype, (launch_stream<T, kLoss>(p, st)));
+    } else if (d_logits && streams(p.a)) {
+      BY_DTYPE(x.dtype, (launch_stream<T, kLossGrad>(p, st)));
     } else if (d_logits) {
       BY_DTYPE(x.dtype, (launch_team<T, kLossGrad>(p, st)));
     } else {

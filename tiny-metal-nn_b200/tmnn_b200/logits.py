@@ -11,15 +11,32 @@ is recorded (the backward passes are calls of their own, as in the Trainer's
 split API)."""
 from __future__ import annotations
 
-import ctypes as C
 from typing import NamedTuple, Optional
 
 from . import _abi
 from ._abi import lib
 
-_DTYPE = {"torch.float32": _abi.DTYPE_F32, "torch.float16": _abi.DTYPE_F16,
-          "torch.bfloat16": _abi.DTYPE_BF16}
-_INDEX = {"torch.int32": _abi.INDEX_I32, "torch.int64": _abi.INDEX_I64}
+# torch, its dtypes' C values and the function that gives a device's current
+# stream; filled at the first call (importing this package does not import
+# torch, and small calls cost as much in Python as on the GPU)
+_torch = None
+_DTYPE: dict = {}
+_INDEX: dict = {}
+_F32: dict = {}
+_raw_stream = None
+
+
+def _load_torch():
+    global _torch, _raw_stream
+    import torch
+    _DTYPE.update({torch.float32: _abi.DTYPE_F32, torch.float16: _abi.DTYPE_F16,
+                   torch.bfloat16: _abi.DTYPE_BF16})
+    _INDEX.update({torch.int32: _abi.INDEX_I32, torch.int64: _abi.INDEX_I64})
+    _F32[torch.float32] = _abi.DTYPE_F32
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+        lambda index: torch.cuda.current_stream(index).cuda_stream)
+    _torch = torch
+    return torch
 
 
 class TokenLogprobs(NamedTuple):
@@ -52,50 +69,49 @@ def _logits(x, temperature):
     """The C descriptor of a [n, classes] tensor of logits."""
     if not getattr(x, "is_cuda", False):
         raise ValueError("logits must be a CUDA tensor")
-    dtype = _DTYPE.get(str(x.dtype))
+    if _torch is None:
+        _load_torch()
+    dtype = _DTYPE.get(x.dtype)
     if dtype is None:
         raise _dtype_error(
             f"logits must be float32, float16 or bfloat16, got {x.dtype}")
     if x.dim() != 2:
         raise ValueError("logits must be 2D (rows, classes)")
     n, v = x.shape
-    if v > 1 and x.stride(1) != 1:
+    stride, step = x.stride()
+    if step != 1 and v > 1:
         raise ValueError("the classes of a row of logits must be contiguous")
     if n >= 1 << 32 or v >= 1 << 32:
         raise ValueError("logits must have fewer than 2^32 rows and classes")
-    return _abi.Logits(x.data_ptr(), x.stride(0), n, v, dtype, temperature)
+    return _abi.Logits(x.data_ptr(), stride, n, v, dtype, temperature)
 
 
-def _vector(t, name, like, shape, kinds):
-    """Pointer of a contiguous tensor of the given shape on like's device;
+def _vector(t, name, device, shape, kinds):
+    """(pointer, C type) of a contiguous tensor of the given shape on `device`;
     `kinds` maps the dtypes it may have to their C values."""
-    if not getattr(t, "is_cuda", False) or t.device != like.device:
+    if not getattr(t, "is_cuda", False) or t.device != device:
         raise ValueError(f"{name} must be a CUDA tensor on the logits' device")
-    kind = kinds.get(str(t.dtype))
+    kind = kinds.get(t.dtype)
     if kind is None:
         raise _dtype_error(f"{name} must be "
-                           + " or ".join(k[6:] for k in kinds)
+                           + " or ".join(str(k)[6:] for k in kinds)
                            + f", got {t.dtype}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
     return t.data_ptr(), kind
 
 
-_F32 = {"torch.float32": _abi.DTYPE_F32}
-
-
 def _gradient(out, x):
-    import torch
     if out is None:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        return _torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if (not getattr(out, "is_cuda", False) or out.device != x.device
             or out.shape != x.shape):
         raise ValueError("out must be a CUDA tensor of the logits' shape and device")
     if out.dtype != x.dtype:
         raise _dtype_error(f"out must have the logits' type {x.dtype}")
-    if out.dim() == 2 and out.shape[1] > 1 and out.stride(1) != 1:
+    if out.shape[1] > 1 and out.stride(1) != 1:
         raise ValueError("the classes of a row of out must be contiguous")
     return out
 
@@ -104,11 +120,6 @@ def _grad_stride(out):
     """Distance of the gradient's rows; of one row or none it is never used."""
     n, v = out.shape
     return out.stride(0) if n > 1 else max(v, out.stride(0))
-
-
-def _stream(x):
-    import torch
-    return x.device.index, torch.cuda.current_stream(x.device).cuda_stream
 
 
 def token_logprobs(logits, tokens=None, *, top_k=0, temperature=1.0,
@@ -121,26 +132,30 @@ def token_logprobs(logits, tokens=None, *, top_k=0, temperature=1.0,
     tokens [n]: int32 or int64; below 0 marks a padded row (results 0, no
     alternatives), at or above `classes` gives NaN.  stats=True also returns
     what token_logprobs_backward needs."""
-    import torch
     x = _logits(logits, temperature)
-    n = logits.shape[0]
-    tp, it = (None, 0) if tokens is None else _vector(tokens, "tokens", logits,
-                                                      (n,), _INDEX)
+    n, dev = x.rows, logits.device
     k = int(top_k)
-    if not 0 <= k <= min(logits.shape[1], _abi.MAX_TOP):
+    if not 0 <= k <= min(x.classes, _abi.MAX_TOP):
         raise ValueError("top_k must be in [0, min(classes, 128)]")
-    dev = logits.device
-    new = torch.empty
-    lp = None if tokens is None else new((n,), dtype=torch.float32, device=dev)
-    ent = new((n,), dtype=torch.float32, device=dev)
-    ids = new((n, k), dtype=torch.int32, device=dev) if k else None
-    top = new((n, k), dtype=torch.float32, device=dev) if k else None
-    st = new((n, 3), dtype=torch.float32, device=dev) if stats else None
-    d, s = _stream(logits)
+    empty, f32 = _torch.empty, _torch.float32
+    lp = lpp = tp = ids = top = idp = topp = st = stp = None
+    it = 0
+    if tokens is not None:
+        tp, it = _vector(tokens, "tokens", dev, (n,), _INDEX)
+        lp = empty(n, dtype=f32, device=dev)
+        lpp = lp.data_ptr()
+    ent = empty(n, dtype=f32, device=dev)
+    if k:
+        ids = empty(n, k, dtype=_torch.int32, device=dev)
+        top = empty(n, k, dtype=f32, device=dev)
+        idp, topp = ids.data_ptr(), top.data_ptr()
+    if stats:
+        st = empty(n, 3, dtype=f32, device=dev)
+        stp = st.data_ptr()
+    index = dev.index
     _check(lib.tmnn_cuda_token_logprobs(
-        d, s, x, tp, it, k, None if lp is None else lp.data_ptr(),
-        ent.data_ptr(), ids.data_ptr() if k else None,
-        top.data_ptr() if k else None, st.data_ptr() if stats else None))
+        index, _raw_stream(index), x, tp, it, k, lpp, ent.data_ptr(), idp, topp,
+        stp))
     return TokenLogprobs(lp, ent, ids, top, st)
 
 
@@ -153,38 +168,39 @@ def token_logprobs_backward(logits, tokens, stats, d_logprob=None,
     may be `logits` itself, whose values are then lost.  The alternatives'
     log probabilities carry no gradient."""
     x = _logits(logits, temperature)
-    n = logits.shape[0]
-    tp, it = (None, 0) if tokens is None else _vector(tokens, "tokens", logits,
+    n, dev = x.rows, logits.device
+    tp, it = (None, 0) if tokens is None else _vector(tokens, "tokens", dev,
                                                       (n,), _INDEX)
-    sp, _ = _vector(stats, "stats", logits, (n, 3), _F32)
-    gp = None if d_logprob is None else _vector(d_logprob, "d_logprob", logits,
+    sp, _ = _vector(stats, "stats", dev, (n, 3), _F32)
+    gp = None if d_logprob is None else _vector(d_logprob, "d_logprob", dev,
                                                 (n,), _F32)[0]
-    hp = None if d_entropy is None else _vector(d_entropy, "d_entropy", logits,
+    hp = None if d_entropy is None else _vector(d_entropy, "d_entropy", dev,
                                                 (n,), _F32)[0]
     out = _gradient(out, logits)
-    d, s = _stream(logits)
+    index = dev.index
     _check(lib.tmnn_cuda_token_logprobs_backward(
-        d, s, x, tp, it, sp, gp, hp, out.data_ptr(), _grad_stride(out)))
+        index, _raw_stream(index), x, tp, it, sp, gp, hp, out.data_ptr(),
+        _grad_stride(out)))
     return out
 
 
-def _distill(logits, teacher_ids, teacher_logits, temperature, row_weight, out):
-    import torch
-    x = _logits(logits, temperature)
-    n = logits.shape[0]
-    if teacher_ids.dim() != 2:
-        raise ValueError("teacher_ids must be 2D (rows, k)")
+def _distill(x, logits, teacher_ids, teacher_logits, row_weight, out):
+    n, dev = x.rows, logits.device
+    if not getattr(teacher_ids, "is_cuda", False) or teacher_ids.dim() != 2:
+        raise ValueError("teacher_ids must be a 2D CUDA tensor (rows, k)")
     k = teacher_ids.shape[1]
-    ip, it = _vector(teacher_ids, "teacher_ids", logits, (n, k), _INDEX)
-    yp, yt = _vector(teacher_logits, "teacher_logits", logits, (n, k), _DTYPE)
-    wp = None if row_weight is None else _vector(row_weight, "row_weight",
-                                                 logits, (n,), _F32)[0]
-    loss = torch.empty((n,), dtype=torch.float32, device=logits.device)
-    d, s = _stream(logits)
-    _check(lib.tmnn_cuda_distill(
-        d, s, x, ip, it, yp, yt, k, wp, loss.data_ptr(),
-        None if out is None else out.data_ptr(),
-        0 if out is None else _grad_stride(out)))
+    ip, it = _vector(teacher_ids, "teacher_ids", dev, (n, k), _INDEX)
+    yp, yt = _vector(teacher_logits, "teacher_logits", dev, (n, k), _DTYPE)
+    wp = dp = None
+    stride = 0
+    if row_weight is not None:
+        wp, _ = _vector(row_weight, "row_weight", dev, (n,), _F32)
+    if out is not None:
+        dp, stride = out.data_ptr(), _grad_stride(out)
+    loss = _torch.empty(n, dtype=_torch.float32, device=dev)
+    index = dev.index
+    _check(lib.tmnn_cuda_distill(index, _raw_stream(index), x, ip, it, yp, yt, k,
+                                 wp, loss.data_ptr(), dp, stride))
     return loss
 
 
@@ -195,7 +211,8 @@ def distill_loss(logits, teacher_ids, teacher_logits, *, temperature=1.0):
     teacher_ids [n, k] int32 or int64 (below 0: no entry; a row without
     entries is padding with loss 0), teacher_logits [n, k] float32, float16 or
     bfloat16 -- the top_ids and top_logprobs of token_logprobs fit both."""
-    return _distill(logits, teacher_ids, teacher_logits, temperature, None, None)
+    return _distill(_logits(logits, temperature), logits, teacher_ids,
+                    teacher_logits, None, None)
 
 
 def distill_forward_backward(logits, teacher_ids, teacher_logits, *,
@@ -204,7 +221,6 @@ def distill_forward_backward(logits, teacher_ids, teacher_logits, *,
     of the logits, the gradient of sum(row_weight * loss) in the logits' type.
     row_weight float32 [n]; None is 1 / n, the gradient of the mean loss.  out:
     where to write the gradient; it may be `logits` itself."""
-    _logits(logits, temperature)
+    x = _logits(logits, temperature)
     out = _gradient(out, logits)
-    return _distill(logits, teacher_ids, teacher_logits, temperature,
-                    row_weight, out), out
+    return _distill(x, logits, teacher_ids, teacher_logits, row_weight, out), out
