@@ -70,7 +70,8 @@ SIZES = [(1, 1), (3, 2), (40, 3), (13, 19), (70000, 5), (33, 31), (300, 64),
          (12, 65), (50, 127), (11, 257), (64, 1000), (5, 1023), (17, 1024),
          (17, 1025), (10, 2047), (12, 2311), (10, 4097), (21, 8192), (2, 32768),
          (11, 32003), (300, 5000), (1, 131072), (10, 50021), (3, 262143),
-         (12, 131071), (1, 524288), (320, 9001), (305, 33000), (600, 2500)]
+         (12, 131071), (1, 524288), (320, 9001), (305, 33000), (600, 2500),
+         (610, 24999), (300, 70001), (303, 40000)]
 DTYPES = ["f32", "bf16", "fp16"]
 
 

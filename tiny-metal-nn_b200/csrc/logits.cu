@@ -370,7 +370,7 @@ __host__ __device__ inline TeamLayout team_layout(int mode, int threads,
   l.stats = off;
   off += cluster * (threads / 32) * 16;
   l.teacher = off;
-  if (mode >= kLoss) off += (k * 8 + 15) / 16 * 16;
+  if (mode >= kLoss) off += (k * 8 + 4 + 15) / 16 * 16;
   l.misc = off;
   if (mode == kReadTop) {
     off += 16 + 2 * kMaxCluster * 4;  // count, threshold; counts of the CTAs
@@ -423,22 +423,21 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
   const int G = n > 0 ? (mis + n + E - 1) / E : 0;
   uint4 *slab = reinterpret_cast<uint4 *>(smem);
   T *sx = reinterpret_cast<T *>(smem) + mis;  // sx[e] = x[e]
+  // whole granules [lo, hi), the thread's from `mine0` on
+  const int lo = mis ? 1 : 0, hi = (mis + n) / E;
+  const int mine0 = lo && tid == 0 ? NT : tid;
+  // the thread's elements outside whole granules: f(element)
+  auto edges = [&](auto &&f) {
+    if (lo && tid == 0)
+      for (int j = 0; j < E; ++j) f(j - mis);
+    if (G > hi && (hi || !lo) && tid == hi % NT)
+      for (int j = 0; j < E; ++j) f(hi * E + j - mis);
+  };
   auto load = [&] {
     const uint4 *src = reinterpret_cast<const uint4 *>(x - mis);
-    const int lo = mis ? 1 : 0, hi = (mis + n) / E;  // whole granules
-    for (int g = tid; g < hi; g += NT)
-      if (g >= lo) copy16(slab + g, src + g);
-    // the first and last one, by the threads they belong to
-    if ((lo && tid == 0) || (G > hi && tid == hi % NT)) {
-      for (int i = 0; i < 2; ++i) {
-        const int g = i ? hi : 0;
-        if ((i ? G > hi : lo) && tid == g % NT)
-          for (int j = 0; j < E; ++j) {
-            const int e = g * E + j - mis;
-            sx[e] = e >= 0 && e < n ? x[e] : from_f<T>(-kInf);
-          }
-      }
-    }
+#pragma unroll 4
+    for (int g = mine0; g < hi; g += NT) copy16(slab + g, src + g);
+    edges([&](int e) { sx[e] = e >= 0 && e < n ? x[e] : from_f<T>(-kInf); });
   };
   if (p.eager) load();
 
@@ -446,6 +445,7 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
   int64_t tok = 0;
   float *sq = reinterpret_cast<float *>(smem + p.l.teacher);
   int32_t *sid = reinterpret_cast<int32_t *>(sq + p.te.k);
+  [[maybe_unused]] int32_t *bad_entries = sid + p.te.k;
   [[maybe_unused]] float ty[4], tq[4], ln_ys = 0.0f, ym = 0.0f;
   [[maybe_unused]] int32_t tid_[4];
   bool idle;
@@ -461,23 +461,31 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
         }
     }
   } else {
-    // Every warp reads the entries, entry lane + 32 i in register i.
+    // Entry lane + 32 i in register i of the first warp; the others only look
+    // whether there is any.
     ym = -kInf;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       ty[i] = -kInf;
       tid_[i] = -1;
       const int k = lane + 32 * i;
-      if (k >= p.te.k) continue;
-      const int64_t at = (int64_t)row * p.te.k + k;
-      const int64_t id = load_index(p.te.ids, at, p.te.itype);
-      const float y = load_value(p.te.logits, at, p.te.dtype);
-      if (id < 0 || y == -kInf) continue;  // left out
-      tid_[i] = id < a.classes ? (int32_t)id : 0;
-      ty[i] = id < a.classes ? y : nan;
-      ym = max_nan(ym, ty[i]);
+      if (k < p.te.k && (warp == 0 || ym == -kInf)) {
+        const int64_t at = (int64_t)row * p.te.k + k;
+        const int64_t id = load_index(p.te.ids, at, p.te.itype);
+        const float y = load_value(p.te.logits, at, p.te.dtype);
+        if (id >= 0 && y != -kInf) {  // not left out
+          tid_[i] = id < a.classes ? (int32_t)id : 0;
+          ty[i] = id < a.classes ? y : nan;
+          ym = max_nan(ym, ty[i]);
+        }
+      }
+      if (warp && __any_sync(~0u, ym != -kInf)) {
+        ym = 0.0f;
+        break;
+      }
     }
-    for (int o = 16; o; o >>= 1) ym = max_nan(ym, __shfl_xor_sync(~0u, ym, o));
+    if (warp == 0)
+      for (int o = 16; o; o >>= 1) ym = max_nan(ym, __shfl_xor_sync(~0u, ym, o));
     idle = ym == -kInf;
     if (idle && leader && tid == 0) p.loss[row] = 0.0f;
   }
@@ -494,29 +502,31 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
 
   [[maybe_unused]] float xk[4], tok_x = 0.0f;
   if constexpr (!kReads) {
-    // meanwhile the teacher's softmax, and the logits of its entries (read
-    // before any CTA of the row writes its gradient: the exchange below is a
-    // barrier of them all)
-    float ys = 0.0f;
+    // meanwhile the first warp: the teacher's softmax, and the logits of its
+    // entries (read before any CTA of the row writes its gradient: the exchange
+    // below is a barrier of them all)
+    if (warp == 0) {
+      float ys = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      xk[i] = 0.0f;
-      ty[i] = tid_[i] >= 0 ? (ty[i] - ym) * a.inv_t : -kInf;
-      tq[i] = expf(ty[i]);
-      ys += tq[i];
-      if (leader && warp == 0 && tid_[i] >= 0)
-        xk[i] = to_f((x - first)[tid_[i]]);
-    }
-    for (int o = 16; o; o >>= 1) ys += __shfl_xor_sync(~0u, ys, o);
-    ln_ys = logf(ys);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      tq[i] = tq[i] / ys;
-      const int k = lane + 32 * i;
-      if (MODE == kLossGrad && warp == 0 && k < p.te.k) {
-        sq[k] = tq[i];
-        sid[k] = tid_[i];
+      for (int i = 0; i < 4; ++i) {
+        xk[i] = 0.0f;
+        ty[i] = tid_[i] >= 0 ? (ty[i] - ym) * a.inv_t : -kInf;
+        tq[i] = expf(ty[i]);
+        ys += tq[i];
+        if (leader && tid_[i] >= 0) xk[i] = to_f((x - first)[tid_[i]]);
       }
+      for (int o = 16; o; o >>= 1) ys += __shfl_xor_sync(~0u, ys, o);
+      ln_ys = logf(ys);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        tq[i] = tq[i] / ys;
+        const int k = lane + 32 * i;
+        if (MODE == kLossGrad && k < p.te.k) {
+          sq[k] = tq[i];
+          sid[k] = tid_[i];
+        }
+      }
+      if (lane == 0) *bad_entries = !(ym < kInf);
     }
   } else {
     if (leader && tid == 0 && p.o.logprob && tok < a.classes)
@@ -532,11 +542,7 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
   {
     const float2 c2 = f2(a.c, a.c);
     float2 s2 = f2(0.0f, 0.0f), u2 = s2;
-    for (int g0 = tid; g0 < G; g0 += kBatch * NT) {
-      uint4 q[kBatch];
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i)
-        q[i] = g0 + i * NT < G ? slab[g0 + i * NT] : no_logits<T>();
+    auto add = [&](const uint4 *q) {
       GranuleMax<T> gm;
       gm.clear();
 #pragma unroll
@@ -554,6 +560,19 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
 #pragma unroll
       for (int i = 0; i < kBatch; ++i)
         accumulate<T, kReads>(q[i], nm, c2, s2, u2);
+    };
+    int g = tid;
+    uint4 q[kBatch];
+    for (; g - tid + kBatch * NT <= G; g += kBatch * NT) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) q[i] = slab[g + i * NT];
+      add(q);
+    }
+    if (g - tid < G) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        q[i] = g + i * NT < G ? slab[g + i * NT] : no_logits<T>();
+      add(q);
     }
     float s0, s1, u0, u1;
     split(s2, s0, s1);
@@ -616,7 +635,7 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
     st = warp_combine(st, a.c);
   }
   RowEnd end(st, a.inv_t);
-  if (!kReads) end.bad |= !(ym < kInf);
+  if (!kReads) end.bad |= *bad_entries != 0;
   const float m = end.m, s = end.s;
   const bool bad = end.bad, empty = end.empty;
 
@@ -775,26 +794,21 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
     const int dm = (int)((uintptr_t)d & 15) / (int)sizeof(T);
     if (dm == mis) {
       uint4 *dst = reinterpret_cast<uint4 *>(d - dm);
-#pragma unroll 2
-      for (int g = tid; g < G; g += NT) {
+#pragma unroll 4
+      for (int g = mine0; g < hi; g += NT) {
         const uint4 q = slab[g];
         float r[E];
 #pragma unroll
         for (int i = 0; i < E / 2; ++i) {
-          float u, v;
-          split(__fmul2_rn(__fadd2_rn(pair_of<T>(q, i), nm), c2), u, v);
-          split(__fmul2_rn(f2(ex2(u), ex2(v)), w2), r[2 * i], r[2 * i + 1]);
+          const float2 t = __fmul2_rn(__fadd2_rn(pair_of<T>(q, i), nm), c2);
+          split(__fmul2_rn(f2(ex2(t.x), ex2(t.y)), w2), r[2 * i], r[2 * i + 1]);
         }
-        if (g * E >= mis && (g + 1) * E <= mis + n) {
-          dst[g] = pack_granule<T>(r);
-        } else {
-#pragma unroll
-          for (int j = 0; j < E; ++j) {
-            const int e = g * E + j - mis;
-            if (e >= 0 && e < n) d[e] = from_f<T>(r[j]);
-          }
-        }
+        dst[g] = pack_granule<T>(r);
       }
+      edges([&](int e) {
+        if (e >= 0 && e < n)
+          d[e] = from_f<T>(ex2((to_f(sx[e]) - m0) * a.c) * ws);
+      });
     } else {
       // rows of another alignment: element by element, lanes side by side
       // (the copies of other threads are visible since the exchange)
@@ -2082,15 +2096,21 @@ int sm_count() {
 
 // Shared memory above 48 KB and clusters above 8 CTAs are asked for once a
 // kernel and device.
+constexpr int kMostShared = 227 * 1024;  // a CTA's, static and dynamic
 template <class K>
-void allow(K kernel, std::atomic<uint64_t> &done) {
+void allow(K kernel, std::atomic<uint64_t> &done, int dynamic = kMostShared) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
   const uint64_t bit = 1ull << (dev & 63);
   if (done.load(std::memory_order_acquire) & bit) return;
-  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                       227 * 1024);
-  cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  cudaError_t e = cudaFuncSetAttribute(
+      kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, dynamic);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(
+        kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess)
+    throw std::runtime_error(std::string("class-logit kernel: ") +
+                             cudaGetErrorString(e));
   done.fetch_or(bit, std::memory_order_release);
 }
 
@@ -2148,6 +2168,8 @@ void launch_team(TeamArgs &p, cudaStream_t st) {
     launch_team_of<T, 256, MODE>(p, st);
 }
 
+// Bytes of a row that a second read finds in the L2 while all SMs stream.
+constexpr int64_t kReread = 48 * 1024;
 // Whether rows of a kernel without gradients are streamed by one CTA each: when
 // there are enough of them to keep every SM loading.
 bool streams(const RowArgs &a) {
@@ -2157,13 +2179,6 @@ template <class T, int MODE>
 void launch_stream(const TeamArgs &p, cudaStream_t st) {
   const StreamArgs q{p.a,  p.tokens,     p.itype,  p.top_k, p.o,       p.te,
                      p.row_weight, p.weight, p.loss, p.dx, p.d_stride};
-  if constexpr (MODE == kLossGrad) {
-    if ((int64_t)p.a.classes * (int)sizeof(T) > 128 * 1024) {
-      k_stream<T, 1024, MODE><<<p.a.rows, 1024, 0, st>>>(q);
-      check_launch(cudaGetLastError());
-      return;
-    }
-  }
   // a few batches a thread at least, and maxima well above the alternatives in
   // number
   if (p.a.classes <= 4 * 4 * 256 * kElems<T> && (MODE != kReadTop || p.top_k <= 32))
@@ -2440,7 +2455,7 @@ int launch_distill(const tmnn_logits &x, const void *ids, int index_type,
         BY_DTYPE(x.dtype, (launch_narrow<T, kLoss>(q, x.dtype, st)));
     } else if (!d_logits && streams(p.a)) {
       BY_DTYPE(x.dtype, (launch_stream<T, kLoss>(p, st)));
-    } else if (d_logits && streams(p.a)) {
+    } else if (d_logits && streams(p.a) && (int64_t)x.classes * size <= kReread) {
       BY_DTYPE(x.dtype, (launch_stream<T, kLossGrad>(p, st)));
     } else if (d_logits) {
       BY_DTYPE(x.dtype, (launch_team<T, kLossGrad>(p, st)));
