@@ -368,7 +368,7 @@ __host__ __device__ inline TeamLayout team_layout(int mode, int threads,
   TeamLayout l{};
   int off = granules * 16;
   l.stats = off;
-  off += cluster * (threads / 32) * 16;
+  off += (threads / 32 + cluster) * 16;
   l.teacher = off;
   if (mode >= kLoss) off += (k * 8 + 4 + 15) / 16 * 16;
   l.misc = off;
@@ -601,38 +601,43 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
     if (tid == 0) misc[0] = 0;  // candidates
   }
   {
+    // the warps' parts, then the CTAs'; all add the same parts in one order
     float *part = reinterpret_cast<float *>(smem + p.l.stats);
-    const int mine_at = ((int)rank * kWarps + warp) * 4;
-    if (C > 1) {
-      if (MODE != kReadTop) cluster_wait();
-      if (lane < (int)C) {
-        const uint32_t to = peer_addr(part + mine_at, lane);
-        peer_store(to, st.m);
-        peer_store(to + 4, st.s);
-        peer_store(to + 8, st.u);
-      }
-      cluster_arrive();
-      cluster_wait();
+    float *whole = part + kWarps * 4;
+    if (lane == 0) {
+      part[warp * 4] = st.m;
+      part[warp * 4 + 1] = st.s;
+      part[warp * 4 + 2] = st.u;
+    }
+    __syncthreads();
+    auto combine = [&](const float *of, int parts) {
+      st = Stat{-kInf, 0.0f, 0.0f};
+      if (lane < parts)
+        st = Stat{of[lane * 4], of[lane * 4 + 1], of[lane * 4 + 2]};
+      st = warp_combine(st, a.c);
+    };
+    if (C == 1) {
+      combine(part, kWarps);
     } else {
-      if (lane == 0) {
-        part[mine_at] = st.m;
-        part[mine_at + 1] = st.s;
-        part[mine_at + 2] = st.u;
+      if (MODE != kReadTop) cluster_wait();
+      if (warp == 0) {
+        combine(part, kWarps);
+        if (lane < (int)C) {
+          const uint32_t to = peer_addr(whole + rank * 4, lane);
+          peer_store(to, st.m);
+          peer_store(to + 4, st.s);
+          peer_store(to + 8, st.u);
+        }
       }
-      __syncthreads();
+      // Whoever wrote to a peer orders that before the barrier (a fence, which
+      // costs); the others have nothing to order.
+      if (warp == 0 || MODE == kReadTop)
+        cluster_arrive();
+      else
+        cluster_arrive_started();
+      cluster_wait();
+      combine(whole, (int)C);
     }
-    // every warp adds the same parts in the same order
-    const int parts = (int)C * kWarps;
-    float m = -kInf;
-    for (int i = lane; i < parts; i += 32) m = max_nan(m, part[i * 4]);
-    st = Stat{m, 0.0f, 0.0f};
-    for (int i = lane; i < parts; i += 32) {
-      Stat v{part[i * 4], part[i * 4 + 1], part[i * 4 + 2]};
-      rescale(v, m, a.c);
-      st.s += v.s;
-      st.u += v.u;
-    }
-    st = warp_combine(st, a.c);
   }
   RowEnd end(st, a.inv_t);
   if (!kReads) end.bad |= *bad_entries != 0;
@@ -816,16 +821,46 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
       for (int e = tid; e < n; e += NT)
         d[e] = from_f<T>(ex2((to_f(sx[e]) - m0) * a.c) * ws);
     }
-    __syncthreads();  // an entry's element is written again, after its first value
+    // An entry's element is written again, after its first value: by the warp
+    // that wrote that (of another alignment: by any one, after all have).
+    // Entries of one class, which add up, meet in the same warp.
+    const bool aligned = dm == mis;
+    if (aligned)
+      __syncwarp();
+    else
+      __syncthreads();
     if (!bad && !empty) {
-      for (int k = tid; k < p.te.k; k += NT) {
-        const int id = sid[k] - first;
-        if (sid[k] < 0 || id < 0 || id >= n) continue;
-        float both = 0.0f;  // entries of one class add up
-        for (int j = 0; j < p.te.k; ++j)
-          both += sid[j] == sid[k] ? sq[j] : 0.0f;
-        d[id] = from_f<T>(w * (ex2((to_f(sx[id]) - m) * a.c) / s - both));
+      int32_t id[4];
+      float q[4], both[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        id[i] = -1;
+        both[i] = 0.0f;
+        const int k = lane + 32 * i;
+        if (k >= p.te.k) continue;
+        const int e = sid[k] - first;
+        if (sid[k] >= 0 && e >= 0 && e < n &&
+            (aligned ? (e + mis) / E % NT >> 5 : e % kWarps) == warp)
+          id[i] = e;
+        q[i] = sq[k];
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (32 * i >= p.te.k) break;
+        for (uint32_t has = __ballot_sync(~0u, id[i] >= 0); has; has &= has - 1) {
+          const int from = __ffs(has) - 1;
+          const int32_t of = __shfl_sync(~0u, id[i], from);
+          const float add = __shfl_sync(~0u, q[i], from);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (id[j] == of) both[j] += add;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (id[i] >= 0)
+          d[id[i]] = from_f<T>(
+              w * (ex2((to_f(sx[id[i]]) - m) * a.c) / s - both[i]));
     }
   }
 }
@@ -1261,13 +1296,13 @@ struct BackRow {
 };
 
 // ------------------------------------------------------------ a thread a row
-// Rows of up to 64 classes (a field's outputs): a warp brings 32 of them into
+// Rows of up to 128 classes (a field has up to 64 outputs): a warp brings 32 of them into
 // shared memory as fp32, side by side as they lie in memory, and each thread
 // works through one row there.  No lane idles on a row's odd end and nothing
 // is reduced over lanes.  Rows of whole quads lie `pitch` apart, an odd number
 // of quads, so that the lanes' 16-byte reads meet different banks; other rows
 // keep their distance V (odd, or twice an odd number).
-constexpr int kTinyClasses = 64;
+constexpr int kTinyClasses = 128;
 
 struct TinyArgs {
   RowArgs a;
@@ -1285,7 +1320,8 @@ struct TinyArgs {
   int packed, d_packed; // rows without gaps from a 16-byte boundary on
 };
 
-template <class T, int MODE, bool QUADS>
+// EIGHTS: eights of classes a row may have
+template <class T, int MODE, bool QUADS, int EIGHTS>
 __global__ void __launch_bounds__(128) k_tiny(TinyArgs p) {
   extern __shared__ __align__(16) float image_all[];
   constexpr bool kReads = MODE == kRead || MODE == kReadTop;
@@ -1446,7 +1482,6 @@ __global__ void __launch_bounds__(128) k_tiny(TinyArgs p) {
     return max_nan(max_nan(max_nan(v[0], v[1]), max_nan(v[2], v[3])),
                    max_nan(max_nan(v[4], v[5]), max_nan(v[6], v[7])));
   };
-  constexpr int kEights = kTinyClasses / 8;
   const int eights = (V + 7) / 8;
 
   if (on) {
@@ -1468,9 +1503,9 @@ __global__ void __launch_bounds__(128) k_tiny(TinyArgs p) {
         for (int k = 0; k < K; ++k) ym = max_nan(ym, ey[k]);
         idle = ym == -kInf;
       }
-      float best[kEights];  // maxima of the eights
+      float best[EIGHTS];  // maxima of the eights
 #pragma unroll
-      for (int j = 0; j < kEights; ++j) {
+      for (int j = 0; j < EIGHTS; ++j) {
         best[j] = -kInf;
         if (j < eights) {
           float v[8];
@@ -1478,7 +1513,10 @@ __global__ void __launch_bounds__(128) k_tiny(TinyArgs p) {
           best[j] = max8(v);
         }
       }
-      Stat st{max8(best), 0.0f, 0.0f};
+      float top = max8(best);
+#pragma unroll
+      for (int j = 8; j < EIGHTS; j += 8) top = max_nan(top, max8(best + j));
+      Stat st{top, 0.0f, 0.0f};
       const float m0 = st.m == -kInf ? 0.0f : st.m;
       const float2 nm = f2(-m0, -m0), c2 = f2(a.c, a.c);
       {
@@ -1524,7 +1562,7 @@ __global__ void __launch_bounds__(128) k_tiny(TinyArgs p) {
             float v = best[0];
             int at = 0;
 #pragma unroll
-            for (int j = 1; j < kEights; ++j)
+            for (int j = 1; j < EIGHTS; ++j)
               if (best[j] > v) {
                 v = best[j];
                 at = j;
@@ -1547,7 +1585,7 @@ __global__ void __launch_bounds__(128) k_tiny(TinyArgs p) {
               lp[k] = end.logp(v);
               mine[id[k]] = -kInf;
 #pragma unroll
-              for (int j = 0; j < kEights; ++j)
+              for (int j = 0; j < EIGHTS; ++j)
                 if (j == at) best[j] = rest;
             }
           }
@@ -1653,6 +1691,7 @@ struct NarrowArgs {
   void *dx;
   int64_t d_stride;
   int lanes;
+  int cap;  // logits listed for a row's alternatives, 0: no list
   // the logits' memory, inside which a whole granule may be read although it
   // holds elements of other rows (null where those may be written meanwhile)
   const void *lo, *hi;
@@ -1660,7 +1699,7 @@ struct NarrowArgs {
 
 template <class T, int NG, int MODE>
 __global__ void __launch_bounds__(128) k_narrow(NarrowArgs p) {
-  extern __shared__ float entries[];
+  extern __shared__ __align__(16) float entries[];
   constexpr int E = kElems<T>;
   constexpr bool kReads = MODE == kRead || MODE == kReadTop;
   constexpr bool kTeacher = MODE == kLoss || MODE == kLossGrad;
@@ -1683,41 +1722,47 @@ __global__ void __launch_bounds__(128) k_narrow(NarrowArgs p) {
   // ---- the row
   const T *x = static_cast<const T *>(a.x) + (int64_t)row * a.stride;
   const int mis = (int)((uintptr_t)x & 15) / (int)sizeof(T);
+  const int G = (mis + V + E - 1) / E, whole = (mis + V) / E;
   uint4 q[NG];
   {
     const uint4 *src = reinterpret_cast<const uint4 *>(x - mis);
+    // the granules that may be read as a whole
+    const int from = mis && !(p.lo && src >= p.lo) ? 1 : 0;
+    const int to = p.lo && src + G <= p.hi ? G : whole;
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
-      const int g = l + L * j, e0 = g * E - mis;
+      const int g = l + L * j;
       q[j] = no_logits<T>();
-      if (e0 >= V) continue;
-      if ((e0 >= 0 && e0 + E <= V) ||
-          (p.lo && src + g >= p.lo && src + g + 1 <= p.hi)) {
+      if (g >= from && g < to) {
         q[j] = src[g];
-      } else {
+      } else if (g < G) {
         T v[E];
 #pragma unroll
-        for (int i = 0; i < E; ++i)
-          v[i] = e0 + i >= 0 && e0 + i < V ? x[e0 + i] : from_f<T>(-kInf);
+        for (int i = 0; i < E; ++i) {
+          const int e = g * E - mis + i;
+          v[i] = e >= 0 && e < V ? x[e] : from_f<T>(-kInf);
+        }
         q[j] = *reinterpret_cast<const uint4 *>(v);
       }
     }
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
-      const int e0 = (l + L * j) * E - mis;
-      if (e0 >= V || (e0 >= 0 && e0 + E <= V)) continue;
+      const int g = l + L * j;
+      if (!(mis && g == 0) && !(g == whole && g < G)) continue;
       T v[E];
       *reinterpret_cast<uint4 *>(v) = q[j];
 #pragma unroll
-      for (int i = 0; i < E; ++i)
-        if (e0 + i < 0 || e0 + i >= V) v[i] = from_f<T>(-kInf);
+      for (int i = 0; i < E; ++i) {
+        const int e = g * E - mis + i;
+        if (e < 0 || e >= V) v[i] = from_f<T>(-kInf);
+      }
       q[j] = *reinterpret_cast<const uint4 *>(v);
     }
   }
   T *d = MODE == kLossGrad || MODE == kBack
              ? static_cast<T *>(p.dx) + (int64_t)row * p.d_stride
              : nullptr;
-  // writes f(value, element) of every element
+  // writes what f(value, next value, element, to, next to) gives of every pair
   auto write_rows = [&](auto &&f) {
     const int dm = (int)((uintptr_t)d & 15) / (int)sizeof(T);
     uint4 *dst = reinterpret_cast<uint4 *>(d - dm);
@@ -1725,16 +1770,15 @@ __global__ void __launch_bounds__(128) k_narrow(NarrowArgs p) {
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
       const int g = l + L * j, e0 = g * E - mis;
-      if (e0 >= V) continue;
+      if (g >= G) continue;
       float r[E];
 #pragma unroll
       for (int i = 0; i < E / 2; ++i) {
         float u, v;
         split(pair_of<T>(q[j], i), u, v);
-        r[2 * i] = f(u, e0 + 2 * i);
-        r[2 * i + 1] = f(v, e0 + 2 * i + 1);
+        f(u, v, e0 + 2 * i, r[2 * i], r[2 * i + 1]);
       }
-      if (dm == mis && e0 >= 0 && e0 + E <= V) {
+      if (dm == mis && !(mis && g == 0) && g < whole) {
         dst[g] = pack_granule<T>(r);
       } else {
 #pragma unroll
@@ -1746,7 +1790,10 @@ __global__ void __launch_bounds__(128) k_narrow(NarrowArgs p) {
 
   if constexpr (MODE == kBack) {
     const BackRow b(a, p.tokens, p.itype, p.stats, p.d_logprob, p.d_entropy, row);
-    write_rows([&](float v, int e) { return b.at(v, e, a.c); });
+    write_rows([&](float u, float v, int e, float &ru, float &rv) {
+      ru = b.at(u, e, a.c);
+      rv = b.at(v, e + 1, a.c);
+    });
     return;
   }
 
@@ -1800,7 +1847,7 @@ __global__ void __launch_bounds__(128) k_narrow(NarrowArgs p) {
     float2 s2 = f2(0.0f, 0.0f), u2 = s2;
 #pragma unroll
     for (int j = 0; j < NG; ++j)
-      if (l + L * j < (mis + V + E - 1) / E)
+      if (l + L * j < G)
         accumulate<T, kReads>(q[j], nm, c2, s2, u2);
     float s0, s1, u0, u1;
     split(s2, s0, s1);
@@ -1820,17 +1867,73 @@ __global__ void __launch_bounds__(128) k_narrow(NarrowArgs p) {
     }
   }
   if constexpr (MODE == kReadTop) {
-    // one alternative after the other: the largest value, of the lowest class
     int32_t *ids = p.o.top_ids + (int64_t)row * p.top_k;
     float *lps = p.o.top_logprobs + (int64_t)row * p.top_k;
+    const int K = p.top_k;
+    const bool none = end.bad || idle;
     float best[NG];  // maximum of each granule
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
       GranuleMax<T> t;
       t.clear();
       t.add(q[j]);
-      best[j] = end.bad || idle ? -kInf : t.get();
+      best[j] = none ? -kInf : t.get();
     }
+    // A value (16 bits of it) that K granules of the row reach is a lower bound
+    // of its K-th largest logit: those above it are listed and ranked.  For a
+    // few alternatives the loop below is the shorter way.
+    bool open = true;  // the row's alternatives are still to be found
+    if (p.cap) {
+      uint32_t o[NG], t = 0;
+#pragma unroll
+      for (int j = 0; j < NG; ++j) o[j] = order_of(best[j]);
+      for (uint32_t b = 1u << 31; b >= 1u << 16; b >>= 1) {
+        int c = 0;
+#pragma unroll
+        for (int j = 0; j < NG; ++j) c += o[j] >= (t | b);
+        for (int i = 1; i < L; i *= 2) c += __shfl_xor_sync(~0u, c, i);
+        if (c >= K) t |= b;
+      }
+      const float floor = value_of(max(t, kLowestOrder));
+      const int of = warp * (32 / L) + lane / L;
+      uint64_t *list = reinterpret_cast<uint64_t *>(entries) + of * p.cap;
+      int *count = reinterpret_cast<int *>(entries) + (128 / L) * p.cap * 2 + of;
+      if (l == 0) *count = 0;
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        if (!(best[j] >= floor)) continue;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          float f[2];
+          split(pair_of<T>(q[j], i >> 1), f[0], f[1]);
+          if (f[i & 1] >= floor) {
+            const int at = atomicAdd(count, 1);
+            if (at < p.cap) list[at] = key_of(f[i & 1], (l + L * j) * E + i - mis);
+          }
+        }
+      }
+      __syncwarp();
+      const int M = *count;
+      open = M > p.cap;
+      if (!open && on) {
+        for (int i = l; i < M; i += L) {
+          const uint64_t key = list[i];
+          int above = 0;
+          for (int j = 0; j < M; ++j) above += list[j] > key;
+          if (above < K) {
+            ids[above] = class_of(key);
+            lps[above] = end.logp(value_of((uint32_t)(key >> 32)));
+          }
+        }
+        for (int k = M + l; k < K; k += L) {
+          ids[k] = -1;
+          lps[k] = end.bad && !idle ? nan : -kInf;
+        }
+      }
+    }
+    // one alternative after the other: the largest value, of the lowest class
+    if (__any_sync(~0u, open))
     for (int k = 0; k < p.top_k; ++k) {
       float v = best[0];
       uint4 w = q[0];
@@ -1873,7 +1976,7 @@ __global__ void __launch_bounds__(128) k_narrow(NarrowArgs p) {
             best[j] = rest;
           }
       }
-      if (l == 0 && on) {
+      if (l == 0 && on && open) {
         const bool some = top > -kInf;
         ids[k] = some ? first : -1;
         lps[k] = some ? end.logp(top) : end.bad && !idle ? nan : -kInf;
@@ -1907,8 +2010,11 @@ __global__ void __launch_bounds__(128) k_narrow(NarrowArgs p) {
       const float ws = zero ? 0.0f : end.bad ? nan : w / end.s;
       const float m0 = zero ? 0.0f : end.m;
       __syncwarp();  // every lane has read what the row's lanes now write
-      write_rows([&](float v, int) {
-        return zero ? 0.0f : ex2((v - m0) * a.c) * ws;
+      const float2 nm = f2(-m0, -m0), c2 = f2(a.c, a.c), w2 = f2(ws, ws);
+      write_rows([&](float u, float v, int, float &ru, float &rv) {
+        const float2 t = __fmul2_rn(__fadd2_rn(f2(u, v), nm), c2);
+        split(__fmul2_rn(f2(ex2(t.x), ex2(t.y)), w2), ru, rv);
+        if (zero) ru = rv = 0.0f;
       });
       __syncwarp();  // an entry's element is written again
       if (on && !zero && !end.bad)
@@ -2188,6 +2294,14 @@ void launch_stream(const TeamArgs &p, cudaStream_t st) {
   check_launch(cudaGetLastError());
 }
 
+template <class T, int MODE, bool QUADS, int EIGHTS>
+void launch_tiny_of(const TinyArgs &p, size_t smem, cudaStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  auto kernel = k_tiny<T, MODE, QUADS, EIGHTS>;
+  allow(kernel, done);
+  kernel<<<(p.a.rows + 127) / 128, 128, smem, st>>>(p);
+  check_launch(cudaGetLastError());
+}
 template <class T, int MODE>
 void launch_tiny(TinyArgs &p, cudaStream_t st) {
   const int V = p.a.classes;
@@ -2198,19 +2312,15 @@ void launch_tiny(TinyArgs &p, cudaStream_t st) {
   };
   p.packed = packed(p.a.x, p.a.stride);
   p.d_packed = packed(p.dx, p.d_stride);
-  static std::atomic<uint64_t> done[2] = {};
   size_t smem = (size_t)((32 * p.pitch + 3) / 4 * 4) * 4 * sizeof(float);
-  if (MODE == kLoss || MODE == kLossGrad) {
-    allow(k_tiny<T, MODE, true>, done[0]);
-    allow(k_tiny<T, MODE, false>, done[1]);
+  if (MODE == kLoss || MODE == kLossGrad)
     smem += (size_t)4 * 64 * (p.te.k | 1) * sizeof(float);
-  }
-  const uint32_t grid = (p.a.rows + 127) / 128;
-  if (quads)
-    k_tiny<T, MODE, true><<<grid, 128, smem, st>>>(p);
+  if (V <= 64)
+    quads ? launch_tiny_of<T, MODE, true, 8>(p, smem, st)
+          : launch_tiny_of<T, MODE, false, 8>(p, smem, st);
   else
-    k_tiny<T, MODE, false><<<grid, 128, smem, st>>>(p);
-  check_launch(cudaGetLastError());
+    quads ? launch_tiny_of<T, MODE, true, 16>(p, smem, st)
+          : launch_tiny_of<T, MODE, false, 16>(p, smem, st);
 }
 
 // Granules of the widest row when rows may start anywhere inside one.
@@ -2231,6 +2341,9 @@ void launch_narrow_of(NarrowArgs &p, cudaStream_t st) {
     allow(kernel, done);
     smem = (size_t)(128 / p.lanes) * p.te.k * 12;
   }
+  // (four rounds of the loop over the alternatives cost about a list)
+  p.cap = MODE == kReadTop && p.top_k > 4 ? 32 + 2 * p.top_k : 0;
+  if (p.cap) smem = (size_t)(128 / p.lanes) * (p.cap * 8 + 4);
   const uint32_t rows = 128 / p.lanes;
   kernel<<<(p.a.rows + rows - 1) / rows, 128, smem, st>>>(p);
   check_launch(cudaGetLastError());
@@ -2361,7 +2474,7 @@ int launch_token_logprobs_backward(const tmnn_logits &x, const void *tokens,
     b.x = at(x.data, (int64_t)i * x.row_stride * size);
     b.rows = n;
     const void *d = at(d_logits, (int64_t)i * d_stride * size);
-    if (x.classes <= kTinyClasses) {
+    if (x.classes <= kTinyClasses / 2) {
       TinyArgs q{};
       q.a = b;
       q.tokens = at(tokens, (int64_t)i * index_size(index_type));
