@@ -1880,8 +1880,9 @@ __global__ void __launch_bounds__(128) k_narrow(NarrowArgs p) {
       best[j] = none ? -kInf : t.get();
     }
     // A value (16 bits of it) that K granules of the row reach is a lower bound
-    // of its K-th largest logit: those above it are listed and ranked.  For a
-    // few alternatives the loop below is the shorter way.
+    // of its K-th largest logit: the granules that reach it are listed, then
+    // their logits above it, which are ranked.  For a few alternatives the loop
+    // below is the shorter way.
     bool open = true;  // the row's alternatives are still to be found
     if (p.cap) {
       uint32_t o[NG], t = 0;
@@ -1891,31 +1892,45 @@ __global__ void __launch_bounds__(128) k_narrow(NarrowArgs p) {
         int c = 0;
 #pragma unroll
         for (int j = 0; j < NG; ++j) c += o[j] >= (t | b);
-        for (int i = 1; i < L; i *= 2) c += __shfl_xor_sync(~0u, c, i);
+        if (L == 32)
+          c = __reduce_add_sync(~0u, c);
+        else
+          for (int i = 1; i < L; i *= 2) c += __shfl_xor_sync(~0u, c, i);
         if (c >= K) t |= b;
       }
       const float floor = value_of(max(t, kLowestOrder));
+      // a row's part of the shared memory: granules, keys, the granules'
+      // classes, two counts
       const int of = warp * (32 / L) + lane / L;
-      uint64_t *list = reinterpret_cast<uint64_t *>(entries) + of * p.cap;
-      int *count = reinterpret_cast<int *>(entries) + (128 / L) * p.cap * 2 + of;
-      if (l == 0) *count = 0;
+      uint4 *kept = reinterpret_cast<uint4 *>(entries) + of * (p.cap * 7 / 4 + 1);
+      uint64_t *list = reinterpret_cast<uint64_t *>(kept + p.cap);
+      int *kept_at = reinterpret_cast<int *>(list + p.cap);
+      int *count = kept_at + p.cap;
+      if (l < 2) count[l] = 0;
+      if (L == 1) count[1] = 0;
       __syncwarp();
 #pragma unroll
-      for (int j = 0; j < NG; ++j) {
-        if (!(best[j] >= floor)) continue;
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-          float f[2];
-          split(pair_of<T>(q[j], i >> 1), f[0], f[1]);
-          if (f[i & 1] >= floor) {
-            const int at = atomicAdd(count, 1);
-            if (at < p.cap) list[at] = key_of(f[i & 1], (l + L * j) * E + i - mis);
+      for (int j = 0; j < NG; ++j)
+        if (best[j] >= floor) {
+          const int at = atomicAdd(count, 1);
+          if (at < p.cap) {
+            kept[at] = q[j];
+            kept_at[at] = (l + L * j) * E - mis;
           }
         }
-      }
       __syncwarp();
-      const int M = *count;
-      open = M > p.cap;
+      const int granules = count[0];
+      if (granules <= p.cap)
+        for (int i = l; i < granules * E; i += L) {
+          const float v = to_f(reinterpret_cast<const T *>(kept)[i]);
+          if (v >= floor) {
+            const int at = atomicAdd(count + 1, 1);
+            if (at < p.cap) list[at] = key_of(v, kept_at[i / E] + i % E);
+          }
+        }
+      __syncwarp();
+      const int M = count[1];
+      open = granules > p.cap || M > p.cap;
       if (!open && on) {
         for (int i = l; i < M; i += L) {
           const uint64_t key = list[i];
@@ -2342,8 +2357,11 @@ void launch_narrow_of(NarrowArgs &p, cudaStream_t st) {
     smem = (size_t)(128 / p.lanes) * p.te.k * 12;
   }
   // (four rounds of the loop over the alternatives cost about a list)
-  p.cap = MODE == kReadTop && p.top_k > 4 ? 32 + 2 * p.top_k : 0;
-  if (p.cap) smem = (size_t)(128 / p.lanes) * (p.cap * 8 + 4);
+  p.cap = MODE == kReadTop && p.top_k > 4 ? (32 + 2 * p.top_k) / 4 * 4 : 0;
+  if (p.cap) {
+    allow(kernel, done);
+    smem = (size_t)(128 / p.lanes) * (p.cap * 7 / 4 + 1) * 16;
+  }
   const uint32_t rows = 128 / p.lanes;
   kernel<<<(p.a.rows + rows - 1) / rows, 128, smem, st>>>(p);
   check_launch(cudaGetLastError());
