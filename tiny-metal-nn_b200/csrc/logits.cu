@@ -342,6 +342,34 @@ __device__ __forceinline__ void write_zeros(T *d, int n) {
   }
 }
 
+// d[e] = e^((x(e) - m) / T) w for e < n in words of 4 bytes, lanes side by side:
+// for gradients that lie otherwise in their granules than the logits.  By all
+// threads; nm, c, w: -m, log2(e) / T and w twice.
+template <class T, int NT, class X>
+__device__ __forceinline__ void write_words(T *d, int n, X &&x, float2 nm,
+                                            float2 c, float2 w) {
+  auto two = [&](float a, float b) {
+    const float2 t = __fmul2_rn(__fadd2_rn(f2(a, b), nm), c);
+    return __fmul2_rn(f2(ex2(t.x), ex2(t.y)), w);
+  };
+  if constexpr (sizeof(T) == 2) {
+    const int first = (int)((uintptr_t)d & 3) / 2;  // elements before a word
+    const int pairs = (n - first) / 2;
+    uint32_t *words = reinterpret_cast<uint32_t *>(d + first);
+#pragma unroll 4
+    for (int i = threadIdx.x; i < pairs; i += NT) {
+      const float2 r = two(x(first + 2 * i), x(first + 2 * i + 1));
+      words[i] = pack2<T>(r.x, r.y);
+    }
+    if (threadIdx.x == 0 && first && n > 0) d[0] = from_f<T>(two(x(0), 0.0f).x);
+    if (threadIdx.x == 1 && first + 2 * pairs < n)
+      d[n - 1] = from_f<T>(two(x(n - 1), 0.0f).x);
+  } else {
+#pragma unroll 4
+    for (int e = threadIdx.x; e < n; e += NT) d[e] = from_f<T>(two(x(e), 0.0f).x);
+  }
+}
+
 // ------------------------------------------------------------ a team a row
 // A team -- a CTA, or a cluster of CTAs each holding a part ("slab") of the
 // row in its shared memory -- reads a row once.  Every thread copies its own
@@ -815,11 +843,9 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
           d[e] = from_f<T>(ex2((to_f(sx[e]) - m0) * a.c) * ws);
       });
     } else {
-      // rows of another alignment: element by element, lanes side by side
-      // (the copies of other threads are visible since the exchange)
-#pragma unroll 4
-      for (int e = tid; e < n; e += NT)
-        d[e] = from_f<T>(ex2((to_f(sx[e]) - m0) * a.c) * ws);
+      // rows of another alignment (the copies of other threads are visible
+      // since the exchange)
+      write_words<T, NT>(d, n, [&](int e) { return to_f(sx[e]); }, nm, c2, w2);
     }
     // An entry's element is written again, after its first value: by the warp
     // that wrote that (of another alignment: by any one, after all have).
@@ -1151,10 +1177,8 @@ __global__ void __launch_bounds__(NT) k_stream(StreamArgs p) {
       if (warp == 0 && lane < 16 && (lane < 8 ? lane < head : odd_class < V))
         d[odd_class] = from_f<T>(ex2((odd - m0) * a.c) * ws);
     } else {
-      // rows of another alignment: element by element, lanes side by side
-#pragma unroll 8
-      for (int e = tid; e < V; e += NT)
-        d[e] = from_f<T>(ex2((to_f(x[e]) - m0) * a.c) * ws);
+      // rows of another alignment
+      write_words<T, NT>(d, V, [&](int e) { return to_f(x[e]); }, nm, c2, w2);
     }
     __syncthreads();  // an entry's element is written again, after its first value
     if (warp == 0 && !end.bad && !end.empty) {

@@ -144,7 +144,7 @@ def token_logprobs(logits, tokens=None, *, top_k=0, temperature=1.0,
         tp, it = _vector(tokens, "tokens", dev, (n,), _INDEX)
         lp = empty(n, dtype=f32, device=dev)
         lpp = lp.data_ptr()
-    ent = empty(n, dtype=f32, device=dev)
+    ent = empty(n, dtype=f32, device=dev) if lp is None else _torch.empty_like(lp)
     if k:
         ids = empty(n, k, dtype=_torch.int32, device=dev)
         top = empty(n, k, dtype=f32, device=dev)
