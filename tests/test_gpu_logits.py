@@ -65,13 +65,13 @@ def make_tokens(n, V, seed, dtype="int64"):
     return torch.from_numpy(tok).to("cuda").to(getattr(torch, dtype)), tok
 
 
-# 300 rows and more: wide rows in numbers that fill the SMs
+# 150 rows and more: wide rows in numbers that fill the SMs
 SIZES = [(1, 1), (3, 2), (40, 3), (13, 19), (70000, 5), (33, 31), (300, 64),
          (12, 65), (50, 127), (11, 257), (64, 1000), (5, 1023), (17, 1024),
          (17, 1025), (10, 2047), (12, 2311), (10, 4097), (21, 8192), (2, 32768),
          (11, 32003), (300, 5000), (1, 131072), (10, 50021), (3, 262143),
-         (12, 131071), (1, 524288), (320, 9001), (305, 33000), (600, 2500),
-         (610, 24999), (300, 70001), (303, 40000)]
+         (12, 131071), (1, 524288), (320, 9001), (160, 33000), (600, 2500),
+         (155, 24999), (152, 66001), (150, 40000)]
 DTYPES = ["f32", "bf16", "fp16"]
 
 
@@ -332,7 +332,10 @@ def test_far_rows_and_repeated_rows():
     x = mem.as_strided((2, V), (far, 1))
     torch.manual_seed(1)
     x.copy_(torch.randn(2, V, device="cuda"))
-    near = x.contiguous()
+    # near rows that start on the same boundaries: rows that start elsewhere are
+    # summed in another order, which is within the bounds but not bit for bit
+    near = torch.empty(2, V + 5, dtype=torch.bfloat16, device="cuda")[:, :V]
+    near.copy_(x)
     tok = torch.tensor([7, V - 1], device="cuda")
     a = t.token_logprobs(x, tok, top_k=9, stats=True)
     b = t.token_logprobs(near, tok, top_k=9, stats=True)
@@ -342,11 +345,9 @@ def test_far_rows_and_repeated_rows():
     ids = torch.tensor([[1, 2], [0, V - 1]], device="cuda")
     y = torch.randn(2, 2, device="cuda")
     wl, wg = t.distill_forward_backward(near, ids, y)
-    l, _ = t.distill_forward_backward(x.clone(), ids, y)
-    assert torch.equal(l, wl)
     save = near.clone()
-    t.distill_forward_backward(x, ids, y, out=x)
-    assert torch.equal(x, wg)
+    l, _ = t.distill_forward_backward(x, ids, y, out=x)
+    assert torch.equal(l, wl) and torch.equal(x, wg)
     x.copy_(save)
     t.token_logprobs_backward(x, tok, b.stats, one, one, out=x)
     assert torch.equal(x, want)

@@ -78,6 +78,7 @@ __device__ __forceinline__ uint32_t order_of(float v) {
 __device__ __forceinline__ float value_of(uint32_t o) {
   return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xFFFFFFFFu));
 }
+constexpr uint32_t kLowestOrder = 0x00800000u;  // order of the lowest finite
 // (value, lowest class first) as one key; 0 is none
 __device__ __forceinline__ uint64_t key_of(float v, int32_t cls) {
   const uint32_t o = order_of(v);
@@ -370,6 +371,36 @@ __device__ __forceinline__ void write_words(T *d, int n, X &&x, float2 nm,
   }
 }
 
+// A value that at least K of n <= N orders reach, and hardly more: the largest
+// one with the low 16 bits zero (all there is to a 16-bit logit), or what all n
+// have in common; the order of the lowest logit if fewer than K are logits.
+// One warp, halving from the first bit in which the orders differ.
+template <int N>
+__device__ __forceinline__ uint32_t reached_by(int K, const uint32_t *values,
+                                               int n) {
+  uint32_t v[N / 32], hi = 0, lo = ~0u;
+#pragma unroll
+  for (int i = 0; i < N / 32; ++i) {
+    const int at = (threadIdx.x & 31) + 32 * i;
+    v[i] = at < n ? values[at] : 0;
+    hi = max(hi, v[i]);
+    lo = at < n ? min(lo, v[i]) : lo;
+  }
+  hi = __reduce_max_sync(~0u, hi);
+  lo = __reduce_min_sync(~0u, lo);
+  const uint32_t same = (uint32_t)__clz(hi ^ lo);  // leading bits
+  uint32_t t = same == 0 ? 0 : same == 32 ? hi : hi >> (32 - same) << (32 - same);
+  if (same < 16)
+    for (uint32_t b = 1u << (31 - same); b >= 1u << 16; b >>= 1) {
+      const uint32_t up = t | b;
+      uint32_t c = 0;
+#pragma unroll
+      for (int i = 0; i < N / 32; ++i) c += v[i] >= up;
+      if (__reduce_add_sync(~0u, c) >= (uint32_t)K) t = up;
+    }
+  return max(t, kLowestOrder);
+}
+
 // ------------------------------------------------------------ a team a row
 // A team -- a CTA, or a cluster of CTAs each holding a part ("slab") of the
 // row in its shared memory -- reads a row once.  Every thread copies its own
@@ -380,7 +411,6 @@ __device__ __forceinline__ void write_words(T *d, int n, X &&x, float2 nm,
 enum Mode { kRead = 0, kReadTop = 1, kLoss = 2, kLossGrad = 3, kBack = 4 };
 
 constexpr int kMaxCluster = 16;
-constexpr uint32_t kLowestOrder = 0x00800000u;  // order of the lowest finite
 constexpr int kMaxGroups = 256;
 
 // Shared memory of a CTA of a team, in bytes from its base: the slab, the
@@ -691,20 +721,8 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
       return;
     }
     if (warp == 0) {
-      // the largest such value with its low 16 bits zero (all there is to a
-      // 16-bit logit), by halving; each lane holds 8 of the maxima
-      uint32_t v[kMaxGroups / 32], t = 0;
-#pragma unroll
-      for (int i = 0; i < kMaxGroups / 32; ++i)
-        v[i] = lane + 32 * i < p.l.groups ? gmax[lane + 32 * i] : 0;
-      for (uint32_t b = 1u << 31; b >= 1u << 16; b >>= 1) {
-        const uint32_t up = t | b;
-        uint32_t c = 0;
-#pragma unroll
-        for (int i = 0; i < kMaxGroups / 32; ++i) c += v[i] >= up;
-        if (__reduce_add_sync(~0u, c) >= (uint32_t)K) t = up;
-      }
-      if (lane == 0) misc[1] = max(t, kLowestOrder);
+      const uint32_t t = reached_by<kMaxGroups>(K, gmax, p.l.groups);
+      if (lane == 0) misc[1] = t;
     }
     __syncthreads();
     const uint32_t tau = misc[1];
@@ -916,23 +934,6 @@ struct StreamArgs {
   int64_t d_stride;
 };
 
-// The largest value, of those with the low 16 bits zero (all there is to a
-// 16-bit logit), that at least K of N orders reach; with none, the order of the
-// lowest logit.  One warp; halving from the top bit.
-template <int N>
-__device__ __forceinline__ uint32_t reached_by(int K, const uint32_t *values) {
-  uint32_t v[N / 32], t = 0;
-#pragma unroll
-  for (int i = 0; i < N / 32; ++i) v[i] = values[(threadIdx.x & 31) + 32 * i];
-  for (uint32_t b = 1u << 31; b >= 1u << 16; b >>= 1) {
-    const uint32_t up = t | b;
-    uint32_t c = 0;
-#pragma unroll
-    for (int i = 0; i < N / 32; ++i) c += v[i] >= up;
-    if (__reduce_add_sync(~0u, c) >= (uint32_t)K) t = up;
-  }
-  return max(t, kLowestOrder);
-}
 template <class T, int NT, int MODE>
 __global__ void __launch_bounds__(NT) k_stream(StreamArgs p) {
   constexpr int E = kElems<T>, kBatch = 4, kWarps = NT / 32;
@@ -1206,7 +1207,7 @@ __global__ void __launch_bounds__(NT) k_stream(StreamArgs p) {
       return;
     }
     if (warp == 0) {
-      const uint32_t t = reached_by<NT>(K, gmax);
+      const uint32_t t = reached_by<NT>(K, gmax, NT);
       if (lane == 0) misc[1] = t;
     }
     __syncthreads();
@@ -2315,18 +2316,25 @@ void launch_team(TeamArgs &p, cudaStream_t st) {
 
 // Bytes of a row that a second read finds in the L2 while all SMs stream.
 constexpr int64_t kReread = 48 * 1024;
-// Whether rows of a kernel without gradients are streamed by one CTA each: when
-// there are enough of them to keep every SM loading.
-bool streams(const RowArgs &a) {
-  return (int64_t)a.rows >= 2 * (int64_t)sm_count();
+// Whether rows are streamed by one CTA each: short rows always (one of 20 KB
+// with 20 alternatives takes 6.4 us, a cluster 7.5; of 64 KB 8.4 and 6.9),
+// others when there are enough of them to keep every SM loading (150 rows of
+// 256 KB: 14.4 us, clusters 16.4; 100 rows: 13.1 and 10.0).  A gradient takes
+// a second read of the row.
+bool streams(const RowArgs &a, int size, bool grad) {
+  const int64_t bytes = (int64_t)a.classes * size;
+  if (grad) return bytes <= kReread;
+  return bytes <= 40 * 1024 || (int64_t)a.rows >= (int64_t)sm_count();
 }
 template <class T, int MODE>
 void launch_stream(const TeamArgs &p, cudaStream_t st) {
   const StreamArgs q{p.a,  p.tokens,     p.itype,  p.top_k, p.o,       p.te,
                      p.row_weight, p.weight, p.loss, p.dx, p.d_stride};
-  // a few batches a thread at least, and maxima well above the alternatives in
-  // number
-  if (p.a.classes <= 4 * 4 * 256 * kElems<T> && (MODE != kReadTop || p.top_k <= 32))
+  // With many rows a few batches a thread at least, and maxima well above the
+  // alternatives in number; few rows are over sooner with more threads.
+  if (p.a.classes <= 4 * 4 * 256 * kElems<T> &&
+      (int64_t)p.a.rows >= (int64_t)sm_count() &&
+      (MODE != kReadTop || p.top_k <= 32))
     k_stream<T, 128, MODE><<<p.a.rows, 128, 0, st>>>(q);
   else
     k_stream<T, 256, MODE><<<p.a.rows, 256, 0, st>>>(q);
@@ -2479,7 +2487,7 @@ int launch_token_logprobs(const tmnn_logits &x, const void *tokens,
         BY_DTYPE(x.dtype, (launch_narrow<T, kReadTop>(q, x.dtype, st)));
       else
         BY_DTYPE(x.dtype, (launch_narrow<T, kRead>(q, x.dtype, st)));
-    } else if (streams(p.a)) {
+    } else if (streams(p.a, elem_size(x.dtype), false)) {
       if (top_k)
         BY_DTYPE(x.dtype, (launch_stream<T, kReadTop>(p, st)));
       else
@@ -2608,9 +2616,9 @@ int launch_distill(const tmnn_logits &x, const void *ids, int index_type,
         BY_DTYPE(x.dtype, (launch_narrow<T, kLossGrad>(q, x.dtype, st)));
       else
         BY_DTYPE(x.dtype, (launch_narrow<T, kLoss>(q, x.dtype, st)));
-    } else if (!d_logits && streams(p.a)) {
+    } else if (!d_logits && streams(p.a, size, false)) {
       BY_DTYPE(x.dtype, (launch_stream<T, kLoss>(p, st)));
-    } else if (d_logits && streams(p.a) && (int64_t)x.classes * size <= kReread) {
+    } else if (d_logits && streams(p.a, size, true)) {
       BY_DTYPE(x.dtype, (launch_stream<T, kLossGrad>(p, st)));
     } else if (d_logits) {
       BY_DTYPE(x.dtype, (launch_team<T, kLossGrad>(p, st)));
