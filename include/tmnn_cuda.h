@@ -534,7 +534,8 @@ const char *tmnn_cuda_mlp_last_error(void);
  * has no distribution: its log probabilities are -inf, its entropy and its
  * gradient 0.  A NaN or +inf in a row makes the row's results NaN.
  * Limits: 1 <= classes <= 524288; temperature in [1e-4, 1e4]; pointers
- * aligned to their element.  n = 0 is a no-op. */
+ * aligned to their element; outputs apart from the inputs and one another.
+ * No rows is a no-op. */
 typedef struct tmnn_logits {
   const void *data;    /* [rows x classes], rows `row_stride` elements apart */
   int64_t row_stride;  /* any value >= 0; the gradient's is >= classes */
@@ -551,7 +552,8 @@ typedef struct tmnn_logits {
  * stats [rows x 3] = max x, sum exp((x - max) / T), entropy: what the backward
  * call needs.  Each output may be NULL (top_ids and top_logprobs only with
  * top_k = 0), and tokens when logprob is.  A token below 0 marks a padded
- * row, which is not read: logprob, entropy and stats 0, no alternatives.  A
+ * row, whose logits count for nothing: logprob, entropy and stats 0, no
+ * alternatives.  A
  * token >= classes makes its logprob NaN. */
 tmnn_status tmnn_cuda_token_logprobs(int device, void *stream,
                                      const tmnn_logits *logits,
@@ -566,7 +568,8 @@ tmnn_status tmnn_cuda_token_logprobs(int device, void *stream,
  *   d_x = (d_logprob (delta_token - p) - d_entropy p (log p + entropy)) / T.
  * d_logprob and tokens, or d_entropy, may be NULL.  d_logits has the logits'
  * type, rows d_row_stride >= classes apart; it may be the logits' own memory
- * (same address and stride) but not overlap them otherwise.  Every row's
+ * (same address and stride), but otherwise its rows may neither overlap them
+ * nor lie between them, and it is apart from every other argument.  Every row's
  * `classes` elements are written, columns behind them are left alone.  A
  * padded row's gradient is 0, and that of a row whose token is >= classes is
  * NaN. */
@@ -583,7 +586,7 @@ tmnn_status tmnn_cuda_token_logprobs_backward(
  *   d_logits[i] = w_i d loss[i] / d x = w_i T (p - q),
  * w_i = row_weight[i], or 1 / rows when row_weight is NULL (the gradient of
  * the mean loss).  Entries with id < 0 or logit -inf are left out, and a row
- * without entries is padding: it is not read, its loss and gradient are 0.
+ * without entries is padding: its loss and gradient are 0.
  * Entries that name one class twice count each on its own.  An id >= classes
  * or a NaN or +inf among the entries makes the row NaN.  d_logits NULL: the
  * loss only (row_weight is not read); otherwise as in

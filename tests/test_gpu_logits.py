@@ -358,6 +358,25 @@ def test_far_rows_and_repeated_rows():
     assert torch.equal(c.top_ids, a.top_ids[:1].expand(5, 9))
 
 
+def test_one_row_in_place():
+    """A single row's stride does not matter, in place either."""
+    import torch
+    import tmnn_b200 as t
+    for V in (7, 900, 70001):
+        x = torch.randn(V, device="cuda").expand(1, V)
+        tok = torch.tensor([V - 1], device="cuda")
+        one = torch.ones(1, device="cuda")
+        st = t.token_logprobs(x, tok, stats=True).stats
+        want = t.token_logprobs_backward(x, tok, st, one, one)
+        _, dist = t.distill_forward_backward(x, tok.view(1, 1), one.view(1, 1))
+        y = x.clone().as_strided((1, V), (0, 1))
+        assert torch.equal(t.token_logprobs_backward(y, tok, st, one, one, out=y),
+                           want)
+        y = x.clone().as_strided((1, V), (0, 1))
+        t.distill_forward_backward(y, tok.view(1, 1), one.view(1, 1), out=y)
+        assert torch.equal(y, dist)
+
+
 def test_empty_batches():
     import torch
     import tmnn_b200 as t
@@ -405,6 +424,9 @@ def test_refusals():
                     x, ids, y, out=torch.zeros(10, device="cuda").expand(4, 10)),
                 lambda: t.distill_forward_backward(
                     x[:, :9], ids, y, out=x[:, 1:]),
+                lambda: t.distill_forward_backward(
+                    x, ids, y, out=torch.zeros(8, 10, device="cuda")[::2, :8]),
+                lambda: t.token_logprobs_backward(x, tok, st[:, :2], y[:, 0]),
                 lambda: t.token_logprobs_backward(x, None, st, y[:, 0].contiguous())):
         with pytest.raises(ValueError):
             bad()

@@ -35,6 +35,8 @@ def _refused(st, frag):
     (dict(temperature=float("nan")), "temperature must be in"),
     (dict(temperature=float("inf")), "temperature must be in"),
     (dict(row_stride=-1), "row_stride must be in"),
+    (dict(row_stride=(1 << 40) + 1), "row_stride must be in"),
+    (dict(row_stride=1 << 40, rows=1 << 17), "span more than memory"),
     (dict(data=0), "logits is null"),
     (dict(data=P + 2), "logits is not aligned"),
 ])
@@ -64,6 +66,10 @@ def test_null_logits():
     ((P + 4, 1, 0, P, P, None, None, None), "tokens is not aligned"),
     ((P, 0, 0, P + 1, P, None, None, None), "logprob is not aligned"),
     ((P, 0, 0, P, P, None, None, P + 2), "stats is not aligned"),
+    ((2 * P, 0, 0, P + 1596, 3 * P, None, None, None), "an output overlaps"),
+    ((2 * P, 0, 0, 3 * P, 2 * P + 12, None, None, None), "an output overlaps"),
+    ((2 * P, 0, 0, 3 * P, 3 * P + 12, None, None, None), "an output overlaps"),
+    ((2 * P, 0, 3, 3 * P, 4 * P, 5 * P, 5 * P + 44, None), "an output overlaps"),
 ])
 def test_token_logprobs_refusals(args, frag):
     from tmnn_b200 import lib
@@ -87,6 +93,10 @@ def test_top_k_limit():
     ((P, 0, P, P, None, P + 4 * 399, 100), "overlaps the logits in part"),
     ((P, 0, P, P, None, P - 4 * 399, 100), "overlaps the logits in part"),
     ((P, 3, P, P, None, 2 * P, 100), "index_type"),
+    ((2 * P + 8, 0, P, P, None, 2 * P, 100), "d_logits overlaps another"),
+    ((3 * P, 0, 2 * P + 1596, P, None, 2 * P, 100), "d_logits overlaps another"),
+    ((3 * P, 0, 4 * P, P, 2 * P, 2 * P, 100), "d_logits overlaps another"),
+    ((3 * P, 0, 4 * P, P, None, 2 * P, 1 << 41), "d_row_stride must be in"),
 ])
 def test_backward_refusals(args, frag):
     from tmnn_b200 import lib
@@ -102,9 +112,15 @@ def test_backward_refusals(args, frag):
     ((None, 0, P, 0, 4, None, P, None, 0), "teacher_ids is null"),
     ((P, 0, None, 0, 4, None, P, None, 0), "teacher_logits is null"),
     ((P, 0, P, 0, 4, None, None, None, 0), "loss is null"),
-    ((P, 0, P, 0, 4, None, P, 2 * P, 50), "d_row_stride must be in"),
+    ((2 * P, 0, 3 * P, 0, 4, None, 4 * P, 5 * P, 50), "d_row_stride must be in"),
     ((P, 0, P, 0, 4, P + 2, P, 2 * P, 100), "row_weight is not aligned"),
-    ((P, 0, P, 0, 4, None, P, P + 40, 100), "overlaps the logits in part"),
+    ((2 * P, 0, 3 * P, 0, 4, None, 4 * P, P + 40, 100),
+     "overlaps the logits in part"),
+    ((2 * P, 0, 3 * P, 0, 4, None, P, None, 0), "loss overlaps another"),
+    ((2 * P, 0, 3 * P, 0, 4, None, 3 * P + 60, None, 0), "loss overlaps another"),
+    ((2 * P, 0, 3 * P, 0, 4, None, 4 * P, 2 * P, 100), "d_logits overlaps another"),
+    ((2 * P, 0, 3 * P, 0, 4, 5 * P, 4 * P, 5 * P - 1596, 100),
+     "d_logits overlaps another"),
 ])
 def test_distill_refusals(args, frag):
     from tmnn_b200 import lib

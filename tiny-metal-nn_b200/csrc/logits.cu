@@ -13,6 +13,7 @@
 
 #include <atomic>
 #include <cmath>
+#include <initializer_list>
 #include <stdexcept>
 #include <string>
 #include <type_traits>
@@ -22,7 +23,6 @@
 using namespace tmnn;
 
 namespace {
-
 
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kInf = __builtin_huge_valf();
@@ -244,8 +244,8 @@ __device__ __forceinline__ void copies_done() {
 __device__ __forceinline__ void cluster_arrive() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 }
-// Says that this CTA runs; its peers may write to it when all have said so.
-// Orders no memory (that costs a fence).
+// Arrives without ordering memory, which costs a fence: by threads that have
+// nothing to show to the other CTAs but that they came here.
 __device__ __forceinline__ void cluster_arrive_started() {
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 }
@@ -371,6 +371,39 @@ __device__ __forceinline__ void write_words(T *d, int n, X &&x, float2 nm,
   }
 }
 
+// put(entry, q of all entries of its class) of every entry k that is the warp's:
+// mine(class) says so of a class.  Entries of one class, which add up, so meet
+// in one warp, where each lane holds entries lane + 32 i.
+template <class Mine, class Put>
+__device__ __forceinline__ void each_entry(const int32_t *ids, const float *qs,
+                                           int K, Mine &&mine, Put &&put) {
+  const int lane = threadIdx.x & 31;
+  int32_t id[4];
+  float q[4], both[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int k = lane + 32 * i;
+    id[i] = k < K && ids[k] >= 0 && mine(ids[k]) ? ids[k] : -1;
+    q[i] = k < K ? qs[k] : 0.0f;
+    both[i] = 0.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (32 * i >= K) break;
+    for (uint32_t has = __ballot_sync(~0u, id[i] >= 0); has; has &= has - 1) {
+      const int from = __ffs(has) - 1;
+      const int32_t of = __shfl_sync(~0u, id[i], from);
+      const float add = __shfl_sync(~0u, q[i], from);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (id[j] == of) both[j] += add;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (id[i] >= 0) put(lane + 32 * i, both[i]);
+}
+
 // A value that at least K of n <= N orders reach, and hardly more: the largest
 // one with the low 16 bits zero (all there is to a 16-bit logit), or what all n
 // have in common; the order of the lowest logit if fewer than K are logits.
@@ -408,6 +441,15 @@ __device__ __forceinline__ uint32_t reached_by(int K, const uint32_t *values,
 // before the one exchange of (m, s, u) over the team; then the alternatives or
 // the gradient come from the slab.  Memory traffic is that of the operator
 // itself: the row once in, results or gradient once out.
+//
+// For a gradient three slabs of 64 KB lie on an SM (two load while one
+// computes): 3687 rows of 131072 bf16 logits, in clusters of four, take 410 us,
+// 5.0 TB/s.  What bounds it is a CTA's life, not the memory: load, exchange and
+// two bursts of ex2 one after the other (without any ex2 it is 378 us, rows of
+// one CTA each 345).  Measured and not kept: slabs of 32 KB (the same with 128
+// threads), one CTA an SM that takes row after row and copies the next into
+// its place (510 us), the second read out of the L2 (440 us and more; of
+// 77 MB of rows in work a third is still there).
 enum Mode { kRead = 0, kReadTop = 1, kLoss = 2, kLossGrad = 3, kBack = 4 };
 
 constexpr int kMaxCluster = 16;
@@ -867,52 +909,37 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
     }
     // An entry's element is written again, after its first value: by the warp
     // that wrote that (of another alignment: by any one, after all have).
-    // Entries of one class, which add up, meet in the same warp.
     const bool aligned = dm == mis;
     if (aligned)
       __syncwarp();
     else
       __syncthreads();
-    if (!bad && !empty) {
-      int32_t id[4];
-      float q[4], both[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        id[i] = -1;
-        both[i] = 0.0f;
-        const int k = lane + 32 * i;
-        if (k >= p.te.k) continue;
-        const int e = sid[k] - first;
-        if (sid[k] >= 0 && e >= 0 && e < n &&
-            (aligned ? (e + mis) / E % NT >> 5 : e % kWarps) == warp)
-          id[i] = e;
-        q[i] = sq[k];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (32 * i >= p.te.k) break;
-        for (uint32_t has = __ballot_sync(~0u, id[i] >= 0); has; has &= has - 1) {
-          const int from = __ffs(has) - 1;
-          const int32_t of = __shfl_sync(~0u, id[i], from);
-          const float add = __shfl_sync(~0u, q[i], from);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (id[j] == of) both[j] += add;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (id[i] >= 0)
-          d[id[i]] = from_f<T>(
-              w * (ex2((to_f(sx[id[i]]) - m) * a.c) / s - both[i]));
-    }
+    if (!bad && !empty)
+      each_entry(
+          sid, sq, p.te.k,
+          [&](int32_t id) {
+            const int e = id - first;
+            return e >= 0 && e < n &&
+                   (aligned ? (e + mis) / E % NT / 32 : e % kWarps) == warp;
+          },
+          [&](int k, float q) {
+            const int e = sid[k] - first;
+            d[e] = from_f<T>(w * (ex2((to_f(sx[e]) - m) * a.c) / s - q));
+          });
   }
 }
 
 // ------------------------------------------------------------ a CTA a row
-// Enough wide rows to fill the SMs, and no gradient: a CTA streams its row
-// through registers, four granules a thread at a time with the next four in
-// flight, and nothing of the row is kept.  One exchange at the end.
+// Short rows, and wide ones without a gradient that are enough to fill the SMs:
+// a CTA streams its row through registers, four granules a thread at a time,
+// and nothing of the row is kept.  One exchange at the end; a gradient reads
+// the row again.  Without alternatives the next four granules are on their way
+// while four are worked on; with them (more registers) more CTAs do as well.
+//
+// Bound by the memory: 3687 rows of 131072 bf16 logits take 141 us, 6.9 TB/s
+// (measured with alternatives: 2048 rows and 64 of them 109 us, 83 without --
+// the search after a row's end is what is left over).  One ex2 a logit keeps
+// the special-function unit busy for two thirds of that time.
 //
 // For the alternatives each thread notes the maximum of every run of granules
 // it read.  The K-th largest of the threads' maxima is a lower bound of the
@@ -945,7 +972,7 @@ __global__ void __launch_bounds__(NT) k_stream(StreamArgs p) {
   __shared__ uint64_t picked[kTop ? kPicked : 1];
   __shared__ uint32_t misc[4];  // runs to read, tau, logits picked
   constexpr bool kGrad = MODE == kLossGrad;
-  __shared__ float sq[kGrad ? kMaxTop : 1];
+  __shared__ float sq[kGrad ? kMaxTop : 1], sxk[kGrad ? kMaxTop : 1];
   __shared__ int32_t sid[kGrad ? kMaxTop : 1];
   const RowArgs &a = p.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -1148,6 +1175,7 @@ __global__ void __launch_bounds__(NT) k_stream(StreamArgs p) {
         const int k = lane + 32 * i;
         if (k < p.te.k) {
           sq[k] = tq[i] / ys;
+          sxk[k] = xk[i];
           sid[k] = tid_[i];
         }
       }
@@ -1182,16 +1210,13 @@ __global__ void __launch_bounds__(NT) k_stream(StreamArgs p) {
       write_words<T, NT>(d, V, [&](int e) { return to_f(x[e]); }, nm, c2, w2);
     }
     __syncthreads();  // an entry's element is written again, after its first value
-    if (warp == 0 && !end.bad && !end.empty) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (tid_[i] < 0) continue;
-        float both = 0.0f;  // entries of one class add up
-        for (int j = 0; j < p.te.k; ++j) both += sid[j] == tid_[i] ? sq[j] : 0.0f;
-        d[tid_[i]] =
-            from_f<T>(w * (ex2((xk[i] - end.m) * a.c) / end.s - both));
-      }
-    }
+    if (!end.bad && !end.empty)
+      each_entry(
+          sid, sq, p.te.k, [&](int32_t id) { return id % kWarps == warp; },
+          [&](int k, float q) {
+            d[sid[k]] =
+                from_f<T>(w * (ex2((sxk[k] - end.m) * a.c) / end.s - q));
+          });
   }
   if constexpr (kTop) {
     const int K = p.top_k;
@@ -2177,6 +2202,8 @@ RowArgs check_logits(const char *who, const tmnn_logits &x) {
     bad(std::string(who) + ": temperature must be in [1e-4, 1e4]");
   if (x.row_stride < 0 || x.row_stride > (int64_t)1 << 40)
     bad(std::string(who) + ": row_stride must be in [0, 2^40]");
+  if (x.rows > 1 && x.row_stride > ((int64_t)1 << 56) / (int64_t)x.rows)
+    bad(std::string(who) + ": the rows span more than memory");
   if (x.rows) check_ptr(who, "logits", x.data, elem_size(x.dtype));
   RowArgs a;
   a.x = x.data;
@@ -2195,20 +2222,40 @@ void check_index(const char *who, int type) {
 }
 size_t index_size(int type) { return type == TMNN_INDEX_I64 ? 8 : 4; }
 
+// The bytes from a first to behind a last one.
+struct Span {
+  uintptr_t from, to;
+  Span(const void *p, uint64_t bytes)
+      : from((uintptr_t)p), to(p ? (uintptr_t)p + bytes : (uintptr_t)p) {}
+  bool meets(const Span &o) const { return from < o.to && o.from < to; }
+};
+Span rows_of(const void *p, uint64_t rows, int64_t stride, uint64_t classes,
+             int size) {
+  return Span(p, ((rows - 1) * (uint64_t)stride + classes) * size);
+}
+Span logits_of(const tmnn_logits &x) {
+  return rows_of(x.data, x.rows, x.row_stride, x.classes, elem_size(x.dtype));
+}
+void check_apart(const char *who, const char *what, const Span &out,
+                 std::initializer_list<Span> others) {
+  for (const Span &o : others)
+    if (out.meets(o))
+      bad(std::string(who) + ": " + what + " overlaps another argument");
+}
+
 // The gradient's rows: as wide as the classes, and either the logits' own
 // memory or apart from it.
-void check_grad(const char *who, const tmnn_logits &x, const void *d,
+Span check_grad(const char *who, const tmnn_logits &x, const void *d,
                 int64_t stride) {
   check_ptr(who, "d_logits", d, elem_size(x.dtype));
-  if (stride < (int64_t)x.classes || stride > (int64_t)1 << 40)
+  if (stride < (int64_t)x.classes || stride > (int64_t)1 << 40 ||
+      (x.rows > 1 && stride > ((int64_t)1 << 56) / (int64_t)x.rows))
     bad(std::string(who) + ": d_row_stride must be in [classes, 2^40]");
-  if (d == x.data && stride == x.row_stride) return;
-  const uintptr_t size = elem_size(x.dtype), n = x.rows;
-  const uintptr_t xb = (uintptr_t)x.data, db = (uintptr_t)d;
-  const uintptr_t xe = xb + ((n - 1) * x.row_stride + x.classes) * size;
-  const uintptr_t de = db + ((n - 1) * stride + x.classes) * size;
-  if (db < xe && xb < de)
+  const Span span = rows_of(d, x.rows, stride, x.classes, elem_size(x.dtype));
+  const bool same = d == x.data && (stride == x.row_stride || x.rows == 1);
+  if (!same && span.meets(logits_of(x)))
     bad(std::string(who) + ": d_logits overlaps the logits in part");
+  return span;
 }
 
 #define BY_DTYPE(dtype, ...)                 \
@@ -2452,6 +2499,17 @@ int launch_token_logprobs(const tmnn_logits &x, const void *tokens,
     check_ptr(who, "top_ids", o.top_ids, 4);
     check_ptr(who, "top_logprobs", o.top_logprobs, 4);
   }
+  const uint64_t n = x.rows;
+  const Span in = logits_of(x), toks(tokens, n * index_size(index_type));
+  const Span out[] = {{o.logprob, n * 4},
+                      {o.entropy, n * 4},
+                      {top_k ? o.top_ids : nullptr, n * top_k * 4},
+                      {top_k ? o.top_logprobs : nullptr, n * top_k * 4},
+                      {o.stats, n * 12}};
+  for (int i = 0; i < 5; ++i) {
+    check_apart(who, "an output", out[i], {in, toks});
+    for (int j = 0; j < i; ++j) check_apart(who, "an output", out[i], {out[j]});
+  }
   return in_parts(x.rows, [&](uint32_t i, uint32_t n) {
     TeamArgs p{};
     p.a = a;
@@ -2515,7 +2573,12 @@ int launch_token_logprobs_backward(const tmnn_logits &x, const void *tokens,
   check_ptr(who, "stats", stats, 4);
   check_opt(who, "d_logprob", d_logprob, 4);
   check_opt(who, "d_entropy", d_entropy, 4);
-  check_grad(who, x, d_logits, d_stride);
+  const uint64_t rows = x.rows;
+  check_apart(who, "d_logits", check_grad(who, x, d_logits, d_stride),
+              {{tokens, rows * index_size(index_type)},
+               {stats, rows * 12},
+               {d_logprob, rows * 4},
+               {d_entropy, rows * 4}});
   const int size = elem_size(x.dtype), per_run = 32 * kRun * (16 / size);
   // one granule more than the row's bytes hold: rows may start inside one
   const uint32_t runs = (x.classes + 16 / size + per_run - 1) / per_run;
@@ -2575,7 +2638,15 @@ int launch_distill(const tmnn_logits &x, const void *ids, int index_type,
   check_ptr(who, "teacher_logits", teacher, elem_size(teacher_dtype));
   check_opt(who, "row_weight", row_weight, 4);
   check_ptr(who, "loss", loss, 4);
-  if (d_logits) check_grad(who, x, d_logits, d_stride);
+  const uint64_t rows = x.rows;
+  const Span id_span(ids, rows * k * index_size(index_type)),
+      teacher_span(teacher, rows * k * elem_size(teacher_dtype)),
+      weights(d_logits ? row_weight : nullptr, rows * 4), losses(loss, rows * 4);
+  check_apart(who, "loss", losses,
+              {logits_of(x), id_span, teacher_span, weights});
+  if (d_logits)
+    check_apart(who, "d_logits", check_grad(who, x, d_logits, d_stride),
+                {id_span, teacher_span, weights, losses});
   const int size = elem_size(x.dtype);
   return in_parts(x.rows, [&](uint32_t i, uint32_t n) {
     TeamArgs p{};
