@@ -550,12 +550,14 @@ class Trainer:
     inference_with_gradient = evaluate_with_gradient
 
     # ------------------------------------------------- class-logit outputs
-    def _class_ids(self, ids, name, shape, flags):
+    def _class_ids(self, ids, name, shape, flags, input):
         """(pointer, index type, keepalive) of class ids placed like input."""
         if ids is None:
             return None, 0, None
         if _is_cuda_tensor(ids) != bool(flags & _abi.PTR_DEVICE):
             raise ValueError(f"input and {name} must both be host or both CUDA")
+        if flags & _abi.PTR_DEVICE and ids.device != input.device:
+            raise ValueError(f"input and {name} must be on one device")
         if flags & _abi.PTR_DEVICE:
             contiguous, ptr = ids.is_contiguous(), C.c_void_p(ids.data_ptr())
         else:
@@ -585,7 +587,7 @@ class Trainer:
         arrays or CUDA tensors, like inference()."""
         h = self._handle()
         pp, n, flags, _k = _arg(input, "input", self.n_input)
-        ip, it, _k2 = self._class_ids(tokens, "tokens", (n,), flags)
+        ip, it, _k2 = self._class_ids(tokens, "tokens", (n,), flags, input)
         k = int(top_k)
         if not 0 <= k <= min(self.n_output, _abi.MAX_TOP):
             raise ValueError("top_k must be in [0, min(n_output, 128)]")
@@ -624,10 +626,13 @@ class Trainer:
         if len(teacher_ids.shape) != 2:
             raise ValueError("teacher_ids must be 2D (batch_size, k)")
         k = int(teacher_ids.shape[1])
-        ip, it, _k2 = self._class_ids(teacher_ids, "teacher_ids", (n, k), flags)
+        ip, it, _k2 = self._class_ids(teacher_ids, "teacher_ids", (n, k), flags,
+                                      input)
         yp, ny, fy, _k3 = _arg(teacher_logits, "teacher_logits", k)
-        if ny != n or fy != flags:
-            raise ValueError("input and teacher_logits must match")
+        if ny != n or fy != flags or (
+                fy and teacher_logits.device != input.device):
+            raise ValueError("input and teacher_logits must match in rows and "
+                             "placement")
         if flags & _abi.PTR_DEVICE:
             self._after_current_stream(input)
         loss = C.c_float()
