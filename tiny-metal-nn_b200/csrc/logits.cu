@@ -56,13 +56,7 @@ __global__ void __launch_bounds__(256)
       const int g = g0 + 32 * i, e0 = g * E - mis;
       if (e0 >= 0 && e0 + E <= V) {
         float r[E];
-#pragma unroll
-        for (int j = 0; j < E / 2; ++j) {
-          float u, v;
-          split(pair_of<T>(q[i], j), u, v);
-          r[2 * j] = b.at(u, e0 + 2 * j, a.c);
-          r[2 * j + 1] = b.at(v, e0 + 2 * j + 1, a.c);
-        }
+        b.granule<T>(q[i], e0, a.c, r);
         dst[g] = pack_granule<T>(r);
       } else {
         for (int j = 0; j < E; ++j) {
@@ -73,11 +67,17 @@ __global__ void __launch_bounds__(256)
       }
     }
   } else {
-    const int e0 = run * 32 * kRun * E + lane;
-#pragma unroll 8
-    for (int i = 0; i < kRun * E; ++i) {
-      const int e = e0 + 32 * i;
-      if (e < V) d[e] = from_f<T>(b.idle ? 0.0f : b.at(to_f(x[e]), e, a.c));
+    // rows of another alignment: the run's part of the row, in granules of d
+    const int e0 = max(0, run * 32 * kRun * E - dm);
+    const int e1 = min(V, (run + 1) * 32 * kRun * E - dm);
+    if (b.idle) {
+      for (int e = e0 + lane; e < e1; e += 32) d[e] = from_f<T>(0.0f);
+    } else {
+      write_shifted<T>(d + e0, x + e0, e1 - e0, lane, 32,
+                       e1 + E <= V ? 0 : E,
+                       [&](const uint4 &q, int e, float *r) {
+                         b.granule<T>(q, e0 + e, a.c, r);
+                       });
     }
   }
 }

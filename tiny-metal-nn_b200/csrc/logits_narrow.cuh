@@ -473,22 +473,17 @@ __global__ void __launch_bounds__(128) k_narrow(NarrowArgs p) {
   T *d = MODE == kLossGrad || MODE == kBack
              ? static_cast<T *>(p.dx) + (int64_t)row * p.d_stride
              : nullptr;
-  // writes what f(value, next value, element, to, next to) gives of every pair
+  // writes what f(granule, first element, to) gives
   auto write_rows = [&](auto &&f) {
     const int dm = (int)((uintptr_t)d & 15) / (int)sizeof(T);
-    uint4 *dst = reinterpret_cast<uint4 *>(d - dm);
     if (!on) return;
+    uint4 *dst = reinterpret_cast<uint4 *>(d - dm);
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
       const int g = l + L * j, e0 = g * E - mis;
       if (g >= G) continue;
       float r[E];
-#pragma unroll
-      for (int i = 0; i < E / 2; ++i) {
-        float u, v;
-        split(pair_of<T>(q[j], i), u, v);
-        f(u, v, e0 + 2 * i, r[2 * i], r[2 * i + 1]);
-      }
+      f(q[j], e0, r);
       if (dm == mis && !(mis && g == 0) && g < whole) {
         dst[g] = pack_granule<T>(r);
       } else {
@@ -501,10 +496,7 @@ __global__ void __launch_bounds__(128) k_narrow(NarrowArgs p) {
 
   if constexpr (MODE == kBack) {
     const BackRow b(a, p.tokens, p.itype, p.stats, p.d_logprob, p.d_entropy, row);
-    write_rows([&](float u, float v, int e, float &ru, float &rv) {
-      ru = b.at(u, e, a.c);
-      rv = b.at(v, e + 1, a.c);
-    });
+    write_rows([&](const uint4 &g, int e, float *r) { b.granule<T>(g, e, a.c, r); });
     return;
   }
 
@@ -737,10 +729,11 @@ __global__ void __launch_bounds__(128) k_narrow(NarrowArgs p) {
       const float m0 = zero ? 0.0f : end.m;
       __syncwarp();  // every lane has read what the row's lanes now write
       const float2 nm = f2(-m0, -m0), c2 = f2(a.c, a.c), w2 = f2(ws, ws);
-      write_rows([&](float u, float v, int, float &ru, float &rv) {
-        const float2 t = __fmul2_rn(__fadd2_rn(f2(u, v), nm), c2);
-        split(__fmul2_rn(f2(ex2(t.x), ex2(t.y)), w2), ru, rv);
-        if (zero) ru = rv = 0.0f;
+      write_rows([&](const uint4 &g, int, float *r) {
+        softmax_granule<T>(g, nm, c2, w2, r);
+        if (zero)
+#pragma unroll
+          for (int i = 0; i < E; ++i) r[i] = 0.0f;
       });
       __syncwarp();  // an entry's element is written again
       if (on && !zero && !end.bad)

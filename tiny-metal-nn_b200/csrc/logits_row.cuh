@@ -342,11 +342,74 @@ __device__ __forceinline__ void write_zeros(T *d, int n) {
   }
 }
 
-// d[e] = e^((x(e) - m) / T) w for e < n in words of 4 bytes, lanes side by side:
-// for gradients that lie otherwise in their granules than the logits.  By all
+// The granule that starts at any element: the two around it, shifted.  All of
+// its elements are the caller's; the second granule may end up to 16 bytes
+// behind them.
+template <class T>
+__device__ __forceinline__ uint4 granule_at(const T *p) {
+  const uint32_t at = (uint32_t)(uintptr_t)p & 15;
+  const uint4 *base = reinterpret_cast<const uint4 *>(
+      reinterpret_cast<const unsigned char *>(p) - at);
+  const uint4 a = base[0], b = at ? base[1] : a;
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  if (at & 8)
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+  if (at & 4)
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+  const uint32_t bits = (at & 3) * 8;
+  return uint4{
+      __funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+      __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits)};
+}
+
+// The n elements of a row part x in memory as gradients to d, whose granules lie
+// otherwise than those of x: thread `tid` of `threads` takes granules of d, body(granule
+// of x, first element, its E results).  `slack`: how near to the end of x a
+// granule of it may not be read whole, E at a row's end and 0 where the row goes
+// on.
+template <class T, class Body>
+__device__ __forceinline__ void write_shifted(T *d, const T *x, int n, int tid,
+                                              int threads, int slack,
+                                              Body &&body) {
+  constexpr int E = kElems<T>;
+  const int dm = (int)((uintptr_t)d & 15) / (int)sizeof(T);
+  uint4 *dst = reinterpret_cast<uint4 *>(d - dm);
+  const int G = n > 0 ? (dm + n + E - 1) / E : 0;
+  for (int g0 = tid; g0 < G; g0 += 4 * threads) {
+    uint4 q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int e = (g0 + i * threads) * E - dm;
+      if (e >= 0 && e + E + slack <= n) q[i] = granule_at(x + e);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int g = g0 + i * threads, e = g * E - dm;
+      float r[E];
+      if (e >= 0 && e + E + slack <= n) {
+        body(q[i], e, r);
+        dst[g] = pack_granule<T>(r);
+      } else if (g < G) {  // the ends
+        T v[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          v[j] = e + j >= 0 && e + j < n ? x[e + j] : from_f<T>(-kInf);
+        body(*reinterpret_cast<const uint4 *>(v), e, r);
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          if (e + j >= 0 && e + j < n) d[e + j] = from_f<T>(r[j]);
+      }
+    }
+  }
+}
+
+// d[e] = e^((x[e] - m) / T) w for e < n, where d lies otherwise in its granules
+// than x in shared memory: in words of 4 bytes, lanes side by side.  By all
 // threads; nm, c, w: -m, log2(e) / T and w twice.
-template <class T, int NT, class X>
-__device__ __forceinline__ void write_words(T *d, int n, X &&x, float2 nm,
+template <class T, int NT>
+__device__ __forceinline__ void write_words(T *d, const T *x, int n, float2 nm,
                                             float2 c, float2 w) {
   auto two = [&](float a, float b) {
     const float2 t = __fmul2_rn(__fadd2_rn(f2(a, b), nm), c);
@@ -358,15 +421,28 @@ __device__ __forceinline__ void write_words(T *d, int n, X &&x, float2 nm,
     uint32_t *words = reinterpret_cast<uint32_t *>(d + first);
 #pragma unroll 4
     for (int i = threadIdx.x; i < pairs; i += NT) {
-      const float2 r = two(x(first + 2 * i), x(first + 2 * i + 1));
+      const float2 r = two(to_f(x[first + 2 * i]), to_f(x[first + 2 * i + 1]));
       words[i] = pack2<T>(r.x, r.y);
     }
-    if (threadIdx.x == 0 && first && n > 0) d[0] = from_f<T>(two(x(0), 0.0f).x);
+    if (threadIdx.x == 0 && first && n > 0)
+      d[0] = from_f<T>(two(to_f(x[0]), 0.0f).x);
     if (threadIdx.x == 1 && first + 2 * pairs < n)
-      d[n - 1] = from_f<T>(two(x(n - 1), 0.0f).x);
+      d[n - 1] = from_f<T>(two(to_f(x[n - 1]), 0.0f).x);
   } else {
 #pragma unroll 4
-    for (int e = threadIdx.x; e < n; e += NT) d[e] = from_f<T>(two(x(e), 0.0f).x);
+    for (int e = threadIdx.x; e < n; e += NT)
+      d[e] = from_f<T>(two(to_f(x[e]), 0.0f).x);
+  }
+}
+
+// r = e^((x - m) / T) w of a granule; nm, c, w: -m, log2(e) / T and w twice
+template <class T>
+__device__ __forceinline__ void softmax_granule(const uint4 &g, float2 nm,
+                                                float2 c, float2 w, float *r) {
+#pragma unroll
+  for (int i = 0; i < kElems<T> / 2; ++i) {
+    const float2 t = __fmul2_rn(__fadd2_rn(pair_of<T>(g, i), nm), c);
+    split(__fmul2_rn(f2(ex2(t.x), ex2(t.y)), w), r[2 * i], r[2 * i + 1]);
   }
 }
 
@@ -460,6 +536,16 @@ struct BackRow {
     const float inv_s = 1.0f / s;
     k1 = -b * kLn2 * inv_s;
     k0 = -(b == 0.0f ? g : g + b * (h - logf(s))) * inv_s;
+  }
+  template <class T>
+  __device__ __forceinline__ void granule(const uint4 &g, int e, float c,
+                                          float *r) const {
+#pragma unroll
+    for (int i = 0; i < kElems<T> / 2; ++i) {
+      const float2 v = pair_of<T>(g, i);
+      r[2 * i] = at(v.x, e + 2 * i, c);
+      r[2 * i + 1] = at(v.y, e + 2 * i + 1, c);
+    }
   }
   // element e of value v
   __device__ __forceinline__ float at(float v, int e, float c) const {

@@ -461,11 +461,7 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
       for (int g = mine0; g < hi; g += NT) {
         const uint4 q = slab[g];
         float r[E];
-#pragma unroll
-        for (int i = 0; i < E / 2; ++i) {
-          const float2 t = __fmul2_rn(__fadd2_rn(pair_of<T>(q, i), nm), c2);
-          split(__fmul2_rn(f2(ex2(t.x), ex2(t.y)), w2), r[2 * i], r[2 * i + 1]);
-        }
+        softmax_granule<T>(q, nm, c2, w2, r);
         dst[g] = pack_granule<T>(r);
       }
       edges([&](int e) {
@@ -475,7 +471,7 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
     } else {
       // rows of another alignment (the copies of other threads are visible
       // since the exchange)
-      write_words<T, NT>(d, n, [&](int e) { return to_f(sx[e]); }, nm, c2, w2);
+      write_words<T, NT>(d, sx, n, nm, c2, w2);
     }
     // An entry's element is written again, after its first value: by the warp
     // that wrote that (of another alignment: by any one, after all have).
@@ -764,11 +760,7 @@ __global__ void __launch_bounds__(NT) k_stream(StreamArgs p) {
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
           float r[E];
-#pragma unroll
-          for (int j = 0; j < E / 2; ++j) {
-            const float2 t = __fmul2_rn(__fadd2_rn(pair_of<T>(g[i], j), nm), c2);
-            split(__fmul2_rn(f2(ex2(t.x), ex2(t.y)), w2), r[2 * j], r[2 * j + 1]);
-          }
+          softmax_granule<T>(g[i], nm, c2, w2, r);
           const int f = (b * kBatch + i) * NT + tid;
           if (b < whole || f < F) dst[f] = pack_granule<T>(r);
         }
@@ -777,7 +769,9 @@ __global__ void __launch_bounds__(NT) k_stream(StreamArgs p) {
         d[odd_class] = from_f<T>(ex2((odd - m0) * a.c) * ws);
     } else {
       // rows of another alignment
-      write_words<T, NT>(d, V, [&](int e) { return to_f(x[e]); }, nm, c2, w2);
+      write_shifted<T>(d, x, V, tid, NT, E, [&](const uint4 &g, int, float *r) {
+        softmax_granule<T>(g, nm, c2, w2, r);
+      });
     }
     __syncthreads();  // an entry's element is written again, after its first value
     if (!end.bad && !end.empty)

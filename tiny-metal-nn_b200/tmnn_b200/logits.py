@@ -146,8 +146,8 @@ def token_logprobs(logits, tokens=None, *, top_k=0, temperature=1.0,
         lpp = lp.data_ptr()
     ent = empty(n, dtype=f32, device=dev) if lp is None else _torch.empty_like(lp)
     if k:
-        ids = empty(n, k, dtype=_torch.int32, device=dev)
-        top = empty(n, k, dtype=f32, device=dev)
+        top = ent.new_empty(n, k)
+        ids = _torch.empty_like(top, dtype=_torch.int32)
         idp, topp = ids.data_ptr(), top.data_ptr()
     if stats:
         st = empty(n, 3, dtype=f32, device=dev)
