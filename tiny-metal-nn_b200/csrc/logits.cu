@@ -305,11 +305,17 @@ template <class T, int MODE>
 void launch_stream(const TeamArgs &p, cudaStream_t st) {
   const StreamArgs q{p.a,  p.tokens,     p.itype,  p.top_k, p.o,       p.te,
                      p.row_weight, p.weight, p.loss, p.dx, p.d_stride};
-  // With many rows a few batches a thread at least, and maxima well above the
-  // alternatives in number; few rows are over sooner with more threads.
-  if (p.a.classes <= 4 * 4 * 256 * kElems<T> &&
-      (int64_t)p.a.rows >= (int64_t)sm_count() &&
-      (MODE != kReadTop || p.top_k <= 32))
+  // With many rows a few batches a thread, so that little of its time goes into
+  // a row's start and end (70130 rows of 2215 bf16 logits, distilled: 239 us
+  // with 64 threads, 303 with 128; 16384 of 8192 fp32: 236 and 185); few rows
+  // are over sooner with more threads.  For alternatives the threads' maxima
+  // must be well above them in number.
+  const int granules = p.a.classes / kElems<T>;
+  const bool many = (int64_t)p.a.rows >= (int64_t)sm_count() &&
+                    (MODE != kReadTop || p.top_k <= 32);
+  if (many && granules <= 1024)
+    k_stream<T, 64, MODE><<<p.a.rows, 64, 0, st>>>(q);
+  else if (many && granules <= 4096)
     k_stream<T, 128, MODE><<<p.a.rows, 128, 0, st>>>(q);
   else
     k_stream<T, 256, MODE><<<p.a.rows, 256, 0, st>>>(q);
