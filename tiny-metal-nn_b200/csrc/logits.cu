@@ -336,7 +336,9 @@ void launch_tiny(TinyArgs &p, cudaStream_t st) {
   const bool quads = V % 4 == 0;
   p.pitch = quads ? (V / 4 | 1) * 4 : V;
   auto packed = [&](const void *at, int64_t stride) {
-    return (uintptr_t)at % 16 == 0 && (stride == V || p.a.rows == 1);
+    return (uintptr_t)at % 16 == 0 &&
+           (stride == V || p.a.rows == 1 ||
+            (quads && stride % 4 == 0 && stride < 1 << 25));
   };
   p.packed = packed(p.a.x, p.a.stride);
   p.d_packed = packed(p.dx, p.d_stride);

@@ -28,7 +28,8 @@ struct TinyArgs {
   void *dx;
   int64_t d_stride;
   int pitch;            // floats between rows in shared memory
-  int packed, d_packed; // rows without gaps from a 16-byte boundary on
+  int packed, d_packed; // rows from a 16-byte boundary on that have no gaps, or
+                        // whose quads lie on boundaries of their size
 };
 
 // EIGHTS: eights of classes a row may have
@@ -69,19 +70,20 @@ __global__ void __launch_bounds__(128) k_tiny(TinyArgs p) {
         if (rs[i] < rows) use(rs[i], cs[i], v[i]);
     }
   };
-  // The same of every quad of packed rows: load(quad), then use(first of its
-  // four places in the image, quad, value).
-  auto each_quad = [&](int end, auto &&load, auto &&use) {
+  // The same of every quad of packed rows `stride` apart: load(its first place in
+  // the image, in memory), then use(both, value); four in flight.
+  auto each_quad = [&](int end, int stride, auto &&load, auto &&use) {
     const int R = QUADS ? V / 4 : 1;  // quads a row
     int r = lane / R, c = lane - r * R;
     const int dr = 32 / R, dc = 32 - dr * R;
     for (int i0 = lane; i0 - lane < end; i0 += 128) {
-      int at[4];
+      int at[4], from[4];
       decltype(load(0, 0)) v[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         at[i] = QUADS ? r * P + c * 4 : (i0 + 32 * i) * 4;
-        if (i0 + 32 * i < end) v[i] = load(at[i], i0 + 32 * i);
+        from[i] = QUADS ? r * stride + c * 4 : at[i];
+        if (i0 + 32 * i < end) v[i] = load(at[i], from[i]);
         if (QUADS) {
           r += dr;
           c += dc;
@@ -90,7 +92,7 @@ __global__ void __launch_bounds__(128) k_tiny(TinyArgs p) {
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (i0 + 32 * i < end) use(at[i], i0 + 32 * i, v[i]);
+        if (i0 + 32 * i < end) use(at[i], from[i], v[i]);
     }
   };
 
@@ -106,16 +108,16 @@ __global__ void __launch_bounds__(128) k_tiny(TinyArgs p) {
   if (p.packed) {
     if constexpr (sizeof(T) == 4) {
       each_quad(
-          quads,
-          [&](int at, int i) {
-            copy16(image + at, reinterpret_cast<const uint4 *>(x) + i);
+          quads, (int)a.stride,
+          [&](int at, int from) {
+            copy16(image + at, x + from);
             return 0;
           },
           [](int, int, int) {});
     } else {
       each_quad(
-          quads,
-          [&](int, int i) { return reinterpret_cast<const uint2 *>(x)[i]; },
+          quads, (int)a.stride,
+          [&](int, int from) { return *reinterpret_cast<const uint2 *>(x + from); },
           [&](int at, int, const uint2 &w) {
             const uint4 g{w.x, w.y, 0, 0};
             float4 v;
@@ -363,13 +365,13 @@ __global__ void __launch_bounds__(128) k_tiny(TinyArgs p) {
     T *d = static_cast<T *>(p.dx) + (int64_t)row0 * p.d_stride;
     if (p.d_packed) {
       each_quad(
-          quads,
+          quads, (int)p.d_stride,
           [&](int at, int) { return *reinterpret_cast<const float4 *>(image + at); },
-          [&](int, int i, const float4 &v) {
+          [&](int, int to, const float4 &v) {
             if constexpr (sizeof(T) == 4)
-              reinterpret_cast<float4 *>(d)[i] = v;
+              *reinterpret_cast<float4 *>(d + to) = v;
             else
-              reinterpret_cast<uint2 *>(d)[i] =
+              *reinterpret_cast<uint2 *>(d + to) =
                   uint2{pack2<T>(v.x, v.y), pack2<T>(v.z, v.w)};
           });
       const int e = quads * 4 + lane;
