@@ -13,6 +13,10 @@ namespace logits {
 // is reduced over lanes.  Rows of whole quads lie `pitch` apart, an odd number
 // of quads, so that the lanes' 16-byte reads meet different banks; other rows
 // keep their distance V (odd, or twice an odd number).
+//
+// Bound by the instructions, 40 to 50 of a warp a row: 262144 rows of 64 fp32
+// logits with 4 alternatives take 21 us, 3.8 TB/s (lanes side by side: 43 us),
+// of 19 classes, distilled from 4 entries, 17 us, 3.3 TB/s (27 us).
 constexpr int kTinyClasses = 128;
 
 struct TinyArgs {
@@ -389,8 +393,14 @@ __global__ void __launch_bounds__(128) k_tiny(TinyArgs p) {
 // ------------------------------------------------------------ lanes a row
 // Narrow rows: 1 to 32 neighbouring lanes hold a row in registers, NG granules
 // each (granule lane + lanes * j), and reduce over one another with shuffles.
-// There is no shared memory but for a teacher's entries, and nothing is read
-// or written twice.
+// There is no shared memory but for a teacher's entries and the listed
+// alternatives, and nothing is read or written twice.
+//
+// 65536 rows of 1000 bf16 logits: backward 52 us, 5.1 TB/s; distilled from 10
+// entries 87 us; with 10 alternatives 95 us, bound by the instructions (1440 of
+// a warp a row; 193 us with one search through the row an alternative).  Two
+// granules more a lane than 8 cost more registers than they save (rows of 4039
+// fp16 logits: 190 us, streamed 144).
 struct NarrowArgs {
   RowArgs a;
   const void *tokens;

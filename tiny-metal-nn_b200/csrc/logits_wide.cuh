@@ -502,10 +502,11 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
 // the row again.  Without alternatives the next four granules are on their way
 // while four are worked on; with them (more registers) more CTAs do as well.
 //
-// Bound by the memory: 3687 rows of 131072 bf16 logits take 141 us, 6.9 TB/s
-// (measured with alternatives: 2048 rows and 64 of them 109 us, 83 without --
-// the search after a row's end is what is left over).  One ex2 a logit keeps
-// the special-function unit busy for two thirds of that time.
+// Bound by the memory: 3687 rows of 131072 bf16 logits take 155 us, 6.2 TB/s
+// (162 without the loads ahead, 170 with eight granules at a time).  One ex2 a
+// logit keeps the special-function unit busy for two thirds of that time.
+// With alternatives, 2048 rows and 64 of them: 110 us, 82 without; the search
+// after a row's end is what is left over.
 //
 // For the alternatives each thread notes the maximum of every run of granules
 // it read.  The K-th largest of the threads' maxima is a lower bound of the
