@@ -474,6 +474,51 @@ def test_streams_graphs_and_repeats():
             assert all(torch.equal(a, b) for a, b in zip(out, w))
 
 
+def test_two_threads_on_two_streams():
+    """Calls of several threads, each on a stream of its own, at once."""
+    import threading
+    import torch
+    import tmnn_b200 as t
+    out, errors = {}, []
+
+    def work(seed, V):
+        try:
+            g = torch.Generator(device="cuda").manual_seed(seed)
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                x = torch.randn(150, V, device="cuda", generator=g)
+                tok = torch.randint(0, V, (150,), device="cuda", generator=g)
+                y = torch.randn(150, 3, device="cuda", generator=g)
+                ids = torch.randint(0, V, (150, 3), device="cuda", generator=g)
+                one = torch.ones(150, device="cuda")
+                for _ in range(20):
+                    r = t.token_logprobs(x, tok, top_k=5, stats=True)
+                    d = t.token_logprobs_backward(x, tok, r.stats, one, one)
+                    e = t.distill_forward_backward(x, ids, y)
+            stream.synchronize()
+            out.setdefault((seed, V), []).append([*r, d, *e])
+        except Exception as ex:  # reported by the test's thread
+            errors.append(ex)
+
+    for _ in range(2):  # the second round's results are the first's
+        threads = [threading.Thread(target=work, args=(i, V))
+                   for i, V in enumerate((40, 700, 5000, 30000))]
+        for th in threads:
+            th.start()
+        for th in threads:
+            th.join()
+    assert not errors, errors
+    for first, second in out.values():
+        assert all(torch.equal(a, b) for a, b in zip(first, second))
+    for (seed, V), (first, _) in out.items():
+        torch.manual_seed(0)
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        x = torch.randn(150, V, device="cuda", generator=g)
+        tok = torch.randint(0, V, (150,), device="cuda", generator=g)
+        lone = t.token_logprobs(x, tok, top_k=5, stats=True)
+        assert all(torch.equal(a, b) for a, b in zip(first, lone))
+
+
 # ------------------------------------------------------ as they are used
 def test_teacher_to_student_run():
     """A teacher's logits -> its top classes -> the student's distillation

@@ -622,7 +622,6 @@ __global__ void __launch_bounds__(128) k_narrow(NarrowArgs p) {
       int *kept_at = reinterpret_cast<int *>(list + p.cap);
       int *count = kept_at + p.cap;
       if (l < 2) count[l] = 0;
-      if (L == 1) count[1] = 0;
       __syncwarp();
 #pragma unroll
       for (int j = 0; j < NG; ++j)

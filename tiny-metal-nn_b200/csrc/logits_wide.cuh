@@ -258,15 +258,11 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
     const int size = (int)C * NT / p.l.groups;
     for (int i = 1; i < size; i *= 2)
       o = max(o, __shfl_xor_sync(~0u, o, i));
-    if (C > 1) cluster_wait();
+    cluster_wait();
     if (tid % size == 0) {
       uint32_t *to = gmax + ((int)rank * NT + tid) / size;
-      if (C > 1) {
-        for (uint32_t r = 0; r < C; ++r)
-          peer_store(peer_addr(to, r), __uint_as_float(o));
-      } else {
-        *to = o;
-      }
+      for (uint32_t r = 0; r < C; ++r)
+        peer_store(peer_addr(to, r), __uint_as_float(o));
     }
     if (tid == 0) misc[0] = 0;  // candidates
   }
@@ -318,8 +314,9 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
     if (leader && tid == 0) write_read(p.o, row, end, tok_x, tok < a.classes);
 
   if constexpr (MODE == kReadTop) {
-    // ---- alternatives.  A value that at least K groups' maxima reach is a
-    // lower bound of the K-th largest logit, and few logits lie above it.
+    // ---- alternatives (of clusters only: what one CTA could hold is streamed).
+    // A value that at least K groups' maxima reach is a lower bound of the K-th
+    // largest logit, and few logits lie above it.
     const int K = p.top_k;
     int32_t *ids = p.o.top_ids + (int64_t)row * K;
     float *lps = p.o.top_logprobs + (int64_t)row * K;
@@ -347,8 +344,7 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
     int round = 0;
     auto collect = [&](uint64_t least) {
       const float floor = value_of((uint32_t)(least >> 32));
-      uint64_t *part = cand + (int)rank * p.l.cap;
-      const uint32_t to = C > 1 ? peer_addr(part, 0) : smem_addr(part);
+      const uint32_t to = peer_addr(cand + (int)rank * p.l.cap, 0);
       // The warp goes together through the granules of each thread that has
       // such a key: lanes 2 i and 2 i + 1 take the halves of granule i.
       uint32_t have = __ballot_sync(
@@ -369,25 +365,13 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
                   key_of(v, first + g * E + (lane & 1) * (E / 2) + i - mis);
               if (key >= least) {
                 const uint32_t at = atomicAdd(misc, 1u);
-                if (at < (uint32_t)p.l.cap) {
-                  if (C > 1)
-                    peer_store(to + at * 8, key);
-                  else
-                    part[at] = key;
-                }
+                if (at < (uint32_t)p.l.cap) peer_store(to + at * 8, key);
               }
             }
           }
         }
       }
       __syncthreads();
-      if (C == 1) {
-        const int M = (int)misc[0];
-        counts[0] = M;
-        __syncthreads();
-        if (tid == 0) misc[0] = 0;
-        return M;
-      }
       // two sets of counts in turn: one is written while the other is read
       uint32_t *now = counts + (round++ & 1) * kMaxCluster;
       if (tid < (int)C)
@@ -402,7 +386,7 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
       }
       return most > p.l.cap ? 0x7FFFFFFF : M;
     };
-    const int limit = C > 1 ? p.l.cap * 2 : p.l.cap;  // the first CTA ranks them
+    const int limit = p.l.cap * 2;  // the first CTA ranks them
     int M = collect((uint64_t)tau << 32);
     // Rows with many equal or regularly placed values overflow the buffers:
     // halve the interval of keys (which are distinct) until few enough, but K
@@ -417,7 +401,6 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
     }
     if (!leader) return;  // nothing of this CTA is read from here on
     const uint32_t *now = counts + ((round - 1) & 1) * kMaxCluster;
-    if (C == 1) now = counts;
     auto held = [&](uint32_t r) { return min((int)now[r], p.l.cap); };
     int all = 0;
     for (uint32_t r = 0; r < C; ++r) all += held(r);
