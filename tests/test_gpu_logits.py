@@ -600,6 +600,20 @@ def test_trainer_token_logprobs(n_out, family):
         tr.token_logprobs(pos, tok)
 
 
+def test_trainer_empty_cuda_batch():
+    """An empty CUDA batch, whose tensors have no address, is a no-op."""
+    import torch
+    with _field(16) as tr:
+        pos = torch.empty(0, 3, device="cuda")
+        r = tr.token_logprobs(pos, torch.empty(0, dtype=torch.int64,
+                                               device="cuda"), top_k=3)
+        assert r.logprob.shape == (0,) and r.top_ids.shape == (0, 3)
+        assert tr.token_logprobs(pos, top_k=2).entropy.shape == (0,)
+        ids = torch.empty(0, 2, dtype=torch.int32, device="cuda")
+        assert tr.distill_step(pos, ids, torch.empty(0, 2, device="cuda")) == 0.0
+        assert tr.step() == 0
+
+
 def _teacher(n, n_out, K, seed):
     rng = np.random.default_rng(seed)
     pos = rng.uniform(-1, 1, (n, 3)).astype(np.float32)

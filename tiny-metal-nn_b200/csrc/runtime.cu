@@ -1730,11 +1730,11 @@ void ctx_token_logprobs(tmnn_ctx &c, const float *pos, const void *tokens,
   // the arguments' checks, before anything is queued
   launch_token_logprobs(output_logits(c, nullptr, 0, temperature), tokens,
                         index_type, top_k, o, c.stream);
+  if (N == 0) return;
   if (top_k && (!o.top_ids || !o.top_logprobs))
     throw std::invalid_argument("token_logprobs: null top_ids or top_logprobs");
   if (o.logprob && !tokens)
     throw std::invalid_argument("token_logprobs: logprob needs tokens");
-  if (N == 0) return;
   CK(cudaSetDevice(c.device));
   ensure_batch(c, N);
   const float *p = stage_in(c, pos, (size_t)N * c.nd.d, c.pos_in, flags);
