@@ -603,6 +603,7 @@ const char *tmnn_cuda_logits_last_error(void);
 /* The same on a context whose outputs are class logits (classes =
  * num_outputs).  Host arrays, or device pointers with TMNN_PTR_DEVICE, like
  * the context's other calls; they run on the context's stream and wait.
+ * Pointers to another device's memory, or the host's own, are refused there.
  * token_logprobs: evaluate, then tmnn_cuda_token_logprobs.  Any output may be
  * NULL as above. */
 tmnn_status tmnn_cuda_ctx_token_logprobs(

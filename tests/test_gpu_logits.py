@@ -294,6 +294,68 @@ def test_distill_entry_counts(V, K):
         ref.assert_close(g.double().cpu(), d, _round(d, td, dtype), dtype)
 
 
+# a size of every kernel: rows of a thread, of some lanes, of a CTA, of a cluster
+EVERY = [(40, 19), (30, 1000), (20, 9001), (170, 33000), (5, 131072)]
+
+
+@pytest.mark.parametrize("n,V", EVERY)
+def test_ids_beyond_32_bits(n, V):
+    """Ids keep their 64 bits: one whose low half names a class is still none,
+    one below -2^31 is still padding."""
+    import torch
+    import tmnn_b200 as t
+    x, _ = make(n, V, "bf16", seed=V)
+    x[:5] = torch.linspace(-2, 2, V, device="cuda").bfloat16()
+    far = torch.tensor([(1 << 32) + 1, 1 << 31, (1 << 63) - 1, -(1 << 63),
+                        -(1 << 32) + 1], device="cuda")
+    tok = torch.ones(n, dtype=torch.int64, device="cuda")
+    tok[:5] = far
+    r = t.token_logprobs(x, tok, top_k=2, stats=True)
+    assert r.logprob[:3].isnan().all() and not r.entropy[:5].isnan().any()
+    assert (r.logprob[3:5] == 0).all() and (r.entropy[3:5] == 0).all()
+    first = (x[0] == x[0].max()).nonzero()[0]  # several classes round to 2
+    assert (r.top_ids[:3, 0] == first).all() and (r.top_ids[3:5] == -1).all()
+    one = torch.ones(n, device="cuda")
+    g = t.token_logprobs_backward(x, tok, r.stats, one, one)
+    assert g[:3].isnan().all() and (g[3:5] == 0).all()
+    ids = torch.stack([tok, torch.full_like(tok, 2)], 1)
+    y = torch.zeros(n, 2, device="cuda")
+    loss, g = t.distill_forward_backward(x, ids, y)
+    assert loss[:3].isnan().all() and g[:3].isnan().all()
+    ids[3:5, 0] = -1  # left out like the entries far below 0
+    l2, g2 = t.distill_forward_backward(x, ids, y)
+    assert torch.equal(loss[3:5], l2[3:5]) and torch.equal(g[3:5], g2[3:5])
+    assert not l2[3:5].isnan().any()
+    assert torch.equal(t.distill_loss(x, ids, y)[:3].isnan(), loss[:3].isnan())
+
+
+@pytest.mark.parametrize("n,V", EVERY)
+def test_gradient_factors_of_padding(n, V):
+    """Whatever the row weights and incoming gradients of padded rows and of
+    rows without a distribution hold, their gradient is 0; a weight of 0 gives
+    0 elsewhere."""
+    import torch
+    import tmnn_b200 as t
+    torch.manual_seed(V)
+    x = torch.randn(n, V, device="cuda")
+    x[2] = float("nan")
+    x[3] = float("-inf")
+    tok = torch.ones(n, dtype=torch.int64, device="cuda")
+    tok[1:3] = -1
+    ids = torch.ones(n, 3, dtype=torch.int64, device="cuda")
+    ids[1:3] = -1
+    w = torch.ones(n, device="cuda")
+    w[0], w[1], w[2], w[3] = 0.0, float("nan"), float("inf"), float("nan")
+    y = torch.zeros(n, 3, device="cuda")
+    _, g = t.distill_forward_backward(x, ids, y, row_weight=w)
+    assert (g[:4] == 0).all() and not g.isnan().any()
+    assert (g[4:].abs().amax(1) > 0).all()
+    r = t.token_logprobs(x, tok, stats=True)
+    g = t.token_logprobs_backward(x, tok, r.stats, w, w)
+    assert (g[:4] == 0).all() and not g.isnan().any()
+    assert (g[4:].abs().amax(1) > 0).all()
+
+
 def test_gradients_by_differences():
     """Central differences of the kernels' own values.  f32 values are off by
     about 16 u |value| < 4e-5 (derived bounds are below that at V = 9), so a
@@ -612,6 +674,35 @@ def test_trainer_empty_cuda_batch():
         ids = torch.empty(0, 2, dtype=torch.int32, device="cuda")
         assert tr.distill_step(pos, ids, torch.empty(0, 2, device="cuda")) == 0.0
         assert tr.step() == 0
+
+
+def test_trainer_refuses_host_memory_as_device_memory():
+    """Pointers flagged as device pointers that are the host's are refused
+    before anything is queued (another device's go the same way)."""
+    import ctypes as C
+    import torch
+    from tmnn_b200 import _abi
+    pos = torch.zeros(8, 3, device="cuda")
+    ids = torch.zeros(8, 2, dtype=torch.int32, device="cuda")
+    y = torch.zeros(8, 2, device="cuda")
+    ent = torch.zeros(8, device="cuda")
+    host = np.zeros((8, 3), np.float32)
+    at, far = (lambda t: C.c_void_p(t.data_ptr())), C.c_void_p(host.ctypes.data)
+    with _field(16) as tr:
+        h, lib, dev = tr._handle(), _abi.lib, _abi.PTR_DEVICE
+        for a in ((far, None, at(ent)), (at(pos), far, at(ent)),
+                  (at(pos), None, far)):
+            assert lib.tmnn_cuda_ctx_token_logprobs(
+                h, a[0], a[1], _abi.INDEX_I32, 8, 0, 1.0, dev, None, a[2], None,
+                None) == _abi.ERR_INVALID_ARGUMENT
+        loss = C.c_float(1.0)
+        for a in ((far, at(ids), at(y)), (at(pos), far, at(y)),
+                  (at(pos), at(ids), far)):
+            assert lib.tmnn_cuda_distill_step(
+                h, a[0], a[1], _abi.INDEX_I32, a[2], 8, 2, 1.0, dev,
+                C.byref(loss)) == _abi.ERR_INVALID_ARGUMENT
+        assert tr.step() == 0
+        assert tr.distill_step(pos, ids, y) >= 0.0
 
 
 def _teacher(n, n_out, K, seed):

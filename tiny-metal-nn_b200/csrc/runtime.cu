@@ -15,6 +15,7 @@
 #include <cmath>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <memory>
 #include <mutex>
 #include <stdexcept>
@@ -1717,6 +1718,23 @@ const void *stage_ids(tmnn_ctx &c, const void *src, int type, size_t count,
   return c.cls_ids.p;
 }
 
+// Refuses device pointers that the context's kernels cannot follow: memory of
+// another device or the host's own.
+void check_home(const tmnn_ctx &c, const char *who, uint32_t flags,
+                std::initializer_list<const void *> pointers) {
+  if (!(flags & TMNN_PTR_DEVICE)) return;
+  for (const void *p : pointers) {
+    if (!p) continue;
+    cudaPointerAttributes at{};
+    const cudaError_t e = cudaPointerGetAttributes(&at, p);
+    if (e != cudaSuccess) cudaGetLastError();
+    if (e != cudaSuccess || at.type == cudaMemoryTypeUnregistered ||
+        (at.type == cudaMemoryTypeDevice && at.device != c.device))
+      throw std::invalid_argument(std::string(who) +
+                                  ": a pointer is not the context's device's");
+  }
+}
+
 tmnn_logits output_logits(const tmnn_ctx &c, const float *out, uint32_t N,
                           float temperature) {
   return {out, c.nd.O, N, (uint32_t)c.nd.O, TMNN_DTYPE_F32, temperature};
@@ -1735,6 +1753,8 @@ void ctx_token_logprobs(tmnn_ctx &c, const float *pos, const void *tokens,
     throw std::invalid_argument("token_logprobs: null top_ids or top_logprobs");
   if (o.logprob && !tokens)
     throw std::invalid_argument("token_logprobs: logprob needs tokens");
+  check_home(c, "token_logprobs", flags,
+             {pos, tokens, o.logprob, o.entropy, o.top_ids, o.top_logprobs});
   CK(cudaSetDevice(c.device));
   ensure_batch(c, N);
   const float *p = stage_in(c, pos, (size_t)N * c.nd.d, c.pos_in, flags);
@@ -1786,6 +1806,7 @@ void distill_step(tmnn_ctx &c, const float *pos, const void *ids,
   const uint64_t global_n = (uint64_t)N * (uint64_t)c.world;
   if (loss) *loss = 0.0f;
   if (N == 0) return;
+  check_home(c, "distill_step", flags, {pos, ids, teacher});
   CK(cudaSetDevice(c.device));
   ensure_batch(c, N);
   const float *p = stage_in(c, pos, (size_t)N * c.nd.d, c.pos_in, flags);
