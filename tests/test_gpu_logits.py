@@ -439,6 +439,37 @@ def test_one_row_in_place():
         assert torch.equal(y, dist)
 
 
+def test_in_place_gradients_are_seen_by_autograd():
+    """A gradient written over a tensor that an autograd graph has saved makes
+    that graph's backward pass an error, as torch's own in-place calls do;
+    tensors without a version are written as well."""
+    import torch
+    import tmnn_b200 as t
+    w = torch.ones(4, 9, device="cuda", requires_grad=True)
+    ids = torch.ones(4, 2, dtype=torch.int64, device="cuda")
+    y = torch.zeros(4, 2, device="cuda")
+    tok = torch.zeros(4, dtype=torch.int64, device="cuda")
+    one = torch.ones(4, device="cuda")
+
+    def distil(x):
+        t.distill_forward_backward(x, ids, y, out=x)
+
+    def policy(x):
+        r = t.token_logprobs(x, tok, stats=True)
+        t.token_logprobs_backward(x, tok, r.stats, one, out=x)
+
+    for write in (distil, policy):
+        x = w * 2
+        z = (x * x).sum()  # saves x
+        write(x.detach())
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            z.backward()
+        with torch.inference_mode():
+            x = w * 2
+            write(x)
+            assert not torch.equal(x, w * 2)
+
+
 def test_empty_batches():
     import torch
     import tmnn_b200 as t

@@ -116,6 +116,13 @@ def _gradient(out, x):
     return out
 
 
+def _written(out):
+    """Tells autograd that a tensor of the caller's has new values, so that a
+    graph that saved the old ones refuses its backward pass."""
+    if not out.is_inference():  # those have no version
+        _torch.autograd.graph.increment_version(out)
+
+
 def _grad_stride(out):
     """Distance of the gradient's rows; of one row or none it is never used."""
     n, v = out.shape
@@ -176,11 +183,13 @@ def token_logprobs_backward(logits, tokens, stats, d_logprob=None,
                                                 (n,), _F32)[0]
     hp = None if d_entropy is None else _vector(d_entropy, "d_entropy", dev,
                                                 (n,), _F32)[0]
-    out = _gradient(out, logits)
+    given, out = out, _gradient(out, logits)
     index = dev.index
     _check(lib.tmnn_cuda_token_logprobs_backward(
         index, _raw_stream(index), x, tp, it, sp, gp, hp, out.data_ptr(),
         _grad_stride(out)))
+    if given is not None:
+        _written(out)
     return out
 
 
@@ -222,5 +231,8 @@ def distill_forward_backward(logits, teacher_ids, teacher_logits, *,
     row_weight float32 [n]; None is 1 / n, the gradient of the mean loss.  out:
     where to write the gradient; it may be `logits` itself."""
     x = _logits(logits, temperature)
-    out = _gradient(out, logits)
-    return _distill(x, logits, teacher_ids, teacher_logits, row_weight, out), out
+    given, out = out, _gradient(out, logits)
+    loss = _distill(x, logits, teacher_ids, teacher_logits, row_weight, out)
+    if given is not None:
+        _written(out)
+    return loss, out
