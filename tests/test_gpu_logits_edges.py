@@ -1,0 +1,46 @@
+"""Class-logit operators on the GPU at the edges of their number range and of
+what may be asked of them, in a size of every kernel (test_gpu_logits.py has
+the ordinary range and the tolerances' reference)."""
+import numpy as np
+import pytest
+
+import _logits_ref as ref
+import test_gpu_logits as base
+
+pytestmark = pytest.mark.gpu
+
+# rows of a thread, of some lanes, of a CTA, of a CTA for the loss and a cluster
+# for the gradient, of a cluster, of a cluster of 16
+KERNELS = [(40, 19), (33, 127), (30, 1000), (20, 9001), (170, 33000), (5, 131072),
+           (2, 300007)]
+
+
+@pytest.mark.parametrize("T", [0.5, 0.7, 1.0, 2.0])
+@pytest.mark.parametrize("n,V", KERNELS)
+def test_entries_of_classes_at_the_lowest_value(n, V, T):
+    """A teacher's entries that name classes masked with fp32's lowest value:
+    the loss is in range although the log probability, divided by T, is not."""
+    import torch
+    import tmnn_b200 as t
+    rng = np.random.default_rng(V)
+    K = 5
+    x = rng.normal(size=(n, V)).astype(np.float32) * 2
+    x[:, 3:9] = base.LOWEST["f32"]
+    ids = np.tile([0, 4, 1, 8, 5], (n, 1))
+    ids[0] = [0, 1, 2, 10, 11]  # none of them
+    y = rng.normal(size=(n, K)).astype(np.float32)
+    w = rng.uniform(0.5, 1.5, n).astype(np.float32)
+    loss, tl, d, td = ref.distill(x.astype(np.float64), T, ids, y, w)
+    # a share is at least e^(-13 / 0.5) / 5 > 1e-12
+    assert np.isfinite(loss).all() and (loss[1:] > 1e25).all()
+    # T times a difference of 3.4e38 may be out of fp32's range, which is
+    # infinity then; no loss is as near to its border as its bound
+    most = -base.LOWEST["f32"]
+    assert (np.abs(loss - most) > 2 * tl + 1e32).all() and (T > 1 or loss.max() < most)
+    loss[loss > most] = np.inf
+    args = [torch.from_numpy(a).cuda() for a in (x, ids, y)]
+    ref.assert_close(t.distill_loss(*args, temperature=T).cpu(), loss, tl, "loss")
+    l, g = t.distill_forward_backward(*args, temperature=T,
+                                      row_weight=torch.from_numpy(w).cuda())
+    ref.assert_close(l.cpu(), loss, tl, "loss with gradient")
+    ref.assert_close(g.double().cpu(), d, base._round(d, td, "f32"), "gradient")

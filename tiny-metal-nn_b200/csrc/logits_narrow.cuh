@@ -321,22 +321,26 @@ __global__ void __launch_bounds__(128) k_tiny(TinyArgs p) {
         }
       }
       if constexpr (kTeacher) {
-        // loss = sum q (log q - log p) = (sum e (y - log p)) / sum e
-        //        - log sum e  with e = e^y, y = (teacher - max) / T
+        // loss / T = sum q T (log q - log p) = (sum e T (y - log p)) / sum e
+        //            - T log sum e  with e = e^y, y = (teacher - max) / T;
+        // the sum is kept in units of 2^8 > K, so that it stays in range
         const float w = weight * a.t;
         const bool zero = idle || (end.empty && !end.bad);
         float ys = 0.0f, loss = 0.0f;
         for (int k = 0; k < K; ++k) {
-          const float y = (ey[k] - ym) * a.inv_t, e = eid[k] >= 0 ? expf(y) : 0.0f;
+          const float dy = ey[k] - ym;
+          const float e = eid[k] >= 0 ? expf(dy * a.inv_t) : 0.0f;
           ys += e;
           if (e > 0.0f)
-            loss += end.empty ? kInf : e * (y - end.logp(mine[eid[k]]));
+            loss += end.empty ? kInf
+                              : e * 0x1p-8f *
+                                    entry_gap(end, a.t, dy, 0.0f, mine[eid[k]]);
           if (MODE == kLossGrad) ey[k] = e;
         }
         const float inv_ys = 1.0f / ys;
         p.loss[row] = idle      ? 0.0f
                       : end.bad ? nan
-                                : a.t * a.t * (loss * inv_ys - logf(ys));
+                                : a.t * (loss * (0x1p8f * inv_ys) - a.t * logf(ys));
         if constexpr (MODE == kLossGrad) {
           const float ws = zero ? 0.0f : end.bad ? nan : w / end.s;
           const float2 w2 = f2(ws, ws);
@@ -515,7 +519,7 @@ __global__ void __launch_bounds__(128) k_narrow(NarrowArgs p) {
   // ---- the teacher's entries, entry l + lanes * i of a row by lane l
   const int K = kTeacher ? p.te.k : 0;
   float *sq = entries + (warp * (32 / L) + lane / L) * K * 3;  // e^(y - max)
-  float *sy = sq + K;                                          // y, then own d
+  float *sy = sq + K;                                          // y - max, then own d
   int32_t *sid = reinterpret_cast<int32_t *>(sy + K);
   float ym = 0.0f, ys = 1.0f;
   int64_t tok = 0;
@@ -537,9 +541,9 @@ __global__ void __launch_bounds__(128) k_narrow(NarrowArgs p) {
     idle = ym == -kInf;
     ys = 0.0f;
     for (int k = l; k < K; k += L) {
-      const float y = sid[k] >= 0 ? (sy[k] - ym) * a.inv_t : -kInf;
-      sy[k] = y;
-      sq[k] = expf(y);
+      const float dy = sid[k] >= 0 ? sy[k] - ym : -kInf;
+      sy[k] = dy;
+      sq[k] = expf(dy * a.inv_t);
       ys += sq[k];
     }
     ys = group_sum(ys);
@@ -724,7 +728,7 @@ __global__ void __launch_bounds__(128) k_narrow(NarrowArgs p) {
         const float xv = to_f(x[sid[k]]);
         if (e > 0.0f)
           loss += end.empty ? kInf
-                            : e / ys * ((sy[k] - ln_ys) - end.logp(xv));
+                            : e / ys * entry_gap(end, a.t, sy[k], ln_ys, xv);
         if constexpr (MODE == kLossGrad) {
           float both = 0.0f;  // entries of one class add up
           for (int j = 0; j < K; ++j) both += sid[j] == sid[k] ? sq[j] : 0.0f;
@@ -733,7 +737,7 @@ __global__ void __launch_bounds__(128) k_narrow(NarrowArgs p) {
       }
     loss = group_sum(loss);
     if (l == 0 && on)
-      p.loss[row] = idle ? 0.0f : end.bad ? nan : a.t * a.t * loss;
+      p.loss[row] = idle ? 0.0f : end.bad ? nan : a.t * loss;
     if constexpr (MODE == kLossGrad) {
       const bool zero = idle || (end.empty && !end.bad);
       const float ws = zero ? 0.0f : end.bad ? nan : w / end.s;

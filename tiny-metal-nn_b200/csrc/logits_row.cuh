@@ -298,6 +298,13 @@ struct RowEnd {
     return (x - m) * inv_t - ln_s;
   }
 };
+// T (log q - log p) of a teacher's entry: dy = its logit less the largest one,
+// x the logit of its class.  A loss is T times the mean of these; divided by T
+// first, differences near the lowest fp32 value would leave its range.
+__device__ __forceinline__ float entry_gap(const RowEnd &end, float t, float dy,
+                                           float ln_ys, float x) {
+  return (dy - t * ln_ys) - ((x - end.m) - t * end.ln_s);
+}
 __device__ __forceinline__ float not_a_number() {
   return __int_as_float(0x7FFFFFFF);
 }

@@ -180,8 +180,8 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         xk[i] = 0.0f;
-        ty[i] = tid_[i] >= 0 ? (ty[i] - ym) * a.inv_t : -kInf;
-        tq[i] = expf(ty[i]);
+        ty[i] = tid_[i] >= 0 ? ty[i] - ym : -kInf;
+        tq[i] = expf(ty[i] * a.inv_t);
         ys += tq[i];
         if (leader && tid_[i] >= 0) xk[i] = to_f((x - first)[tid_[i]]);
       }
@@ -426,9 +426,10 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (tq[i] > 0.0f)
-          l += empty ? kInf : tq[i] * ((ty[i] - ln_ys) - end.logp(xk[i]));
+          l += empty ? kInf
+                     : tq[i] * entry_gap(end, a.t, ty[i], ln_ys, xk[i]);
       for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
-      if (lane == 0) p.loss[row] = bad ? nan : a.t * a.t * l;
+      if (lane == 0) p.loss[row] = bad ? nan : a.t * l;
     }
   }
   if constexpr (MODE == kLossGrad) {
@@ -706,8 +707,8 @@ __global__ void __launch_bounds__(NT) k_stream(StreamArgs p) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const bool in = !(ty[i] == -kInf);
-      ty[i] = (ty[i] - ym) * a.inv_t;
-      tq[i] = in ? expf(ty[i]) : 0.0f;
+      ty[i] -= ym;
+      tq[i] = in ? expf(ty[i] * a.inv_t) : 0.0f;
       ys += tq[i];
     }
     for (int o = 16; o; o >>= 1) ys += __shfl_xor_sync(~0u, ys, o);
@@ -716,9 +717,9 @@ __global__ void __launch_bounds__(NT) k_stream(StreamArgs p) {
     for (int i = 0; i < 4; ++i)
       if (tq[i] > 0.0f)
         l += end.empty ? kInf
-                       : tq[i] / ys * ((ty[i] - ln_ys) - end.logp(xk[i]));
+                       : tq[i] / ys * entry_gap(end, a.t, ty[i], ln_ys, xk[i]);
     for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
-    if (lane == 0) p.loss[row] = end.bad ? nan : a.t * a.t * l;
+    if (lane == 0) p.loss[row] = end.bad ? nan : a.t * l;
     if constexpr (kGrad) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
