@@ -44,3 +44,32 @@ def test_entries_of_classes_at_the_lowest_value(n, V, T):
                                       row_weight=torch.from_numpy(w).cuda())
     ref.assert_close(l.cpu(), loss, tl, "loss with gradient")
     ref.assert_close(g.double().cpu(), d, base._round(d, td, "f32"), "gradient")
+
+
+@pytest.mark.parametrize("T", [1.0, 2.0])
+@pytest.mark.parametrize("n,V", KERNELS)
+def test_small_shares_of_masked_classes(n, V, T):
+    """A masked class (-inf) under an entry whose e^y is above fp32's zero makes
+    the loss infinite, also where the share of all entries rounds to zero;
+    one whose e^y is zero counts nothing.  Gradients are finite."""
+    import torch
+    import tmnn_b200 as t
+    torch.manual_seed(V)
+    x = torch.randn(n, V, device="cuda")
+    x[:, 5] = float("-inf")
+    ids = torch.tensor([[0, 1, 2, 5]], device="cuda").repeat(n, 1)
+    # the smallest number above zero is 2^-149: e^-103 is 1.3 of it, and a third
+    # of that rounds to none; e^-110 is none of it
+    for far, inf in ((-95.0, True), (-103.0, True), (-110.0, False)):
+        y = torch.tensor([[0.0, 0.0, 0.0, far * T]], device="cuda").repeat(n, 1)
+        loss = t.distill_loss(x, ids, y, temperature=T)
+        both, g = t.distill_forward_backward(x, ids, y, temperature=T)
+        assert not loss.isnan().any() and not both.isnan().any(), far
+        assert bool(loss.isinf().all()) == inf and bool(both.isinf().all()) == inf
+        assert g.isfinite().all()
+        if not inf:
+            want = t.distill_loss(x, ids[:, :3].contiguous(),
+                                  y[:, :3].contiguous(), temperature=T)
+            # the same shares and sums: three roundings of terms below 20 T
+            assert (loss - want).abs().max() <= 3 * 2 ** -24 * 20 * T * T
+            assert loss.isfinite().all()

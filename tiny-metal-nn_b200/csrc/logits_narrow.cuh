@@ -332,9 +332,8 @@ __global__ void __launch_bounds__(128) k_tiny(TinyArgs p) {
           const float e = eid[k] >= 0 ? expf(dy * a.inv_t) : 0.0f;
           ys += e;
           if (e > 0.0f)
-            loss += end.empty ? kInf
-                              : e * 0x1p-8f *
-                                    entry_gap(end, a.t, dy, 0.0f, mine[eid[k]]);
+            loss += entry_part(end, e * 0x1p-8f,
+                               entry_gap(end, a.t, dy, 0.0f, mine[eid[k]]));
           if (MODE == kLossGrad) ey[k] = e;
         }
         const float inv_ys = 1.0f / ys;
@@ -727,8 +726,7 @@ __global__ void __launch_bounds__(128) k_narrow(NarrowArgs p) {
         if (sid[k] < 0) continue;
         const float xv = to_f(x[sid[k]]);
         if (e > 0.0f)
-          loss += end.empty ? kInf
-                            : e / ys * entry_gap(end, a.t, sy[k], ln_ys, xv);
+          loss += entry_part(end, e / ys, entry_gap(end, a.t, sy[k], ln_ys, xv));
         if constexpr (MODE == kLossGrad) {
           float both = 0.0f;  // entries of one class add up
           for (int j = 0; j < K; ++j) both += sid[j] == sid[k] ? sq[j] : 0.0f;

@@ -305,6 +305,13 @@ __device__ __forceinline__ float entry_gap(const RowEnd &end, float t, float dy,
                                            float ln_ys, float x) {
   return (dy - t * ln_ys) - ((x - end.m) - t * end.ln_s);
 }
+// An entry's part of a row's loss, q times its gap.  A class at -inf under an
+// entry that counts (e^y > 0) makes the loss infinite, also where its share
+// q = e^y / sum rounds to 0 and the product would be NaN.
+__device__ __forceinline__ float entry_part(const RowEnd &end, float q,
+                                            float gap) {
+  return end.empty || gap == kInf ? kInf : q * gap;
+}
 __device__ __forceinline__ float not_a_number() {
   return __int_as_float(0x7FFFFFFF);
 }

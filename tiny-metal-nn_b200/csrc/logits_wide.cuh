@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
   int32_t *sid = reinterpret_cast<int32_t *>(sq + p.te.k);
   [[maybe_unused]] int32_t *bad_entries = sid + p.te.k;
   [[maybe_unused]] float ty[4], tq[4], ln_ys = 0.0f, ym = 0.0f;
-  [[maybe_unused]] int32_t tid_[4];
+  [[maybe_unused]] int32_t tid_[4], counts = 0;
   bool idle;
   if constexpr (kReads) {
     if (p.tokens) tok = load_index(p.tokens, row, p.itype);
@@ -183,6 +183,7 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
         ty[i] = tid_[i] >= 0 ? ty[i] - ym : -kInf;
         tq[i] = expf(ty[i] * a.inv_t);
         ys += tq[i];
+        counts |= (tq[i] > 0.0f) << i;
         if (leader && tid_[i] >= 0) xk[i] = to_f((x - first)[tid_[i]]);
       }
       for (int o = 16; o; o >>= 1) ys += __shfl_xor_sync(~0u, ys, o);
@@ -425,9 +426,8 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
       float l = 0.0f;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (tq[i] > 0.0f)
-          l += empty ? kInf
-                     : tq[i] * entry_gap(end, a.t, ty[i], ln_ys, xk[i]);
+        if (counts >> i & 1)
+          l += entry_part(end, tq[i], entry_gap(end, a.t, ty[i], ln_ys, xk[i]));
       for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
       if (lane == 0) p.loss[row] = bad ? nan : a.t * l;
     }
@@ -716,8 +716,7 @@ __global__ void __launch_bounds__(NT) k_stream(StreamArgs p) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (tq[i] > 0.0f)
-        l += end.empty ? kInf
-                       : tq[i] / ys * entry_gap(end, a.t, ty[i], ln_ys, xk[i]);
+        l += entry_part(end, tq[i] / ys, entry_gap(end, a.t, ty[i], ln_ys, xk[i]));
     for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
     if (lane == 0) p.loss[row] = end.bad ? nan : a.t * l;
     if constexpr (kGrad) {
