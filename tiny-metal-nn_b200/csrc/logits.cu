@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(256)
     if (b.idle) {
       for (int e = e0 + lane; e < e1; e += 32) d[e] = from_f<T>(0.0f);
     } else {
-      write_shifted<T>(d + e0, x + e0, e1 - e0, lane, 32,
+      write_shifted<T>(d + e0, x + e0, e1 - e0, lane, 32, e0 ? 0 : E,
                        e1 + E <= V ? 0 : E,
                        [&](const uint4 &q, int e, float *r) {
                          b.granule<T>(q, e0 + e, a.c, r);

@@ -433,7 +433,10 @@ __global__ void __launch_bounds__(128) k_narrow(NarrowArgs p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int L = p.lanes, l = lane & (L - 1), V = a.classes;
   const uint32_t want = (blockIdx.x * 4 + warp) * (32 / L) + lane / L;
-  const bool on = want < a.rows;  // lanes of no row repeat the last one
+  // A warp without a row ends here: the last one may be another warp's, which
+  // writes it in place.  Lanes of no row in a warp that has one repeat its last.
+  if ((blockIdx.x * 4 + warp) * (32 / L) >= a.rows) return;
+  const bool on = want < a.rows;
   const uint32_t row = on ? want : a.rows - 1;
   const float nan = not_a_number();
   auto group_max = [&](float v) {
@@ -511,6 +514,7 @@ __global__ void __launch_bounds__(128) k_narrow(NarrowArgs p) {
 
   if constexpr (MODE == kBack) {
     const BackRow b(a, p.tokens, p.itype, p.stats, p.d_logprob, p.d_entropy, row);
+    __syncwarp();  // every lane has read what the row's lanes now write
     write_rows([&](const uint4 &g, int e, float *r) { b.granule<T>(g, e, a.c, r); });
     return;
   }

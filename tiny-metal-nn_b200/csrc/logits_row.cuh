@@ -357,8 +357,9 @@ __device__ __forceinline__ void write_zeros(T *d, int n) {
 }
 
 // The granule that starts at any element: the two around it, shifted.  All of
-// its elements are the caller's; the second granule may end up to 16 bytes
-// behind them.
+// its elements are the caller's; the first granule begins up to 14 bytes before
+// them and the second one ends up to 14 bytes behind them, so a row's first
+// and last elements are not read this way.
 template <class T>
 __device__ __forceinline__ uint4 granule_at(const T *p) {
   const uint32_t at = (uint32_t)(uintptr_t)p & 15;
@@ -380,12 +381,12 @@ __device__ __forceinline__ uint4 granule_at(const T *p) {
 
 // The n elements of a row part x in memory as gradients to d, whose granules lie
 // otherwise than those of x: thread `tid` of `threads` takes granules of d, body(granule
-// of x, first element, its E results).  `slack`: how near to the end of x a
-// granule of it may not be read whole, E at a row's end and 0 where the row goes
-// on.
+// of x, first element, its E results).  `lead`, `slack`: how near to the start
+// and the end of x a granule of it may not be read whole, E at a row's start or
+// end and 0 where the row goes on.
 template <class T, class Body>
 __device__ __forceinline__ void write_shifted(T *d, const T *x, int n, int tid,
-                                              int threads, int slack,
+                                              int threads, int lead, int slack,
                                               Body &&body) {
   constexpr int E = kElems<T>;
   const int dm = (int)((uintptr_t)d & 15) / (int)sizeof(T);
@@ -396,13 +397,13 @@ __device__ __forceinline__ void write_shifted(T *d, const T *x, int n, int tid,
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int e = (g0 + i * threads) * E - dm;
-      if (e >= 0 && e + E + slack <= n) q[i] = granule_at(x + e);
+      if (e >= lead && e + E + slack <= n) q[i] = granule_at(x + e);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int g = g0 + i * threads, e = g * E - dm;
       float r[E];
-      if (e >= 0 && e + E + slack <= n) {
+      if (e >= lead && e + E + slack <= n) {
         body(q[i], e, r);
         dst[g] = pack_granule<T>(r);
       } else if (g < G) {  // the ends

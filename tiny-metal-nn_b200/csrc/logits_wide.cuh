@@ -753,7 +753,7 @@ __global__ void __launch_bounds__(NT) k_stream(StreamArgs p) {
         d[odd_class] = from_f<T>(ex2((odd - m0) * a.c) * ws);
     } else {
       // rows of another alignment
-      write_shifted<T>(d, x, V, tid, NT, E, [&](const uint4 &g, int, float *r) {
+      write_shifted<T>(d, x, V, tid, NT, E, E, [&](const uint4 &g, int, float *r) {
         softmax_granule<T>(g, nm, c2, w2, r);
       });
     }
