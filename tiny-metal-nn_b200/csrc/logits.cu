@@ -123,7 +123,7 @@ void check_opt(const char *who, const char *what, const void *p, size_t align) {
   if (p) check_ptr(who, what, p, align);
 }
 
-RowArgs check_logits(const char *who, const tmnn_logits &x) {
+void check_logits(const char *who, const tmnn_logits &x) {
   check_dtype(who, "logits", x.dtype);
   if (x.classes < 1 || x.classes > kMaxClasses)
     bad(std::string(who) + ": classes must be in [1, 524288]");
@@ -134,6 +134,9 @@ RowArgs check_logits(const char *who, const tmnn_logits &x) {
   if (x.rows > 1 && x.row_stride > ((int64_t)1 << 56) / (int64_t)x.rows)
     bad(std::string(who) + ": the rows span more than memory");
   if (x.rows) check_ptr(who, "logits", x.data, elem_size(x.dtype));
+}
+
+RowArgs row_args(const tmnn_logits &x) {
   RowArgs a;
   a.x = x.data;
   a.stride = x.row_stride;
@@ -421,17 +424,16 @@ const void *at(const void *p, int64_t bytes) {
 
 namespace tmnn {
 
-int launch_token_logprobs(const tmnn_logits &x, const void *tokens,
-                          int index_type, uint32_t top_k, const LogprobOut &o,
-                          cudaStream_t st) {
+void check_token_logprobs(const tmnn_logits &x, const void *tokens,
+                          int index_type, uint32_t top_k, const LogprobOut &o) {
   const char *who = "token_logprobs";
-  RowArgs a = check_logits(who, x);
+  check_logits(who, x);
   if (top_k > kMaxTop || top_k > x.classes)
     bad("token_logprobs: top_k must be at most min(classes, 128)");
   if (o.logprob && !tokens && x.rows)
     bad("token_logprobs: logprob needs tokens");
   if (tokens) check_index(who, index_type);
-  if (!x.rows) return 0;
+  if (!x.rows) return;
   check_opt(who, "tokens", tokens, index_size(index_type));
   check_opt(who, "logprob", o.logprob, 4);
   check_opt(who, "entropy", o.entropy, 4);
@@ -451,6 +453,13 @@ int launch_token_logprobs(const tmnn_logits &x, const void *tokens,
     check_apart(who, "an output", out[i], {in, toks});
     for (int j = 0; j < i; ++j) check_apart(who, "an output", out[i], {out[j]});
   }
+}
+
+int launch_token_logprobs(const tmnn_logits &x, const void *tokens,
+                          int index_type, uint32_t top_k, const LogprobOut &o,
+                          cudaStream_t st) {
+  check_token_logprobs(x, tokens, index_type, top_k, o);
+  const RowArgs a = row_args(x);
   return in_parts(x.rows, [&](uint32_t i, uint32_t n) {
     TeamArgs p{};
     p.a = a;
@@ -505,7 +514,8 @@ int launch_token_logprobs_backward(const tmnn_logits &x, const void *tokens,
                                    const float *d_entropy, void *d_logits,
                                    int64_t d_stride, cudaStream_t st) {
   const char *who = "token_logprobs_backward";
-  RowArgs a = check_logits(who, x);
+  check_logits(who, x);
+  const RowArgs a = row_args(x);
   if (d_logprob && !tokens && x.rows)
     bad("token_logprobs_backward: d_logprob needs tokens");
   if (tokens) check_index(who, index_type);
@@ -565,16 +575,16 @@ int launch_token_logprobs_backward(const tmnn_logits &x, const void *tokens,
   });
 }
 
-int launch_distill(const tmnn_logits &x, const void *ids, int index_type,
+void check_distill(const tmnn_logits &x, const void *ids, int index_type,
                    const void *teacher, int teacher_dtype, uint32_t k,
-                   const float *row_weight, float weight, float *loss,
-                   void *d_logits, int64_t d_stride, cudaStream_t st) {
+                   const float *row_weight, const float *loss,
+                   const void *d_logits, int64_t d_stride) {
   const char *who = "distill";
-  RowArgs a = check_logits(who, x);
+  check_logits(who, x);
   check_index(who, index_type);
   check_dtype(who, "teacher_logits", teacher_dtype);
   if (k < 1 || k > kMaxTop) bad("distill: k must be in [1, 128]");
-  if (!x.rows) return 0;
+  if (!x.rows) return;
   check_ptr(who, "teacher_ids", ids, index_size(index_type));
   check_ptr(who, "teacher_logits", teacher, elem_size(teacher_dtype));
   check_opt(who, "row_weight", row_weight, 4);
@@ -588,6 +598,15 @@ int launch_distill(const tmnn_logits &x, const void *ids, int index_type,
   if (d_logits)
     check_apart(who, "d_logits", check_grad(who, x, d_logits, d_stride),
                 {id_span, teacher_span, weights, losses});
+}
+
+int launch_distill(const tmnn_logits &x, const void *ids, int index_type,
+                   const void *teacher, int teacher_dtype, uint32_t k,
+                   const float *row_weight, float weight, float *loss,
+                   void *d_logits, int64_t d_stride, cudaStream_t st) {
+  check_distill(x, ids, index_type, teacher, teacher_dtype, k, row_weight, loss,
+                d_logits, d_stride);
+  const RowArgs a = row_args(x);
   const int size = elem_size(x.dtype);
   return in_parts(x.rows, [&](uint32_t i, uint32_t n) {
     TeamArgs p{};

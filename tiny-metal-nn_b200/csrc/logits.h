@@ -21,6 +21,15 @@ struct LogprobOut {
   float *stats;         // [n x 3]
 };
 
+// The checks of the calls below alone (std::invalid_argument), for callers that
+// queue other work before.
+void check_token_logprobs(const tmnn_logits &x, const void *tokens,
+                          int index_type, uint32_t top_k, const LogprobOut &o);
+void check_distill(const tmnn_logits &x, const void *ids, int index_type,
+                   const void *teacher, int teacher_dtype, uint32_t k,
+                   const float *row_weight, const float *loss,
+                   const void *d_logits, int64_t d_stride);
+
 // Each checks its arguments (std::invalid_argument) and queues its kernel on
 // `st`, which belongs to the current device.  Nothing is allocated and the
 // host does not wait, so the calls can be captured.  They return the number

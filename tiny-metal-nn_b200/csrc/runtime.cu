@@ -1735,6 +1735,16 @@ void check_home(const tmnn_ctx &c, const char *who, uint32_t flags,
   }
 }
 
+// Waits for the stream when a call ends by an exception: its kernels and copies
+// may still read the caller's memory.
+struct WaitOnError {
+  cudaStream_t stream;
+  bool on = true;
+  ~WaitOnError() {
+    if (on) cudaStreamSynchronize(stream);
+  }
+};
+
 tmnn_logits output_logits(const tmnn_ctx &c, const float *out, uint32_t N,
                           float temperature) {
   return {out, c.nd.O, N, (uint32_t)c.nd.O, TMNN_DTYPE_F32, temperature};
@@ -1745,9 +1755,8 @@ void ctx_token_logprobs(tmnn_ctx &c, const float *pos, const void *tokens,
                         float temperature, uint32_t flags, LogprobOut o) {
   if (N > 0 && !pos)
     throw std::invalid_argument("token_logprobs: null positions");
-  // the arguments' checks, before anything is queued
-  launch_token_logprobs(output_logits(c, nullptr, 0, temperature), tokens,
-                        index_type, top_k, o, c.stream);
+  check_token_logprobs(output_logits(c, nullptr, 0, temperature), tokens,
+                       index_type, top_k, o);
   if (N == 0) return;
   if (top_k && (!o.top_ids || !o.top_logprobs))
     throw std::invalid_argument("token_logprobs: null top_ids or top_logprobs");
@@ -1757,10 +1766,14 @@ void ctx_token_logprobs(tmnn_ctx &c, const float *pos, const void *tokens,
              {pos, tokens, o.logprob, o.entropy, o.top_ids, o.top_logprobs});
   CK(cudaSetDevice(c.device));
   ensure_batch(c, N);
+  const bool dev = flags & TMNN_PTR_DEVICE;
+  if (dev)  // the kernel's own checks, before anything is queued
+    check_token_logprobs(output_logits(c, c.out_buf.p, N, temperature), tokens,
+                         index_type, top_k, o);
+  WaitOnError wait{c.stream};
   const float *p = stage_in(c, pos, (size_t)N * c.nd.d, c.pos_in, flags);
   forward_dev(c, p, c.out_buf.p, N);
   const void *ids = stage_ids(c, tokens, index_type, N, flags);
-  const bool dev = flags & TMNN_PTR_DEVICE;
   LogprobOut d = o;
   if (!dev) {
     // [logprob | entropy | top_logprobs | top_ids] of the batch
@@ -1785,6 +1798,7 @@ void ctx_token_logprobs(tmnn_ctx &c, const float *pos, const void *tokens,
                reinterpret_cast<float *>(d.top_ids), (size_t)N * top_k, flags);
     }
   }
+  wait.on = false;
   CK(cudaStreamSynchronize(c.stream));
   CK(cudaGetLastError());
 }
@@ -1800,21 +1814,25 @@ void distill_step(tmnn_ctx &c, const float *pos, const void *ids,
   if (c.n_pending)
     throw std::invalid_argument(
         "distill_step: enqueued steps are pending; finalize them first");
-  launch_distill(output_logits(c, nullptr, 0, temperature), ids, index_type,
-                 teacher, TMNN_DTYPE_F32, k, nullptr, 0.0f, nullptr, nullptr, 0,
-                 c.stream);
+  check_distill(output_logits(c, nullptr, 0, temperature), ids, index_type,
+                teacher, TMNN_DTYPE_F32, k, nullptr, nullptr, nullptr, 0);
   const uint64_t global_n = (uint64_t)N * (uint64_t)c.world;
   if (loss) *loss = 0.0f;
   if (N == 0) return;
   check_home(c, "distill_step", flags, {pos, ids, teacher});
   CK(cudaSetDevice(c.device));
   ensure_batch(c, N);
-  const float *p = stage_in(c, pos, (size_t)N * c.nd.d, c.pos_in, flags);
-  const void *id = stage_ids(c, ids, index_type, (size_t)N * k, flags);
   const bool dev = flags & TMNN_PTR_DEVICE;
   c.cls_rows.ensure((size_t)N * (1 + (dev ? 0 : (size_t)k)));
   c.cls_sum.ensure(1);
   float *row_loss = c.cls_rows.p;
+  if (dev)  // the kernel's own checks, before anything is queued
+    check_distill(output_logits(c, c.out_buf.p, N, temperature), ids, index_type,
+                  teacher, TMNN_DTYPE_F32, k, nullptr, row_loss, c.out_buf.p,
+                  c.nd.O);
+  WaitOnError wait{c.stream};
+  const float *p = stage_in(c, pos, (size_t)N * c.nd.d, c.pos_in, flags);
+  const void *id = stage_ids(c, ids, index_type, (size_t)N * k, flags);
   const float *t = teacher;
   if (!dev) {
     float *staged = row_loss + N;
@@ -1845,6 +1863,7 @@ void distill_step(tmnn_ctx &c, const float *pos, const void *ids,
   double sum = 0.0;
   CK(cudaMemcpyAsync(&sum, c.cls_sum.p, sizeof sum, cudaMemcpyDeviceToHost,
                      c.stream));
+  wait.on = false;
   CK(cudaStreamSynchronize(c.stream));
   CK(cudaGetLastError());
   if (loss) *loss = (float)(sum / (double)global_n);
