@@ -614,14 +614,21 @@ tmnn_status tmnn_cuda_ctx_token_logprobs(
 /* One training step of the distillation loss, averaged over the n points
  * (over all ranks' points under data parallelism, equal n on every rank):
  * forward, loss with its gradient, backward, Adam with gradient reset.  *loss
- * = the mean loss.  Like tmnn_cuda_adam_step it runs without the numerics
- * guard.  teacher_logits are float32. */
+ * = the mean loss.  It runs under the numerics guard like
+ * tmnn_cuda_train_step: a row that is NaN (an id >= num_outputs, a NaN or
+ * +inf among its entries) is an anomaly of the step, and bad_step_recovery
+ * says whether the update is applied all the same (SignalOnly, the default:
+ * the weights become NaN), vetoed, or the call fails.  No points: no step,
+ * *loss 0.  teacher_logits are float32. */
 tmnn_status tmnn_cuda_distill_step(tmnn_ctx *ctx, const float *positions,
                                    const void *teacher_ids,
                                    int32_t index_type,
                                    const float *teacher_logits, uint32_t n,
                                    uint32_t k, float temperature,
                                    uint32_t flags, float *loss);
+/* What the numerics guard made of the last distill_step that returned
+ * TMNN_OK (all zero before the first). */
+tmnn_status tmnn_cuda_distill_result(tmnn_ctx *ctx, tmnn_step_result *result);
 
 /* Message of the last failure on this thread ("" if none). */
 const char *tmnn_cuda_last_error(void);

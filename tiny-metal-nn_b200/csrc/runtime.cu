@@ -163,10 +163,10 @@ struct tmnn_ctx {
   DevBuf<__half> feat;   // Tiled family: encoded features [N x In]
   DevBuf<float> dfeat;   // Tiled family: dL/d(features) [N x In]
   // class-logit calls: ids and float rows (teacher entries, results) of a
-  // batch, and the summed loss
+  // batch
   DevBuf<uint8_t> cls_ids;
   DevBuf<float> cls_rows;
-  DevBuf<double> cls_sum;
+  tmnn_step_result last_step{};  // of the last distill_step
   StepStats *h_stats = nullptr;  // pinned copy of the step statistics
   double *h_loss = nullptr;      // &h_stats->loss
   // numerics guard
@@ -1428,14 +1428,107 @@ std::string describe(const StepReport &r) {
          ", max_abs_update=" + std::to_string(r.max_u);
 }
 
-// The step driver with the numerics guard (finalize_training_step,
+// What the numerics guard made of a step.
+struct GuardedStep {
+  StepReport rep;
+  uint32_t step = 0;
+  bool anomaly = false, reported = false;
+  int action = TMNN_RECOVERY_NONE;
+};
+
+// A step under the numerics guard (finalize_training_step,
 // training_step_execution.cpp:1080-1235): the probe is forced on sampled
 // steps and on every step of a recovery mode; in a recovery mode an anomaly
 // vetoes the update on the device (the gradients are still cleared), and
 // the host then throws (Throw), reports Skipped / RolledBack, or switches
 // to the SafeDebug family and re-runs the step (FallbackAndRetry).  The
 // step counter advances as in the reference (default_trainer.cpp:1032),
-// except when an error is thrown.
+// except when an error is thrown.  run(force, gate) is one whole step with the
+// context's family, whose statistics it leaves in c.h_stats.
+template <class Run>
+GuardedStep guarded_step(tmnn_ctx &c, const char *who, uint64_t global_n,
+                         Run &&run) {
+  const std::string name = std::string(who) + ": ";
+  GuardedStep s;
+  const uint32_t done = s.step = c.step;
+  const int mode = c.cfg.bad_step_recovery;
+  const bool gate = mode != TMNN_BAD_STEP_SIGNAL_ONLY;
+  const bool force = gate || c.guard.should_sample(done, false);
+  run(force, gate);
+  s.rep = read_report(*c.h_stats, global_n);
+  s.anomaly = s.rep.anomaly();
+  s.reported = c.guard.should_sample(done, s.anomaly);
+  if (s.reported) c.guard.record(done, s.anomaly);
+  if (!s.anomaly || !gate) return s;
+  if (mode == TMNN_BAD_STEP_THROW) {
+    c.step = done;
+    throw OperationFailed(name + "numerics anomaly detected at step " +
+                          std::to_string(done) + " (" + describe(s.rep) + ")");
+  }
+  if (mode == TMNN_BAD_STEP_SKIP) {
+    s.action = TMNN_RECOVERY_SKIPPED;
+    ++c.n_skipped;
+    return s;
+  }
+  if (mode == TMNN_BAD_STEP_ROLLBACK) {
+    s.action = TMNN_RECOVERY_ROLLED_BACK;
+    ++c.n_rolled_back;
+    return s;
+  }
+  if (c.safe_family_active || c.family == TMNN_FAMILY_SAFE_DEBUG) {
+    c.step = done;
+    throw OperationFailed(name +
+                          "numerics anomaly persisted while SafeDebug is "
+                          "already active at step " +
+                          std::to_string(done) + " (" + describe(s.rep) + ")");
+  }
+  activate_safe_family(c);
+  c.step = done;  // the vetoed update is re-done with the same step
+  // Under the sharded optimizer the fp32 master outside this rank's
+  // shard is out of date (only the fp16 gather copy was all-gathered),
+  // and the SafeDebug kernels read the fp32 master: gather it first.
+  // Every rank reaches this point together (the anomaly decision is
+  // combined over the ranks), so the collective is matched.
+  if (c.stale) dp_sync_state(c);
+  run(true, true);
+  s.rep = read_report(*c.h_stats, global_n);
+  s.anomaly = s.rep.anomaly();
+  c.guard.record(done, s.anomaly);
+  s.reported = true;
+  if (s.anomaly) {
+    c.step = done;
+    throw OperationFailed(name +
+                          "SafeDebug retry still produced a numerics anomaly "
+                          "at step " +
+                          std::to_string(done) + " (" + describe(s.rep) + ")");
+  }
+  s.action = TMNN_RECOVERY_RETRIED_WITH_SAFE_FAMILY;
+  ++c.n_safe_recoveries;
+  return s;
+}
+
+// The result of a guarded step, without the profile's times.
+void fill_result(const tmnn_ctx &c, const GuardedStep &s, uint32_t N,
+                 tmnn_step_result *res) {
+  std::memset(res, 0, sizeof *res);
+  res->loss = s.rep.mean_loss;
+  res->step = s.step;
+  res->batch_size = N;
+  res->numerics_ok = s.anomaly ? 0 : 1;
+  res->family = c.family;
+  res->grad_norm = s.rep.grad_norm;
+  res->finite_forward = s.rep.ff;
+  res->finite_backward = s.rep.fb;
+  res->finite_update = s.rep.fu;
+  res->max_abs_gradient = s.rep.max_g;
+  res->max_abs_update = s.rep.max_u;
+  res->numerics_probed = s.rep.probed;
+  res->numerics_reported = s.reported;
+  res->has_numerics_anomaly = s.anomaly;
+  res->recovery_action = s.action;
+}
+
+// The step driver.
 void train_step(tmnn_ctx &c, const float *pos, const float *tgt, uint32_t N,
                 uint32_t flags, tmnn_step_result *res) {
   if (N > 0 && (!pos || !tgt))
@@ -1452,75 +1545,12 @@ void train_step(tmnn_ctx &c, const float *pos, const float *tgt, uint32_t N,
   if (c.cfg.morton_sort && N > 1) morton_sort(c, p, t, N, &p, &t);
   const uint64_t global_n = (uint64_t)N * (uint64_t)c.world;
   const float inv_N = global_n ? 1.0f / (float)global_n : 0.0f;
-  const uint32_t done = c.step;
-  const int mode = c.cfg.bad_step_recovery;
-  const bool gate = mode != TMNN_BAD_STEP_SIGNAL_ONLY;
-  const bool force = gate || c.guard.should_sample(done, false);
-  run_step(c, p, t, N, inv_N, prof, force, gate);
-  StepReport rep = read_report(*c.h_stats, global_n);
-  bool anomaly = rep.anomaly();
-  bool reported = c.guard.should_sample(done, anomaly);
-  if (reported) c.guard.record(done, anomaly);
-  int action = TMNN_RECOVERY_NONE;
-  if (anomaly && gate) {
-    if (mode == TMNN_BAD_STEP_THROW) {
-      c.step = done;
-      throw OperationFailed("training_step: numerics anomaly detected at step " +
-                            std::to_string(done) + " (" + describe(rep) + ")");
-    } else if (mode == TMNN_BAD_STEP_SKIP) {
-      action = TMNN_RECOVERY_SKIPPED;
-      ++c.n_skipped;
-    } else if (mode == TMNN_BAD_STEP_ROLLBACK) {
-      action = TMNN_RECOVERY_ROLLED_BACK;
-      ++c.n_rolled_back;
-    } else {
-      if (c.safe_family_active || c.family == TMNN_FAMILY_SAFE_DEBUG) {
-        c.step = done;
-        throw OperationFailed(
-            "training_step: numerics anomaly persisted while SafeDebug is "
-            "already active at step " + std::to_string(done) + " (" +
-            describe(rep) + ")");
-      }
-      activate_safe_family(c);
-      c.step = done;  // the vetoed update is re-done with the same step
-      // Under the sharded optimizer the fp32 master outside this rank's
-      // shard is out of date (only the fp16 gather copy was all-gathered),
-      // and the SafeDebug kernels read the fp32 master: gather it first.
-      // Every rank reaches this point together (the anomaly decision is
-      // combined over the ranks), so the collective is matched.
-      if (c.stale) dp_sync_state(c);
-      run_step(c, p, t, N, inv_N, prof, true, true);
-      rep = read_report(*c.h_stats, global_n);
-      anomaly = rep.anomaly();
-      c.guard.record(done, anomaly);
-      reported = true;
-      if (anomaly) {
-        c.step = done;
-        throw OperationFailed(
-            "training_step: SafeDebug retry still produced a numerics anomaly "
-            "at step " + std::to_string(done) + " (" + describe(rep) + ")");
-      }
-      action = TMNN_RECOVERY_RETRIED_WITH_SAFE_FAMILY;
-      ++c.n_safe_recoveries;
-    }
-  }
+  const GuardedStep step =
+      guarded_step(c, "training_step", global_n, [&](bool force, bool gate) {
+        run_step(c, p, t, N, inv_N, prof, force, gate);
+      });
   if (res) {
-    std::memset(res, 0, sizeof *res);
-    res->loss = rep.mean_loss;
-    res->step = done;
-    res->batch_size = N;
-    res->numerics_ok = anomaly ? 0 : 1;
-    res->family = c.family;
-    res->grad_norm = rep.grad_norm;
-    res->finite_forward = rep.ff;
-    res->finite_backward = rep.fb;
-    res->finite_update = rep.fu;
-    res->max_abs_gradient = rep.max_g;
-    res->max_abs_update = rep.max_u;
-    res->numerics_probed = rep.probed;
-    res->numerics_reported = reported;
-    res->has_numerics_anomaly = anomaly;
-    res->recovery_action = action;
+    fill_result(c, step, N, res);
     if (prof) {
       CK(cudaEventElapsedTime(&res->gpu_ms, c.ev[0], c.ev[5]));
       CK(cudaEventElapsedTime(&res->sort_ms, c.ev[0], c.ev[1]));
@@ -1610,24 +1640,7 @@ void train_step_finalize(tmnn_ctx &c, tmnn_step_result *res) {
   const bool anomaly = rep.anomaly();
   const bool reported = c.guard.should_sample(L.step, anomaly);
   if (reported) c.guard.record(L.step, anomaly);
-  if (res) {
-    std::memset(res, 0, sizeof *res);
-    res->loss = rep.mean_loss;
-    res->step = L.step;
-    res->batch_size = L.N;
-    res->numerics_ok = anomaly ? 0 : 1;
-    res->family = c.family;
-    res->grad_norm = rep.grad_norm;
-    res->finite_forward = rep.ff;
-    res->finite_backward = rep.fb;
-    res->finite_update = rep.fu;
-    res->max_abs_gradient = rep.max_g;
-    res->max_abs_update = rep.max_u;
-    res->numerics_probed = rep.probed;
-    res->numerics_reported = reported;
-    res->has_numerics_anomaly = anomaly;
-    res->recovery_action = TMNN_RECOVERY_NONE;
-  }
+  if (res) fill_result(c, {rep, L.step, anomaly, reported, TMNN_RECOVERY_NONE}, L.N, res);
 }
 
 void copy_out(tmnn_ctx &c, float *dst, const float *src, size_t count,
@@ -1805,7 +1818,8 @@ void ctx_token_logprobs(tmnn_ctx &c, const float *pos, const void *tokens,
 
 // One step of the distillation loss: forward, loss and its gradient, backward
 // of that gradient, Adam -- the split API (forward_for_training ->
-// backward_accumulate -> adam_step) on one stream with one wait at the end.
+// backward_accumulate -> adam_step) on one stream with one wait at the end,
+// under the numerics guard like training_step.
 void distill_step(tmnn_ctx &c, const float *pos, const void *ids,
                   int index_type, const float *teacher, uint32_t N, uint32_t k,
                   float temperature, uint32_t flags, float *loss) {
@@ -1824,7 +1838,6 @@ void distill_step(tmnn_ctx &c, const float *pos, const void *ids,
   ensure_batch(c, N);
   const bool dev = flags & TMNN_PTR_DEVICE;
   c.cls_rows.ensure((size_t)N * (1 + (dev ? 0 : (size_t)k)));
-  c.cls_sum.ensure(1);
   float *row_loss = c.cls_rows.p;
   if (dev)  // the kernel's own checks, before anything is queued
     check_distill(output_logits(c, c.out_buf.p, N, temperature), ids, index_type,
@@ -1840,33 +1853,39 @@ void distill_step(tmnn_ctx &c, const float *pos, const void *ids,
                        cudaMemcpyHostToDevice, c.stream));
     t = staged;
   }
-  forward_dev(c, p, c.out_buf.p, N);
-  // the gradient takes the place of the logits
-  c.launches += launch_distill(output_logits(c, c.out_buf.p, N, temperature),
-                               id, index_type, t, TMNN_DTYPE_F32, k, nullptr,
-                               1.0f / (float)global_n, row_loss, c.out_buf.p,
-                               c.nd.O, c.stream);
-  launch_row_sum(row_loss, N, c.cls_sum.p, c.stream);
-  c.launches++;
-  const float *g = c.out_buf.p;
-  if (c.cfg.morton_sort && N > 1) morton_sort(c, p, g, N, &p, &g);
-  fwd_bwd(c, p, nullptr, g, N, 0.0f);
-  if (c.comm && c.world > 1)
-    NK(ncclAllReduce(c.cls_sum.p, c.cls_sum.p, 1, ncclFloat64, ncclSum, c.comm,
-                     c.stream));
-  if (can_shard(c)) {
-    dp_update(c, false, nullptr);
-  } else {
-    allreduce_grads(c, false);
-    adam(c);
-  }
-  double sum = 0.0;
-  CK(cudaMemcpyAsync(&sum, c.cls_sum.p, sizeof sum, cudaMemcpyDeviceToHost,
-                     c.stream));
+  const GuardedStep step =
+      guarded_step(c, "distill_step", global_n, [&](bool force, bool gate) {
+        ensure_batch(c, N);  // of the family that the guard may have changed
+        CK(cudaMemsetAsync(c.loss_acc.p, 0, sizeof(StepStats), c.stream));
+        forward_dev(c, p, c.out_buf.p, N);
+        // the gradient takes the place of the logits
+        c.launches += launch_distill(
+            output_logits(c, c.out_buf.p, N, temperature), id, index_type, t,
+            TMNN_DTYPE_F32, k, nullptr, 1.0f / (float)global_n, row_loss,
+            c.out_buf.p, c.nd.O, c.stream);
+        const float *q = p, *g = c.out_buf.p;
+        if (c.cfg.morton_sort && N > 1) morton_sort(c, q, g, N, &q, &g);
+        fwd_bwd(c, q, nullptr, g, N, 0.0f);
+        // the step's loss, in its statistics; the backward pass adds none
+        launch_row_sum(row_loss, N, &c.stats()->loss, c.stream);
+        c.launches++;
+        if (can_shard(c)) {
+          dp_update(c, true, nullptr, force, gate);
+        } else {
+          allreduce_grads(c, true);
+          probe_numerics(c, force, gate);
+          adam(c, c.stats());
+        }
+        CK(cudaMemcpyAsync(c.h_stats, c.loss_acc.p, sizeof(StepStats),
+                           cudaMemcpyDeviceToHost, c.stream));
+        CK(cudaStreamSynchronize(c.stream));
+        CK(cudaGetLastError());
+      });
   wait.on = false;
-  CK(cudaStreamSynchronize(c.stream));
-  CK(cudaGetLastError());
-  if (loss) *loss = (float)(sum / (double)global_n);
+  fill_result(c, step, N, &c.last_step);
+  const float mean = (float)(c.h_stats->loss / (double)global_n);
+  c.last_step.loss = mean;
+  if (loss) *loss = mean;
 }
 
 }  // namespace
@@ -2281,6 +2300,14 @@ tmnn_status tmnn_cuda_distill_step(tmnn_ctx *c, const float *positions,
     BusyGuard g(c);
     distill_step(*c, positions, teacher_ids, index_type, teacher_logits, n, k,
                  temperature, flags, loss);
+  });
+}
+
+tmnn_status tmnn_cuda_distill_result(tmnn_ctx *c, tmnn_step_result *result) {
+  REQUIRE_CTX(c);
+  return guarded([&] {
+    if (!result) throw std::invalid_argument("distill_result: null result");
+    *result = c->last_step;
   });
 }
 

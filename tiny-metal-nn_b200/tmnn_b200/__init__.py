@@ -414,8 +414,8 @@ class Trainer:
         return res.loss
 
     def last_numerics(self):
-        """NumericsReport of the last training step (dict), with the
-        recovery action the guard took."""
+        """NumericsReport of the last training_step or distill_step (dict),
+        with the recovery action the guard took."""
         r = self.last_result
         if r is None:
             return None
@@ -620,7 +620,13 @@ class Trainer:
         returns the mean loss.  teacher_ids [batch, k] (int32 or int64, below
         0: no entry) and float32 teacher_logits [batch, k] are a teacher's top
         classes of each point, e.g. what token_logprobs(top_k=k) returns.
-        Host arrays or CUDA tensors, all alike."""
+        Host arrays or CUDA tensors, all alike.
+
+        The numerics guard takes part as in training_step: a point with an id
+        at or above n_output, or a NaN or +inf logit, makes the loss NaN and
+        the step an anomaly, which bad_step_recovery deals with (SignalOnly,
+        the default, applies the update: the weights become NaN), and
+        last_numerics() reports it."""
         h = self._handle()
         pp, n, flags, _k = _arg(input, "input", self.n_input)
         if len(teacher_ids.shape) != 2:
@@ -635,10 +641,17 @@ class Trainer:
                              "placement")
         if flags & _abi.PTR_DEVICE:
             self._after_current_stream(input)
-        loss = C.c_float()
-        self._guarded(lambda: _check(lib.tmnn_cuda_distill_step(
-            h, pp, ip, it, yp, n, k, temperature, flags, C.byref(loss)),
-            "distill_step"))
+        loss, res = C.c_float(), _abi.StepResult()
+
+        def step():
+            _check(lib.tmnn_cuda_distill_step(
+                h, pp, ip, it, yp, n, k, temperature, flags, C.byref(loss)),
+                "distill_step")
+            if n:
+                _check(lib.tmnn_cuda_distill_result(h, C.byref(res)),
+                       "distill_step")
+                self.last_result = res
+        self._guarded(step)
         return loss.value
 
     def debug_morton_order(self, input, key_bits=0):

@@ -196,6 +196,7 @@ _SIGS = [
      [P, P, P, C.c_int32, u32, u32, C.c_float, u32, P, P, P, P]),
     ("tmnn_cuda_distill_step", C.c_int,
      [P, P, P, C.c_int32, P, u32, u32, C.c_float, u32, C.POINTER(C.c_float)]),
+    ("tmnn_cuda_distill_result", C.c_int, [P, C.POINTER(StepResult)]),
     ("tmnn_cuda_last_error", C.c_char_p, []),
     ("tmnn_cuda_launch_count", C.c_int, [P, C.POINTER(C.c_uint64)]),
 ]
