@@ -73,3 +73,41 @@ def test_small_shares_of_masked_classes(n, V, T):
             # the same shares and sums: three roundings of terms below 20 T
             assert (loss - want).abs().max() <= 3 * 2 ** -24 * 20 * T * T
             assert loss.isfinite().all()
+
+
+def test_leaves_that_require_a_gradient_are_not_written():
+    """out= a leaf that requires a gradient, or a view of one, is refused where
+    torch's own in-place calls refuse it, and written where they write."""
+    import torch
+    import tmnn_b200 as t
+    tok = torch.zeros(4, dtype=torch.int64, device="cuda")
+    one = torch.ones(4, device="cuda")
+    ids = torch.ones(4, 2, dtype=torch.int64, device="cuda")
+    y = torch.zeros(4, 2, device="cuda")
+
+    def distil(x, out):
+        return t.distill_forward_backward(x, ids, y, out=out)[1]
+
+    def policy(x, out):
+        st = t.token_logprobs(x, tok, stats=True).stats
+        return t.token_logprobs_backward(x, tok, st, one, out=out)
+
+    for write in (distil, policy):
+        values = torch.randn(4, 9, device="cuda")
+        want = write(values, None)
+        leaf = values.clone().requires_grad_()
+        wide = torch.zeros(4, 12, device="cuda", requires_grad=True)
+        for out in (leaf, wide[:, :9]):
+            before, version = out.detach().clone(), out._version
+            with pytest.raises(ValueError, match="leaf"):
+                write(values, out)
+            with pytest.raises(RuntimeError):
+                out.zero_()  # as torch does
+            assert torch.equal(out.detach(), before) and out._version == version
+        assert torch.equal(write(values, leaf.detach()), want)
+        leaf = values.clone().requires_grad_()
+        with torch.no_grad():
+            assert torch.equal(write(leaf, leaf), want)
+        leaf = values.clone().requires_grad_()
+        made = leaf * 1  # no leaf: in place as before
+        assert torch.equal(write(made, made).detach(), want)

@@ -113,6 +113,10 @@ def _gradient(out, x):
         raise _dtype_error(f"out must have the logits' type {x.dtype}")
     if out.shape[1] > 1 and out.stride(1) != 1:
         raise ValueError("the classes of a row of out must be contiguous")
+    if out.requires_grad and _torch.is_grad_enabled() and (
+            out.is_leaf or (out._is_view() and out._base.is_leaf)):
+        raise ValueError("out is a leaf that requires a gradient, or a view of "
+                         "one: pass out.detach(), or call under torch.no_grad()")
     return out
 
 
