@@ -323,23 +323,28 @@ __global__ void __launch_bounds__(128) k_tiny(TinyArgs p) {
       if constexpr (kTeacher) {
         // loss / T = sum q T (log q - log p) = (sum e T (y - log p)) / sum e
         //            - T log sum e  with e = e^y, y = (teacher - max) / T;
-        // the sum is kept in units of 2^8 > K, so that it stays in range
+        // the sum is kept in units of 2^8 > K, so that it stays in range.  A
+        // class at -inf under an e > 0 makes it infinite; in a row without a
+        // distribution (all at -inf) the terms are no numbers.
         const float w = weight * a.t;
         const bool zero = idle || (end.empty && !end.bad);
         float ys = 0.0f, loss = 0.0f;
+        // (not unrolled: 262144 rows of 19 classes with 4 entries take 13.8 us,
+        // 15.0 as the compiler unrolls it)
+#pragma unroll 1
         for (int k = 0; k < K; ++k) {
           const float dy = ey[k] - ym;
           const float e = eid[k] >= 0 ? expf(dy * a.inv_t) : 0.0f;
           ys += e;
           if (e > 0.0f)
-            loss += entry_part(end, e * 0x1p-8f,
-                               entry_gap(end, a.t, dy, 0.0f, mine[eid[k]]));
+            loss += e * (0x1p-8f * entry_gap(end, a.t, dy, mine[eid[k]]));
           if (MODE == kLossGrad) ey[k] = e;
         }
         const float inv_ys = 1.0f / ys;
-        p.loss[row] = idle      ? 0.0f
-                      : end.bad ? nan
-                                : a.t * (loss * (0x1p8f * inv_ys) - a.t * logf(ys));
+        p.loss[row] = idle        ? 0.0f
+                      : end.bad   ? nan
+                      : end.empty ? kInf
+                                  : a.t * (loss * (0x1p8f * inv_ys) - a.t * logf(ys));
         if constexpr (MODE == kLossGrad) {
           const float ws = zero ? 0.0f : end.bad ? nan : w / end.s;
           const float2 w2 = f2(ws, ws);
@@ -730,7 +735,8 @@ __global__ void __launch_bounds__(128) k_narrow(NarrowArgs p) {
         if (sid[k] < 0) continue;
         const float xv = to_f(x[sid[k]]);
         if (e > 0.0f)
-          loss += entry_part(end, e / ys, entry_gap(end, a.t, sy[k], ln_ys, xv));
+          loss += entry_part(end, e / ys,
+                             entry_gap(end, a.t, sy[k] - a.t * ln_ys, xv));
         if constexpr (MODE == kLossGrad) {
           float both = 0.0f;  // entries of one class add up
           for (int j = 0; j < K; ++j) both += sid[j] == sid[k] ? sq[j] : 0.0f;

@@ -298,12 +298,12 @@ struct RowEnd {
     return (x - m) * inv_t - ln_s;
   }
 };
-// T (log q - log p) of a teacher's entry: dy = its logit less the largest one,
-// x the logit of its class.  A loss is T times the mean of these; divided by T
-// first, differences near the lowest fp32 value would leave its range.
-__device__ __forceinline__ float entry_gap(const RowEnd &end, float t, float dy,
-                                           float ln_ys, float x) {
-  return (dy - t * ln_ys) - ((x - end.m) - t * end.ln_s);
+// T (log q - log p) of a teacher's entry: t_lq = T log q, x the logit of its
+// class.  A loss is T times the mean of these; divided by T first, differences
+// near the lowest fp32 value would leave its range.
+__device__ __forceinline__ float entry_gap(const RowEnd &end, float t,
+                                           float t_lq, float x) {
+  return t_lq - ((x - end.m) - t * end.ln_s);
 }
 // An entry's part of a row's loss, q times its gap.  A class at -inf under an
 // entry that counts (e^y > 0) makes the loss infinite, also where its share

@@ -427,7 +427,8 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (counts >> i & 1)
-          l += entry_part(end, tq[i], entry_gap(end, a.t, ty[i], ln_ys, xk[i]));
+          l += entry_part(end, tq[i],
+                          entry_gap(end, a.t, ty[i] - a.t * ln_ys, xk[i]));
       for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
       if (lane == 0) p.loss[row] = bad ? nan : a.t * l;
     }
@@ -716,7 +717,8 @@ __global__ void __launch_bounds__(NT) k_stream(StreamArgs p) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (tq[i] > 0.0f)
-        l += entry_part(end, tq[i] / ys, entry_gap(end, a.t, ty[i], ln_ys, xk[i]));
+        l += entry_part(end, tq[i] / ys,
+                        entry_gap(end, a.t, ty[i] - a.t * ln_ys, xk[i]));
     for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
     if (lane == 0) p.loss[row] = end.bad ? nan : a.t * l;
     if constexpr (kGrad) {
