@@ -111,3 +111,46 @@ def test_leaves_that_require_a_gradient_are_not_written():
         leaf = values.clone().requires_grad_()
         made = leaf * 1  # no leaf: in place as before
         assert torch.equal(write(made, made).detach(), want)
+
+
+def _device_us(call):
+    """Device time of a call, the best of several replays of a graph of them."""
+    import torch
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(5):
+            call()
+    best = np.inf
+    for _ in range(8):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        graph.replay()
+        b.record()
+        b.synchronize()
+        best = min(best, a.elapsed_time(b) * 1e3 / 5)
+    return best
+
+
+@pytest.mark.parametrize("n,V,k", [(1024, 65536, 64), (64, 131072, 20),
+                                   (2000, 5000, 20), (4096, 600, 64)])
+def test_a_constant_added_to_the_logits(n, V, k):
+    """softmax does not see a constant added to fp32 logits: the alternatives are
+    those of the shifted values, and are found in about the same time (a bound
+    with 8 bits of a logit's fraction took 4 to 7 times as long)."""
+    import torch
+    import tmnn_b200 as t
+    g = torch.Generator(device="cuda").manual_seed(V)
+    x = torch.randn(n, V, device="cuda", generator=g) * 2.5
+    far = x + 30000.0  # a step of 2^-9
+    near = far - 30000.0  # exact: the same order and the same ties
+    a, b = (t.token_logprobs(v, top_k=k) for v in (near, far))
+    assert torch.equal(a.top_ids, b.top_ids)
+    # each is off by the reference's bound of a log probability: V / 256 + 80
+    # additions, differences d of at most 30, ln s of at most 20
+    tol = 2 * 1.1 * ref.U * (3 * 30 + ref.chain(V) + 4 + 3 * 30 + 4 * 20)
+    assert (a.top_logprobs - b.top_logprobs).abs().max() <= tol
+    plain = _device_us(lambda: t.token_logprobs(near, top_k=k))
+    shifted = _device_us(lambda: t.token_logprobs(far, top_k=k))
+    assert shifted <= 2.5 * plain + 2, (shifted, plain)

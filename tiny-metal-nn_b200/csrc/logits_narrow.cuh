@@ -606,24 +606,36 @@ __global__ void __launch_bounds__(128) k_narrow(NarrowArgs p) {
       t.add(q[j]);
       best[j] = none ? -kInf : t.get();
     }
-    // A value (16 bits of it) that K granules of the row reach is a lower bound
-    // of its K-th largest logit: the granules that reach it are listed, then
-    // their logits above it, which are ranked.  For a few alternatives the loop
-    // below is the shorter way.
+    // A value (16 bits of it, and more where too many reach it) that K granules of
+    // the row reach is a lower bound of its K-th largest logit: the granules that
+    // reach it are listed, then their logits above it, which are ranked.  For a
+    // few alternatives the loop below is the shorter way.
     bool open = true;  // the row's alternatives are still to be found
     if (p.cap) {
-      uint32_t o[NG], t = 0;
+      uint32_t o[NG], t = 0, have = 0;
 #pragma unroll
       for (int j = 0; j < NG; ++j) o[j] = order_of(best[j]);
-      for (uint32_t b = 1u << 31; b >= 1u << 16; b >>= 1) {
+      auto raise = [&](uint32_t up) {  // to `up`, if K granules reach it
         int c = 0;
 #pragma unroll
-        for (int j = 0; j < NG; ++j) c += o[j] >= (t | b);
+        for (int j = 0; j < NG; ++j) c += o[j] >= up;
         if (L == 32)
           c = __reduce_add_sync(~0u, c);
         else
           for (int i = 1; i < L; i *= 2) c += __shfl_xor_sync(~0u, c, i);
-        if (c >= K) t |= b;
+        if (c >= K) {
+          t = up;
+          have = c;
+        }
+      };
+      for (uint32_t b = 1u << 31; b >= 1u << 16; b >>= 1) raise(t | b);
+      if (kLastBit<T> < 1u << 16 && !__all_sync(~0u, hardly_more(have, K))) {
+        const uint32_t most = order_of(end.m);
+        raise(most);  // many equal ones
+        for (uint32_t b = 1u << 15; b >= kLastBit<T>; b >>= 1) {
+          if (__all_sync(~0u, t == most || hardly_more(have, K))) break;
+          raise(t == most ? most : t | b);
+        }
       }
       const float floor = value_of(max(t, kLowestOrder));
       // a row's part of the shared memory: granules, keys, the granules'

@@ -494,14 +494,26 @@ __device__ __forceinline__ void each_entry(const int32_t *ids, const float *qs,
     if (id[i] >= 0) put(lane + 32 * i, both[i]);
 }
 
-// A value that at least K of n <= N orders reach, and hardly more: the largest
-// one with the low 16 bits zero (all there is to a 16-bit logit), or what all n
-// have in common; the order of the lowest logit if fewer than K are logits.
-// One warp, halving from the first bit in which the orders differ.
-template <int N>
+// The last bit in which the orders of two values of T can differ and not by
+// their sign alone: 7, 10 and 23 bits of fraction.
+template <class T>
+constexpr uint32_t kLastBit = sizeof(T) == 4                   ? 1u
+                              : std::is_same<T, __half>::value ? 1u << 13
+                                                               : 1u << 16;
+// Whether a bound that `have` of the orders reach serves to find the K largest.
+__device__ __forceinline__ bool hardly_more(uint32_t have, int K) {
+  return have <= (uint32_t)(K + K / 4 + 8);
+}
+
+// A value that at least K of n <= N orders of T's reach, and hardly more: its
+// first 16 bits are searched, and the others as long as too many reach it (fp32
+// and fp16 logits that have much in common, like a large constant added to
+// all); the order of the lowest logit if fewer than K are logits.  One warp,
+// halving from the first bit in which the orders differ.
+template <class T, int N>
 __device__ __forceinline__ uint32_t reached_by(int K, const uint32_t *values,
                                                int n) {
-  uint32_t v[N / 32], hi = 0, lo = ~0u;
+  uint32_t v[N / 32], hi = 0, lo = ~0u, have = n;
 #pragma unroll
   for (int i = 0; i < N / 32; ++i) {
     const int at = (threadIdx.x & 31) + 32 * i;
@@ -513,14 +525,22 @@ __device__ __forceinline__ uint32_t reached_by(int K, const uint32_t *values,
   lo = __reduce_min_sync(~0u, lo);
   const uint32_t same = (uint32_t)__clz(hi ^ lo);  // leading bits
   uint32_t t = same == 0 ? 0 : same == 32 ? hi : hi >> (32 - same) << (32 - same);
-  if (same < 16)
-    for (uint32_t b = 1u << (31 - same); b >= 1u << 16; b >>= 1) {
-      const uint32_t up = t | b;
-      uint32_t c = 0;
+  auto raise = [&](uint32_t up) {  // to `up`, if K of them reach it
+    uint32_t c = 0;
 #pragma unroll
-      for (int i = 0; i < N / 32; ++i) c += v[i] >= up;
-      if (__reduce_add_sync(~0u, c) >= (uint32_t)K) t = up;
+    for (int i = 0; i < N / 32; ++i) c += v[i] >= up;
+    c = __reduce_add_sync(~0u, c);
+    if (c >= (uint32_t)K) {
+      t = up;
+      have = c;
     }
+  };
+  if (same < 16)
+    for (uint32_t b = 1u << (31 - same); b >= 1u << 16; b >>= 1) raise(t | b);
+  if (kLastBit<T> < 1u << 16 && same < 32)
+    for (uint32_t b = 1u << (31 - max(same, 16u));
+         b >= kLastBit<T> && !hardly_more(have, K); b >>= 1)
+      raise(t | b);
   return max(t, kLowestOrder);
 }
 

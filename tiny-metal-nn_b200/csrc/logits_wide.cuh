@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
       return;
     }
     if (warp == 0) {
-      const uint32_t t = reached_by<kMaxGroups>(K, gmax, p.l.groups);
+      const uint32_t t = reached_by<T, kMaxGroups>(K, gmax, p.l.groups);
       if (lane == 0) misc[1] = t;
     }
     __syncthreads();
@@ -782,7 +782,7 @@ __global__ void __launch_bounds__(NT) k_stream(StreamArgs p) {
       return;
     }
     if (warp == 0) {
-      const uint32_t t = reached_by<NT>(K, gmax, NT);
+      const uint32_t t = reached_by<T, NT>(K, gmax, NT);
       if (lane == 0) misc[1] = t;
     }
     __syncthreads();
