@@ -202,3 +202,20 @@ def test_guard_between_training_steps():
         loss = tr.training_step(pos, tgt)
         assert np.isfinite(loss) and tr.last_result.loss == loss
         assert not tr.last_numerics()["anomaly"] and tr.step() == 4
+
+
+@pytest.mark.parametrize("n", [2, 777, 4096])
+def test_the_tiled_family_takes_the_split_step(n):
+    """The family of large tables: distill_step is the split step there too."""
+    base.test_distill_step_is_the_split_step(16, "Tiled", n)
+
+
+def test_result_before_any_step():
+    from tmnn_b200 import _abi
+    res = _abi.StepResult()
+    with base._field(16) as tr:
+        assert _abi.lib.tmnn_cuda_distill_result(tr._handle(), C.byref(res)) == 0
+        assert res.batch_size == 0 and res.loss == 0.0
+        assert _abi.lib.tmnn_cuda_distill_result(tr._handle(), None) \
+            == _abi.ERR_INVALID_ARGUMENT
+    assert _abi.lib.tmnn_cuda_distill_result(None, C.byref(res)) == 2

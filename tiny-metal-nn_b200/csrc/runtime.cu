@@ -2307,6 +2307,7 @@ tmnn_status tmnn_cuda_distill_result(tmnn_ctx *c, tmnn_step_result *result) {
   REQUIRE_CTX(c);
   return guarded([&] {
     if (!result) throw std::invalid_argument("distill_result: null result");
+    BusyGuard g(c);
     *result = c->last_step;
   });
 }
