@@ -154,3 +154,81 @@ def test_a_constant_added_to_the_logits(n, V, k):
     plain = _device_us(lambda: t.token_logprobs(near, top_k=k))
     shifted = _device_us(lambda: t.token_logprobs(far, top_k=k))
     assert shifted <= 2.5 * plain + 2, (shifted, plain)
+
+
+@pytest.mark.parametrize("T", [1e-4, 1e4])
+@pytest.mark.parametrize("n,V", KERNELS)
+def test_first_and_last_temperature(n, V, T):
+    """The ends of the range of temperatures, where a row is one class or all
+    alike."""
+    import torch
+    import tmnn_b200 as t
+    x, xd = base.make(n, V, "f32", seed=V + 1)
+    tk, tok = base.make_tokens(n, V, V)
+    Tf = float(np.float32(T))
+    r = t.token_logprobs(x, tk, top_k=5, temperature=T, stats=True)
+    lp, H, ids, _, stats, rows = ref.token_logprobs(xd, Tf, tok, 5)
+    d = rows.d[np.arange(n), np.clip(tok, 0, V - 1)]
+    # (d is 0 in the reference where e^-d is: there the logit's own distance)
+    with np.errstate(all="ignore"):
+        far = (rows.m - xd[np.arange(n), np.clip(tok, 0, V - 1)]) / Tf
+    d = np.where(np.isfinite(far), np.maximum(d, far), d)
+    ref.assert_close(r.logprob.cpu(), lp, np.nan_to_num(
+        rows.tol_lp(d, np.where(np.isfinite(lp), lp, 0))), "logprob")
+    ref.assert_close(r.entropy.cpu(), H, np.nan_to_num(rows.tol_H), "entropy")
+    assert np.array_equal(r.top_ids.cpu().numpy(), ids)
+    one = np.ones(n, np.float32)
+    want, tol = ref.token_logprobs_backward(xd, Tf, tok, r.stats.cpu().numpy(),
+                                            one, one)
+    c = torch.ones(n, device="cuda")
+    g = t.token_logprobs_backward(x, tk, r.stats, c, c, temperature=T)
+    # an e^-d below 2^-126 may be flushed; the gradient has it times
+    # (g + h (d + ln s + H)) / T with g = h = 1, d of at most 88 there, and ln s
+    # and H of at most ln 524288 < 14
+    flushed = 2.0 ** -126 * (1 + 88 + 2 * 14) / Tf
+    ref.assert_close(g.double().cpu(), want,
+                     base._round(want, np.nan_to_num(tol) + flushed, "f32"),
+                     "backward")
+    ti, ty = base.make_teacher(n, V, min(4, V), V)
+    loss, tl, dx, td = ref.distill(xd, Tf, ti, ty.astype(np.float64), one)
+    at = np.clip(ti, 0, V - 1)
+    with np.errstate(all="ignore"):
+        # the same for an entry's class: its distance counts 3 u, times T^2 q
+        far = np.where(ti < 0, 0, rows.m[:, None] - np.take_along_axis(xd, at, 1)) / Tf
+        far = np.where(np.isfinite(far), far, 0)
+    tl = np.nan_to_num(tl) + 1.1 * Tf * Tf * 3 * ref.U * far.max(1)
+    args = (x, torch.from_numpy(ti).cuda(), torch.from_numpy(ty).cuda())
+    got, gx = t.distill_forward_backward(*args, temperature=T, row_weight=c)
+    ref.assert_close(got.cpu(), loss, tl, "loss with gradient")
+    ref.assert_close(t.distill_loss(*args, temperature=T).cpu(), loss, tl, "loss")
+    ref.assert_close(gx.double().cpu(), dx,
+                     base._round(dx, np.nan_to_num(td) + 2.0 ** -126 * Tf, "f32"),
+                     "gradient")
+
+
+def test_more_rows_than_a_launch_takes():
+    """Rows beyond 2^26 go to a second launch: each row's results are its
+    own."""
+    import torch
+    import tmnn_b200 as t
+    n, V, period = (1 << 26) + 1027, 3, 1024
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(period, V, device="cuda", generator=g).bfloat16()
+    tok = torch.randint(-1, V, (period,), device="cuda", generator=g).int()
+    y = torch.randn(period, 1, device="cuda", generator=g)
+    w = torch.rand(period, device="cuda", generator=g)
+
+    def many(a):
+        return a.repeat(n // period + 1, *[1] * (a.dim() - 1))[:n]
+
+    def run(x, tok, y, w):
+        r = t.token_logprobs(x, tok, top_k=2, stats=True)
+        d = t.token_logprobs_backward(x, tok, r.stats, w, w)
+        loss, e = t.distill_forward_backward(x, tok.view(-1, 1), y, row_weight=w)
+        return [*r, d, loss, e]
+
+    want = run(x, tok, y, w)
+    for got, few in zip(run(many(x), many(tok), many(y), many(w)), want):
+        whole = n // period * period
+        assert (got[:whole].view(-1, period, *few.shape[1:]) == few).all()
+        assert (got[whole:] == few[:n - whole]).all()
