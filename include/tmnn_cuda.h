@@ -528,7 +528,10 @@ const char *tmnn_cuda_mlp_last_error(void);
  * cudaStream_t of `device`; NULL is the device's default stream) and return
  * without waiting.  They allocate nothing and keep nothing between calls, so
  * they may be captured into graphs and run on several streams at once.
- * Arithmetic and sums are fp32.  Results are the same from run to run.
+ * Arithmetic and sums are fp32.  The same call gives the same bits from run
+ * to run.  Another number of rows, another alignment of the row or other
+ * outputs may take the sums in another order, so that a row's values differ in
+ * their last bits (its alternatives do not).
  *
  * Rows: a class at -inf has probability 0.  A row with every class at -inf
  * has no distribution: its log probabilities are -inf, its entropy and its
@@ -585,7 +588,10 @@ tmnn_status tmnn_cuda_token_logprobs_backward(
  *   loss[i] = T^2 sum_k q_k (log q_k - log p[id_k]),
  *   d_logits[i] = w_i d loss[i] / d x = w_i T (p - q),
  * w_i = row_weight[i], or 1 / rows when row_weight is NULL (the gradient of
- * the mean loss).  Entries with id < 0 or logit -inf are left out, and a row
+ * the mean loss).  The teacher's logits are divided by T here: log
+ * probabilities that stand for them are those of temperature 1, whatever T is.
+ * A class at -inf under an entry makes the loss +inf, unless the entry's
+ * exp((logit - largest) / T) is 0 in fp32, when it counts nothing.  Entries with id < 0 or logit -inf are left out, and a row
  * without entries is padding: its loss and gradient are 0.
  * Entries that name one class twice count each on its own.  An id >= classes
  * or a NaN or +inf among the entries makes the row NaN.  d_logits NULL: the
@@ -603,7 +609,9 @@ const char *tmnn_cuda_logits_last_error(void);
 /* The same on a context whose outputs are class logits (classes =
  * num_outputs).  Host arrays, or device pointers with TMNN_PTR_DEVICE, like
  * the context's other calls; they run on the context's stream and wait.
- * Pointers to another device's memory, or the host's own, are refused there.
+ * Device pointers to another device's memory, or to host memory that CUDA does
+ * not know, are refused (pinned and managed memory is read where it is), as
+ * are ids off their alignment and outputs that overlap, before any work.
  * token_logprobs: evaluate, then tmnn_cuda_token_logprobs.  Any output may be
  * NULL as above. */
 tmnn_status tmnn_cuda_ctx_token_logprobs(

@@ -1,5 +1,6 @@
-// logits_narrow.cuh -- class-logit kernels for rows of up to 2040 classes (1020
-// fp32 ones): a thread a row, and 1 to 32 lanes a row.
+// logits_narrow.cuh -- class-logit kernels for rows of up to 256 granules, which
+// is 2048 classes (1024 fp32 ones) where rows start on 16-byte boundaries and
+// 2041 (1021) elsewhere: a thread a row, and 1 to 32 lanes a row.
 #pragma once
 #include "logits_row.cuh"
 
@@ -14,9 +15,13 @@ namespace logits {
 // of quads, so that the lanes' 16-byte reads meet different banks; other rows
 // keep their distance V (odd, or twice an odd number).
 //
-// Bound by the instructions, 40 to 50 of a warp a row: 262144 rows of 64 fp32
-// logits with 4 alternatives take 21 us, 3.8 TB/s (lanes side by side: 43 us),
-// of 19 classes, distilled from 4 entries, 17 us, 3.3 TB/s (27 us).
+// 262144 rows of 64 fp32 logits with 4 alternatives take 22 us, 3.6 TB/s (lanes
+// side by side: 43 us), of 19 classes, distilled from 4 entries, 16.7 us, 3.0
+// TB/s (27 us).  Their 55 and 45 instructions of a warp a row would be 12 and 10
+// us of all issue slots, of which half are used: a warp loads, computes and
+// stores its 32 rows one after the other, and the images leave room for 24 and
+// 40 of 64 warps on an SM (a third and half of them active over the kernel), too
+// few to cover each other's waits.
 constexpr int kTinyClasses = 128;
 
 struct TinyArgs {
@@ -404,8 +409,8 @@ __global__ void __launch_bounds__(128) k_tiny(TinyArgs p) {
 // There is no shared memory but for a teacher's entries and the listed
 // alternatives, and nothing is read or written twice.
 //
-// 65536 rows of 1000 bf16 logits: backward 52 us, 5.1 TB/s; distilled from 10
-// entries 87 us; with 10 alternatives 95 us, bound by the instructions (1440 of
+// 65536 rows of 1000 bf16 logits: backward 53 us, 4.9 TB/s; distilled from 10
+// entries 90 us; with 10 alternatives 96 us, bound by the instructions (1440 of
 // a warp a row; 193 us with one search through the row an alternative).  Two
 // granules more a lane than 8 cost more registers than they save (rows of 4039
 // fp16 logits: 190 us, streamed 144).

@@ -15,8 +15,8 @@ namespace logits {
 // itself: the row once in, results or gradient once out.
 //
 // For a gradient three slabs of 64 KB lie on an SM (two load while one
-// computes): 3687 rows of 131072 bf16 logits, in clusters of four, take 410 us,
-// 5.0 TB/s.  What bounds it is a CTA's life, not the memory: load, exchange and
+// computes): 4096 rows of 131072 bf16 logits, 409 of them padding (zeros, not
+// read), in clusters of four, take 413 us for 2.04 GB, 4.9 TB/s.  What bounds it is a CTA's life, not the memory: load, exchange and
 // two bursts of ex2 one after the other (without any ex2 it is 378 us, rows of
 // one CTA each 345).  Measured and not kept: slabs of 32 KB (the same with 128
 // threads), one CTA an SM that takes row after row and copies the next into
@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
   int32_t *sid = reinterpret_cast<int32_t *>(sq + p.te.k);
   [[maybe_unused]] int32_t *bad_entries = sid + p.te.k;
   [[maybe_unused]] float ty[4], tq[4], ln_ys = 0.0f, ym = 0.0f;
-  [[maybe_unused]] int32_t tid_[4], counts = 0;
+  [[maybe_unused]] int32_t tid_[4], counted = 0;  // entries with e^y > 0
   bool idle;
   if constexpr (kReads) {
     if (p.tokens) tok = load_index(p.tokens, row, p.itype);
@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
         ty[i] = tid_[i] >= 0 ? ty[i] - ym : -kInf;
         tq[i] = expf(ty[i] * a.inv_t);
         ys += tq[i];
-        counts |= (tq[i] > 0.0f) << i;
+        counted |= (tq[i] > 0.0f) << i;
         if (leader && tid_[i] >= 0) xk[i] = to_f((x - first)[tid_[i]]);
       }
       for (int o = 16; o; o >>= 1) ys += __shfl_xor_sync(~0u, ys, o);
@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
       float l = 0.0f;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (counts >> i & 1)
+        if (counted >> i & 1)
           l += entry_part(end, tq[i],
                           entry_gap(end, a.t, ty[i] - a.t * ln_ys, xk[i]));
       for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
@@ -487,11 +487,14 @@ __global__ void __launch_bounds__(NT) k_team(TeamArgs p) {
 // the row again.  Without alternatives the next four granules are on their way
 // while four are worked on; with them (more registers) more CTAs do as well.
 //
-// Bound by the memory: 3687 rows of 131072 bf16 logits take 155 us, 6.2 TB/s
-// (162 without the loads ahead, 170 with eight granules at a time).  One ex2 a
+// Bound by the memory: 3687 rows of 131072 bf16 logits take 142 us in a row of
+// calls, 6.8 TB/s, and 159 us each by itself (162 for 155 without the loads
+// ahead, 170 with eight granules at a time, when measured side by side).  One ex2 a
 // logit keeps the special-function unit busy for two thirds of that time.
 // With alternatives, 2048 rows and 64 of them: 110 us, 82 without; the search
-// after a row's end is what is left over.
+// after a row's end is what is left over.  Rows whose bound many equal logits
+// reach are read again for each halving of the keys' interval: 1024 rows of
+// 131072 equal bf16 logits take 3.2 ms with 64 alternatives, 65 us without ties.
 //
 // For the alternatives each thread notes the maximum of every run of granules
 // it read.  The K-th largest of the threads' maxima is a lower bound of the

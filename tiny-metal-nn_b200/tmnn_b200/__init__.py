@@ -619,7 +619,8 @@ class Trainer:
         (classes = n_output): forward, loss with its gradient, backward, Adam;
         returns the mean loss.  teacher_ids [batch, k] (int32 or int64, below
         0: no entry) and float32 teacher_logits [batch, k] are a teacher's top
-        classes of each point, e.g. what token_logprobs(top_k=k) returns.
+        classes of each point, e.g. what token_logprobs(top_k=k) returns at
+        temperature 1 (the temperature here divides the teacher's as well).
         Host arrays or CUDA tensors, all alike.
 
         The numerics guard takes part as in training_step: a point with an id

@@ -176,8 +176,9 @@ def token_logprobs_backward(logits, tokens, stats, d_logprob=None,
     sum(d_logprob * logprob) + sum(d_entropy * entropy), from the arguments of
     a token_logprobs(..., stats=True) call and its stats.  Either of the
     incoming gradients (float32 [n]) may be None.  out: where to write it; it
-    may be `logits` itself, whose values are then lost.  The alternatives'
-    log probabilities carry no gradient."""
+    may be `logits` itself, whose values are then lost, but no leaf that
+    requires a gradient.  The alternatives' log probabilities carry no
+    gradient."""
     x = _logits(logits, temperature)
     n, dev = x.rows, logits.device
     tp, it = (None, 0) if tokens is None else _vector(tokens, "tokens", dev,
@@ -223,7 +224,8 @@ def distill_loss(logits, teacher_ids, teacher_logits, *, temperature=1.0):
     teacher_ids names, and p = softmax(logits / T) over all classes.
     teacher_ids [n, k] int32 or int64 (below 0: no entry; a row without
     entries is padding with loss 0), teacher_logits [n, k] float32, float16 or
-    bfloat16 -- the top_ids and top_logprobs of token_logprobs fit both."""
+    bfloat16 -- the top_ids and top_logprobs of token_logprobs at temperature 1
+    fit both (the temperature here divides them, too)."""
     return _distill(_logits(logits, temperature), logits, teacher_ids,
                     teacher_logits, None, None)
 
@@ -233,7 +235,8 @@ def distill_forward_backward(logits, teacher_ids, teacher_logits, *,
     """(loss [n], d_logits [n, classes]): distill_loss and, from the same read
     of the logits, the gradient of sum(row_weight * loss) in the logits' type.
     row_weight float32 [n]; None is 1 / n, the gradient of the mean loss.  out:
-    where to write the gradient; it may be `logits` itself."""
+    where to write the gradient; it may be `logits` itself, but no leaf that
+    requires a gradient."""
     x = _logits(logits, temperature)
     given, out = out, _gradient(out, logits)
     loss = _distill(x, logits, teacher_ids, teacher_logits, row_weight, out)
